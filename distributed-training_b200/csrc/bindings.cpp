@@ -46,6 +46,21 @@ void scale_f32(torch::Tensor x, double s);
 std::vector<torch::Tensor> attn_fwd(torch::Tensor qkv, int64_t B, int64_t T, int64_t H, int64_t D, bool legacy);
 torch::Tensor attn_bwd(torch::Tensor qkv, torch::Tensor out, torch::Tensor dout, torch::Tensor lse, int64_t B,
                        int64_t T, int64_t H, int64_t D, bool legacy);
+// route.cu
+std::vector<torch::Tensor> route_fwd(torch::Tensor logits, int64_t k, bool softmax, c10::optional<torch::Tensor> bias,
+                                     int64_t groups, int64_t keep, int64_t top, bool renorm, double scale);
+torch::Tensor route_bwd(torch::Tensor logits, torch::Tensor gates, torch::Tensor idx, torch::Tensor dgates,
+                        bool softmax, bool renorm, double scale);
+// moe.cu
+std::vector<torch::Tensor> experts_fwd(torch::Tensor x, torch::Tensor w1, c10::optional<torch::Tensor> b1,
+                                       torch::Tensor w2, c10::optional<torch::Tensor> b2, torch::Tensor idx,
+                                       torch::Tensor gates, bool save);
+std::vector<torch::Tensor> experts_bwd(torch::Tensor dy, torch::Tensor x, torch::Tensor w1, torch::Tensor w2,
+                                       torch::Tensor gates, std::vector<torch::Tensor> saved, torch::Tensor dw1,
+                                       c10::optional<torch::Tensor> db1, torch::Tensor dw2,
+                                       c10::optional<torch::Tensor> db2);
+// clip.cu
+torch::Tensor clip_grads(std::vector<torch::Tensor> in, std::vector<torch::Tensor> out, double max_norm);
 // comm.cu
 std::tuple<int64_t, torch::Tensor> symm_alloc(int64_t nbytes);
 int64_t symm_open(torch::Tensor handle);
@@ -106,11 +121,12 @@ int status_optim();
 int status_attention();
 int status_comm();
 int status_attention_tc();
+int status_moe();
 
 // First non-zero device status word over all kernel files (and clears them).
 int64_t device_status() {
   int codes[] = {status_gemm(), status_layernorm(), status_embed_xent(), status_optim(), status_attention(),
-                 status_comm(), status_attention_tc()};
+                 status_comm(), status_attention_tc(), status_moe()};
   for (int c : codes)
     if (c) return c;
   return 0;
@@ -151,6 +167,14 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
         py::arg("legacy") = false);
   m.def("attn_bwd", &attn_bwd, py::arg("qkv"), py::arg("out"), py::arg("dout"), py::arg("lse"), py::arg("B"),
         py::arg("T"), py::arg("H"), py::arg("D"), py::arg("legacy") = false);
+  m.def("route_fwd", &route_fwd, py::arg("logits"), py::arg("k"), py::arg("softmax"), py::arg("bias"),
+        py::arg("groups"), py::arg("keep"), py::arg("top"), py::arg("renorm"), py::arg("scale"));
+  m.def("route_bwd", &route_bwd);
+  m.def("experts_fwd", &experts_fwd, py::arg("x"), py::arg("w1"), py::arg("b1"), py::arg("w2"), py::arg("b2"),
+        py::arg("idx"), py::arg("gates"), py::arg("save"));
+  m.def("experts_bwd", &experts_bwd, py::arg("dy"), py::arg("x"), py::arg("w1"), py::arg("w2"), py::arg("gates"),
+        py::arg("saved"), py::arg("dw1"), py::arg("db1"), py::arg("dw2"), py::arg("db2"));
+  m.def("clip_grads", &clip_grads);
   m.def("symm_alloc", &symm_alloc);
   m.def("symm_open", &symm_open);
   m.def("symm_close", &symm_close);

@@ -1,0 +1,524 @@
+// Global gradient norm over many tensors, and clipping, in two launches.
+//
+//   norm = sqrt(sum over tensors and elements of g^2)
+//   f = 1 if norm <= max_norm (or norm is 0), else max_norm / (norm + 1e-6)
+//   out = g * f                       in place, or into tensors of another type
+//
+// The factor is the one of dtrain/optim.py:49-52; csrc/optim.cu applies it to one flat
+// fp32 buffer, this file to a list of tensors of any sizes, types and layouts (a
+// mixture of experts' parameters, bf16 gradients bound for the flat fp32 buffer).
+//
+// The list travels in the kernels' parameters (32 bytes a tensor, up to 960 tensors a
+// launch), so there is no copy to the device and the calls can be captured in a CUDA
+// graph.  Each CTA of the first kernel sums its chunks in a fixed order into one fp64
+// partial; each CTA of the second adds the partials up in the same order, so every CTA
+// gets the same factor, and the result does not depend on scheduling.
+#include <ATen/core/Tensor.h>
+#include <ATen/ops/empty.h>
+#include <ATen/MemoryOverlap.h>
+#include <ATen/cuda/CUDAContext.h>
+#include <c10/cuda/CUDAGuard.h>
+#include <cuda_fp16.h>
+
+#include <algorithm>
+
+#include "common.cuh"
+
+namespace dtb {
+
+constexpr int kClipThreads = 256;
+constexpr int kClipChunk = 8192;     // elements of a tensor that a CTA takes at a time
+constexpr int kClipGrid = 148 * 4;   // most CTAs of a launch: fixed, so the order of the sums is too
+constexpr int kClipStridedMax = 128;
+
+enum ClipType : int { CLIP_F32 = 0, CLIP_BF16 = 1, CLIP_F16 = 2 };
+
+struct ClipDesc {
+  const void* in;
+  void* out;   // null: the norm only
+  long n;
+  int first;   // chunks of the tensors before this one
+  short in_t, out_t;
+};
+template <int CAP>
+struct ClipList {
+  int count, chunks;
+  ClipDesc d[CAP];
+};
+// A tensor that is not dense, or whose output has another order of its elements.
+struct ClipStrided {
+  const void* in;
+  void* out;
+  long n;
+  int size[4];
+  long is[4], os[4];
+  short in_t, out_t;
+};
+struct ClipStridedList {
+  int count;
+  ClipStrided d[kClipStridedMax];
+};
+
+__device__ __forceinline__ float clip_load(const void* p, int t, long i) {
+  if (t == CLIP_F32) return reinterpret_cast<const float*>(p)[i];
+  if (t == CLIP_BF16) return bf2f(reinterpret_cast<const bf16*>(p)[i]);
+  return __half2float(reinterpret_cast<const __half*>(p)[i]);
+}
+__device__ __forceinline__ void clip_store(void* p, int t, long i, float v) {
+  if (t == CLIP_F32) reinterpret_cast<float*>(p)[i] = v;
+  else if (t == CLIP_BF16) reinterpret_cast<bf16*>(p)[i] = f2bf(v);
+  else reinterpret_cast<__half*>(p)[i] = __float2half_rn(v);
+}
+
+// The values of one 16-byte load: 4 fp32, or 8 of 16 bits.
+template <int T>
+struct ClipVec;
+template <>
+struct ClipVec<CLIP_F32> {
+  static constexpr int N = 4;
+  static constexpr unsigned kMask = 0x7fffffffu;
+  static __device__ __forceinline__ void get(const uint4& u, float* v) {
+    v[0] = __uint_as_float(u.x);
+    v[1] = __uint_as_float(u.y);
+    v[2] = __uint_as_float(u.z);
+    v[3] = __uint_as_float(u.w);
+  }
+};
+template <>
+struct ClipVec<CLIP_BF16> {
+  static constexpr int N = 8;
+  static constexpr unsigned kMask = 0x7fff7fffu;
+  static __device__ __forceinline__ void get(const uint4& u, float* v) {
+    const unsigned w[4] = {u.x, u.y, u.z, u.w};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      v[2 * i] = __uint_as_float(w[i] << 16);
+      v[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
+    }
+  }
+};
+template <>
+struct ClipVec<CLIP_F16> {
+  static constexpr int N = 8;
+  static constexpr unsigned kMask = 0x7fff7fffu;
+  static __device__ __forceinline__ void get(const uint4& u, float* v) {
+    const __half2* h = reinterpret_cast<const __half2*>(&u);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const float2 f = __half22float2(h[i]);
+      v[2 * i] = f.x;
+      v[2 * i + 1] = f.y;
+    }
+  }
+};
+
+// Sum of the squares of one 16-byte load: in fp32, added to an fp64 total by the caller.
+// Where fp32 squares would overflow or vanish (the values are not zero), in fp64.
+template <int T>
+__device__ __forceinline__ double clip_squares(const uint4& u) {
+  float v[ClipVec<T>::N];
+  ClipVec<T>::get(u, v);
+  float s = 0.f;
+#pragma unroll
+  for (int i = 0; i < ClipVec<T>::N; ++i) s = fmaf(v[i], v[i], s);
+  if (!(s <= 1e38f) || (s < 1e-30f && ((u.x | u.y | u.z | u.w) & ClipVec<T>::kMask))) {
+    double d = 0.0;
+#pragma unroll
+    for (int i = 0; i < ClipVec<T>::N; ++i) d += (double)v[i] * (double)v[i];
+    return d;
+  }
+  return (double)s;
+}
+
+template <class List>
+__device__ __forceinline__ int clip_find(const List& l, int chunk) {
+  int lo = 0, hi = l.count - 1;
+  while (lo < hi) {
+    const int mid = (lo + hi + 1) >> 1;
+    if (l.d[mid].first <= chunk) lo = mid;
+    else hi = mid - 1;
+  }
+  return lo;
+}
+
+// [lo, hi) elements of the chunk, and the head: elements before the first 16-byte boundary.
+struct ClipSpan {
+  long lo;
+  int head, vecs, len;
+};
+template <int T>
+__device__ __forceinline__ ClipSpan clip_span(const ClipDesc& d, int chunk) {
+  constexpr int N = ClipVec<T>::N, S = 16 / N;
+  ClipSpan s;
+  s.lo = (long)(chunk - d.first) * kClipChunk;
+  s.len = (int)min((long)kClipChunk, d.n - s.lo);
+  const unsigned off = (unsigned)((reinterpret_cast<uintptr_t>(d.in) + s.lo * S) & 15);
+  s.head = min(s.len, off ? (int)(16 - off) / S : 0);
+  s.vecs = (s.len - s.head) / N;
+  return s;
+}
+
+template <int T>
+__device__ __forceinline__ double clip_chunk_squares(const ClipDesc& d, int chunk) {
+  constexpr int N = ClipVec<T>::N, S = 16 / N;
+  const ClipSpan s = clip_span<T>(d, chunk);
+  const char* base = reinterpret_cast<const char*>(d.in) + s.lo * S;
+  double acc = 0.0;
+  const uint4* p = reinterpret_cast<const uint4*>(base + s.head * S);
+  constexpr int U = 4;
+  int i = threadIdx.x;
+  for (; i + (U - 1) * kClipThreads < s.vecs; i += U * kClipThreads) {
+    uint4 u[U];
+#pragma unroll
+    for (int j = 0; j < U; ++j) u[j] = __ldg(p + i + j * kClipThreads);
+#pragma unroll
+    for (int j = 0; j < U; ++j) acc += clip_squares<T>(u[j]);
+  }
+  for (; i < s.vecs; i += kClipThreads) acc += clip_squares<T>(__ldg(p + i));
+  for (int e = threadIdx.x; e < s.len - s.vecs * N; e += kClipThreads) {
+    const double x = (double)clip_load(base, T, e < s.head ? e : e + s.vecs * N);
+    acc += x * x;
+  }
+  return acc;
+}
+
+// Sum over the CTA in a fixed order; every thread gets it.
+__device__ __forceinline__ double clip_block_sum(double v) {
+  __shared__ double sm[kClipThreads / 32];
+#pragma unroll
+  for (int o = 16; o; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+  if ((threadIdx.x & 31) == 0) sm[threadIdx.x >> 5] = v;
+  __syncthreads();
+  double s = 0.0;
+#pragma unroll
+  for (int w = 0; w < kClipThreads / 32; ++w) s += sm[w];
+  __syncthreads();
+  return s;
+}
+
+template <int CAP>
+__global__ void __launch_bounds__(kClipThreads)
+    clip_norm_kernel(const __grid_constant__ ClipList<CAP> l, double* __restrict__ part) {
+  double acc = 0.0;
+  for (int c = blockIdx.x; c < l.chunks; c += gridDim.x) {
+    const ClipDesc& d = l.d[clip_find(l, c)];
+    if (d.in_t == CLIP_F32) acc += clip_chunk_squares<CLIP_F32>(d, c);
+    else if (d.in_t == CLIP_BF16) acc += clip_chunk_squares<CLIP_BF16>(d, c);
+    else acc += clip_chunk_squares<CLIP_F16>(d, c);
+  }
+  acc = clip_block_sum(acc);
+  if (threadIdx.x == 0) part[blockIdx.x] = acc;
+}
+
+__device__ __forceinline__ long clip_offset(const int* size, const long* st, long i) {
+  long o = 0;
+#pragma unroll
+  for (int k = 3; k >= 0; --k) {
+    o += (i % size[k]) * st[k];
+    i /= size[k];
+  }
+  return o;
+}
+
+__global__ void __launch_bounds__(kClipThreads)
+    clip_norm_strided_kernel(const __grid_constant__ ClipStridedList l, double* __restrict__ part) {
+  double acc = 0.0;
+  for (int t = 0; t < l.count; ++t) {
+    const ClipStrided& d = l.d[t];
+    for (long i = (long)blockIdx.x * kClipThreads + threadIdx.x; i < d.n; i += (long)gridDim.x * kClipThreads) {
+      const double x = (double)clip_load(d.in, d.in_t, clip_offset(d.size, d.is, i));
+      acc += x * x;
+    }
+  }
+  acc = clip_block_sum(acc);
+  if (threadIdx.x == 0) part[blockIdx.x] = acc;
+}
+
+// The factor from the partials; CTA 0 of the launch that has `norm` writes it.
+__device__ __forceinline__ float clip_total(const double* part, int np, float max_norm, float* norm) {
+  double s = 0.0;
+  for (int i = threadIdx.x; i < np; i += kClipThreads) s += __ldcg(part + i);
+  const double n = sqrt(clip_block_sum(s));
+  if (norm && blockIdx.x == 0 && threadIdx.x == 0) *norm = (float)n;
+  if (n <= (double)max_norm || n == 0.0) return 1.f;
+  return (float)((double)max_norm / (n + 1e-6));
+}
+
+template <int T>
+__device__ __forceinline__ void clip_store_vec(void* out, long i, const float* v);
+template <>
+__device__ __forceinline__ void clip_store_vec<CLIP_F32>(void* out, long i, const float* v) {
+  *reinterpret_cast<float4*>(reinterpret_cast<float*>(out) + i) = make_float4(v[0], v[1], v[2], v[3]);
+}
+template <>
+__device__ __forceinline__ void clip_store_vec<CLIP_BF16>(void* out, long i, const float* v) {
+  *reinterpret_cast<uint2*>(reinterpret_cast<bf16*>(out) + i) =
+      make_uint2(pack_bf16x2(v[0], v[1]), pack_bf16x2(v[2], v[3]));
+}
+template <>
+__device__ __forceinline__ void clip_store_vec<CLIP_F16>(void* out, long i, const float* v) {
+  const __half2 a = __floats2half2_rn(v[0], v[1]), b = __floats2half2_rn(v[2], v[3]);
+  *reinterpret_cast<uint2*>(reinterpret_cast<__half*>(out) + i) =
+      make_uint2(*reinterpret_cast<const unsigned*>(&a), *reinterpret_cast<const unsigned*>(&b));
+}
+
+template <int T, int TO>
+__device__ __forceinline__ void clip_chunk_scale(const ClipDesc& d, int chunk, float f) {
+  constexpr int N = ClipVec<T>::N, S = 16 / N, SO = TO == CLIP_F32 ? 4 : 2;
+  const ClipSpan s = clip_span<T>(d, chunk);
+  const char* base = reinterpret_cast<const char*>(d.in) + s.lo * S;
+  char* out = reinterpret_cast<char*>(d.out) + s.lo * SO;
+  const uint4* p = reinterpret_cast<const uint4*>(base + s.head * S);
+  char* o = out + s.head * SO;
+  const bool wide = (reinterpret_cast<uintptr_t>(o) & (4 * SO - 1)) == 0;  // four outputs at a time
+  for (int i = threadIdx.x; i < s.vecs; i += kClipThreads) {
+    float v[N];
+    ClipVec<T>::get(p[i], v);
+#pragma unroll
+    for (int j = 0; j < N; ++j) v[j] *= f;
+    if (wide) {
+#pragma unroll
+      for (int j = 0; j < N; j += 4) clip_store_vec<TO>(o, (long)i * N + j, v + j);
+    } else {
+#pragma unroll
+      for (int j = 0; j < N; ++j) clip_store(o, TO, (long)i * N + j, v[j]);
+    }
+  }
+  for (int e = threadIdx.x; e < s.len - s.vecs * N; e += kClipThreads) {
+    const int at = e < s.head ? e : e + s.vecs * N;
+    clip_store(out, TO, at, clip_load(base, T, at) * f);
+  }
+}
+
+template <int T>
+__device__ __forceinline__ void clip_chunk_scale_to(const ClipDesc& d, int chunk, float f) {
+  if (d.out_t == CLIP_F32) clip_chunk_scale<T, CLIP_F32>(d, chunk, f);
+  else if (d.out_t == CLIP_BF16) clip_chunk_scale<T, CLIP_BF16>(d, chunk, f);
+  else clip_chunk_scale<T, CLIP_F16>(d, chunk, f);
+}
+
+template <int CAP>
+__global__ void __launch_bounds__(kClipThreads)
+    clip_scale_kernel(const __grid_constant__ ClipList<CAP> l, const double* __restrict__ part, int np, float max_norm,
+                      float* norm) {
+  const float f = clip_total(part, np, max_norm, norm);
+  for (int c = blockIdx.x; c < l.chunks; c += gridDim.x) {
+    const ClipDesc& d = l.d[clip_find(l, c)];
+    if (d.out == nullptr || (f == 1.f && d.in == d.out)) continue;
+    if (d.in_t == CLIP_F32) clip_chunk_scale_to<CLIP_F32>(d, c, f);
+    else if (d.in_t == CLIP_BF16) clip_chunk_scale_to<CLIP_BF16>(d, c, f);
+    else clip_chunk_scale_to<CLIP_F16>(d, c, f);
+  }
+}
+
+__global__ void __launch_bounds__(kClipThreads)
+    clip_scale_strided_kernel(const __grid_constant__ ClipStridedList l, const double* __restrict__ part, int np,
+                              float max_norm) {
+  const float f = clip_total(part, np, max_norm, nullptr);
+  for (int t = 0; t < l.count; ++t) {
+    const ClipStrided& d = l.d[t];
+    if (f == 1.f && d.in == d.out) continue;
+    for (long i = (long)blockIdx.x * kClipThreads + threadIdx.x; i < d.n; i += (long)gridDim.x * kClipThreads)
+      clip_store(d.out, d.out_t, clip_offset(d.size, d.os, i),
+                 clip_load(d.in, d.in_t, clip_offset(d.size, d.is, i)) * f);
+  }
+}
+
+__global__ void __launch_bounds__(kClipThreads)
+    clip_finish_kernel(const double* __restrict__ part, int np, float* norm) {
+  clip_total(part, np, 0.f, norm);
+}
+
+// ------------------------------------------------------------------ host
+static short clip_type(const at::Tensor& t) {
+  switch (t.scalar_type()) {
+    case at::kFloat: return CLIP_F32;
+    case at::kBFloat16: return CLIP_BF16;
+    case at::kHalf: return CLIP_F16;
+    default: TORCH_CHECK(false, "clip_grads: fp32, bf16 or fp16 tensors expected, got ", t.scalar_type());
+  }
+}
+
+static bool same_order(const at::Tensor& a, const at::Tensor& b) {
+  for (int64_t k = 0; k < a.dim(); ++k)
+    if (a.size(k) != 1 && a.stride(k) != b.stride(k)) return false;
+  return true;
+}
+
+// Common dimensions of `a` and `b`, merged where both allow it; at most four are left.
+static ClipStrided strided_desc(const at::Tensor& a, const at::Tensor* b) {
+  ClipStrided d{};
+  int nd = 0;
+  for (int64_t k = 0; k < a.dim(); ++k) {
+    const long sz = a.size(k), sa = a.stride(k), sb = b ? b->stride(k) : 0;
+    if (sz == 1) continue;
+    if (nd && d.is[nd - 1] == sa * sz && (!b || d.os[nd - 1] == sb * sz) && (long)d.size[nd - 1] * sz < (1L << 31)) {
+      d.size[nd - 1] *= (int)sz;
+      d.is[nd - 1] = sa;
+      d.os[nd - 1] = sb;
+      continue;
+    }
+    TORCH_CHECK(nd < 4, "clip_grads: a strided tensor of more than four dimensions that cannot be merged");
+    TORCH_CHECK(sz < (1L << 31), "clip_grads: a strided tensor with a dimension over 2^31");
+    d.size[nd] = (int)sz;
+    d.is[nd] = sa;
+    d.os[nd] = sb;
+    ++nd;
+  }
+  for (int k = 3; k >= 0; --k) {  // the dimensions sit at the end
+    const int from = k - (4 - nd);
+    d.size[k] = from >= 0 ? d.size[from] : 1;
+    d.is[k] = from >= 0 ? d.is[from] : 0;
+    d.os[k] = from >= 0 ? d.os[from] : 0;
+  }
+  d.in = a.data_ptr();
+  d.n = a.numel();
+  d.in_t = clip_type(a);
+  if (b) {
+    d.out = b->data_ptr();
+    d.out_t = clip_type(*b);
+  }
+  return d;
+}
+
+struct ClipRange {
+  uintptr_t lo, hi;
+  int i;
+  bool out;
+};
+
+// Outputs must not overlap one another, nor another tensor's input.
+static void check_ranges(std::vector<ClipRange>& r) {
+  const auto less = [](const ClipRange& a, const ClipRange& b) { return a.lo < b.lo; };
+  if (!std::is_sorted(r.begin(), r.end(), less)) std::sort(r.begin(), r.end(), less);
+  uintptr_t out_hi = 0, any_hi = 0;
+  int out_i = -1, any_i = -1;
+  for (const auto& x : r) {
+    TORCH_CHECK(!(x.lo < out_hi && out_i != x.i), "clip_grads: tensors ", out_i, " and ", x.i, " overlap in memory");
+    TORCH_CHECK(!(x.out && x.lo < any_hi && any_i != x.i), "clip_grads: tensors ", any_i, " and ", x.i,
+                " overlap in memory");
+    if (x.out && x.hi > out_hi) { out_hi = x.hi; out_i = x.i; }
+    if (x.hi > any_hi) { any_hi = x.hi; any_i = x.i; }
+  }
+}
+
+template <int CAP>
+static void launch_lists(const std::vector<ClipDesc>& all, size_t at, size_t count, int grid, bool scale, double* part,
+                         int np, float max_norm, float* norm, cudaStream_t st) {
+  ClipList<CAP> l;
+  l.count = (int)count;
+  l.chunks = 0;
+  for (size_t k = 0; k < count; ++k) {
+    l.d[k] = all[at + k];
+    l.d[k].first = l.chunks;
+    l.chunks += (int)((l.d[k].n + kClipChunk - 1) / kClipChunk);
+  }
+  if (scale) clip_scale_kernel<CAP><<<grid, kClipThreads, 0, st>>>(l, part, np, max_norm, norm);
+  else clip_norm_kernel<CAP><<<grid, kClipThreads, 0, st>>>(l, part);
+  count_launch();
+  C10_CUDA_KERNEL_LAUNCH_CHECK();
+}
+
+// The norm (fp32 scalar) of the tensors `in` together; with `out` (as many tensors, of the
+// same shapes) also out[i] = in[i] * factor.  out[i] may be in[i].
+at::Tensor clip_grads(std::vector<at::Tensor> in, std::vector<at::Tensor> out, double max_norm) {
+  TORCH_CHECK(!in.empty(), "clip_grads: an empty list has no device");
+  TORCH_CHECK(out.empty() || out.size() == in.size(), "clip_grads: ", in.size(), " gradients but ", out.size(), " outputs");
+  TORCH_CHECK(max_norm >= 0.0, "clip_grads: max_norm must not be negative");
+  const auto dev = in[0].device();
+  TORCH_CHECK(dev.is_cuda(), "clip_grads: CUDA tensors expected");
+  c10::cuda::CUDAGuard guard(dev);
+  std::vector<ClipDesc> dense;
+  std::vector<ClipStrided> strided;
+  std::vector<ClipRange> ranges;
+  dense.reserve(in.size());
+  ranges.reserve(out.empty() ? 0 : 2 * in.size());
+  for (size_t i = 0; i < in.size(); ++i) {
+    const at::Tensor& a = in[i];
+    const at::Tensor* b = out.empty() ? nullptr : &out[i];
+    TORCH_CHECK(a.device() == dev && (!b || b->device() == dev), "clip_grads: tensor ", i, " is on another device");
+    const short ta = clip_type(a), tb = b ? clip_type(*b) : 0;
+    TORCH_CHECK(!b || b->sizes() == a.sizes(), "clip_grads: output ", i, " has another shape than its gradient");
+    if (a.numel() == 0) continue;
+    const bool same = b && b->data_ptr() == a.data_ptr();
+    TORCH_CHECK(!same || (ta == tb && same_order(a, *b)), "clip_grads: output ", i, " overlays its gradient differently");
+    const bool flat = a.is_non_overlapping_and_dense() &&
+                      (!b || same || (b->is_non_overlapping_and_dense() && same_order(a, *b)));
+    if (b) {
+      TORCH_CHECK(at::has_internal_overlap(*b) != at::MemOverlap::Yes, "clip_grads: output ", i, " overlaps itself");
+      const auto range = [&](const at::Tensor& t, bool o) {
+        long last = 0;
+        for (int64_t k = 0; k < t.dim(); ++k) last += (t.size(k) - 1) * t.stride(k);
+        const uintptr_t lo = reinterpret_cast<uintptr_t>(t.data_ptr());
+        ranges.push_back({lo, lo + (last + 1) * t.element_size(), (int)i, o});
+      };
+      if (flat || b->is_non_overlapping_and_dense()) {
+        if (!same) range(a, false);
+        range(*b, true);
+      }
+    }
+    if (flat)
+      dense.push_back({a.data_ptr(), b ? b->data_ptr() : nullptr, (long)a.numel(), 0, ta, tb});
+    else
+      strided.push_back(strided_desc(a, b));
+  }
+  check_ranges(ranges);
+
+  // launches: lists of at most 960 tensors, each with a grid fixed by its number of chunks
+  struct Part { size_t at, count; int grid; };
+  std::vector<Part> parts;
+  int np = 0;
+  for (size_t at = 0; at < dense.size();) {
+    Part p{at, 0, 0};
+    long chunks = 0;
+    while (at < dense.size() && p.count < 960) {
+      const long c = (dense[at].n + kClipChunk - 1) / kClipChunk;
+      if (p.count && chunks + c >= (1L << 31)) break;
+      chunks += c;
+      ++p.count;
+      ++at;
+    }
+    TORCH_CHECK(chunks < (1L << 31), "clip_grads: a tensor of over 2^43 elements");
+    p.grid = (int)std::min<long>(chunks, kClipGrid);
+    np += p.grid;
+    parts.push_back(p);
+  }
+  const size_t nlists = (strided.size() + kClipStridedMax - 1) / kClipStridedMax;
+  np += (int)nlists * kClipGrid;
+  auto norm = at::empty({}, in[0].options().dtype(at::kFloat));
+  auto part = at::empty({std::max(np, 1)}, in[0].options().dtype(at::kDouble));
+  double* pp = part.data_ptr<double>();
+  float* nn = norm.data_ptr<float>();
+  cudaStream_t st = at::cuda::getCurrentCUDAStream();
+  for (int scale = 0; scale < (out.empty() ? 1 : 2); ++scale) {
+    double* to = pp;
+    bool first = true;
+    for (const auto& p : parts) {
+      double* q = scale ? pp : to;
+      float* wr = scale && first ? nn : nullptr;
+      if (p.count <= 32) launch_lists<32>(dense, p.at, p.count, p.grid, scale, q, np, (float)max_norm, wr, st);
+      else if (p.count <= 256) launch_lists<256>(dense, p.at, p.count, p.grid, scale, q, np, (float)max_norm, wr, st);
+      else launch_lists<960>(dense, p.at, p.count, p.grid, scale, q, np, (float)max_norm, wr, st);
+      to += p.grid;
+      first = false;
+    }
+    for (size_t s = 0; s < nlists; ++s) {
+      ClipStridedList l;
+      l.count = (int)std::min<size_t>(kClipStridedMax, strided.size() - s * kClipStridedMax);
+      std::copy_n(strided.begin() + s * kClipStridedMax, l.count, l.d);
+      if (scale) clip_scale_strided_kernel<<<kClipGrid, kClipThreads, 0, st>>>(l, pp, np, (float)max_norm);
+      else clip_norm_strided_kernel<<<kClipGrid, kClipThreads, 0, st>>>(l, to);
+      to += kClipGrid;
+      count_launch();
+      C10_CUDA_KERNEL_LAUNCH_CHECK();
+    }
+  }
+  if (out.empty() || parts.empty()) {
+    clip_finish_kernel<<<1, kClipThreads, 0, st>>>(pp, np, nn);
+    count_launch();
+    C10_CUDA_KERNEL_LAUNCH_CHECK();
+  }
+  return norm;
+}
+
+}  // namespace dtb

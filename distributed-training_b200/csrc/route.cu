@@ -1,0 +1,372 @@
+// Routing of tokens to experts: scores, choice of k experts a token, gates, and the
+// gates' gradient with respect to the logits.  (No counterpart in the reference,
+// whose MLPs are dense: dtrain/nn.py:90-101.)
+//
+//   s = softmax(z) or 1 / (1 + exp(-z))          z = logits, fp32; -inf masks an expert
+//   c = z, or s + bias with a balancing bias     what the choice goes by
+//   groups: the keep best of G equal groups stay, by their best c or their two best
+//   idx = the k largest c (ties: lowest expert), gates = scale * s[idx] / max(sum, 1e-20)
+//
+// Both scores increase with z, so without a bias the choice goes by the logits
+// themselves: no two experts are made equal by rounding their scores.  A NaN counts as
+// the largest value, so it is chosen and shows in the gates.  Slots that no expert is
+// left for (a row of masked experts) get idx -1 and gate 0.
+#include <ATen/core/Tensor.h>
+#include <ATen/ops/empty.h>
+#include <ATen/ops/empty_like.h>
+#include <ATen/ops/zeros.h>
+#include <ATen/cuda/CUDAContext.h>
+#include <c10/cuda/CUDAGuard.h>
+
+#include "common.cuh"
+
+namespace dtb {
+
+constexpr int kRouteMaxExperts = 512;
+constexpr int kRouteMaxK = 32;
+constexpr float kRouteTiny = 1e-20f;  // the renormalising sum is at least this
+constexpr unsigned kAll = 0xffffffffu;
+
+struct RouteArgs {
+  const void* logits;
+  const float* bias;
+  float* gates;
+  int* idx;
+  int* load;
+  int n, e, k;
+  int groups, keep, top;
+  int softmax, renorm;
+  float scale;
+};
+
+// Unsigned keys in the order of the floats, -0 = +0, NaN above +inf; 0 is free for
+// "taken or absent" (the key of -inf is above it).
+__device__ __forceinline__ unsigned order_key(float x) {
+  if (x != x) return 0xffffffffu;
+  const unsigned b = __float_as_uint(x + 0.f);
+  return (b & 0x80000000u) ? ~b : (b | 0x80000000u);
+}
+constexpr unsigned kKeyNegInf = 0x007fffffu;
+__device__ __forceinline__ float key_value(unsigned k) {
+  if (k == 0xffffffffu) return __uint_as_float(0x7fc00000u);
+  return __uint_as_float((k & 0x80000000u) ? (k & 0x7fffffffu) : ~k);
+}
+
+__device__ __forceinline__ float load_logit(const float* p) { return *p; }
+__device__ __forceinline__ float load_logit(const bf16* p) { return bf2f(*p); }
+__device__ __forceinline__ void store_logit(float* p, float v) { *p = v; }
+__device__ __forceinline__ void store_logit(bf16* p, float v) { *p = f2bf(v); }
+
+__device__ __forceinline__ float warp_sum(float v) {
+#pragma unroll
+  for (int o = 16; o; o >>= 1) v += __shfl_xor_sync(kAll, v, o);
+  return v;
+}
+__device__ __forceinline__ float warp_max(float v) {
+#pragma unroll
+  for (int o = 16; o; o >>= 1) v = fmaxf(v, __shfl_xor_sync(kAll, v, o));
+  return v;
+}
+__device__ __forceinline__ float sigmoid_f(float z) { return 1.f / (1.f + expf(-z)); }
+
+// One warp per token; lane l holds experts l, l + 32, ...
+template <typename T, int VPL>
+__global__ void __launch_bounds__(256) route_fwd_kernel(RouteArgs a) {
+  __shared__ int s_load[kRouteMaxExperts];
+  for (int i = threadIdx.x; i < a.e; i += blockDim.x) s_load[i] = 0;
+  __syncthreads();
+  const int lane = threadIdx.x & 31;
+  const int warps = (gridDim.x * blockDim.x) >> 5;
+  const int per = a.e / a.groups;
+  for (int t = (blockIdx.x * blockDim.x + threadIdx.x) >> 5; t < a.n; t += warps) {
+    const T* row = reinterpret_cast<const T*>(a.logits) + (long)t * a.e;
+    float z[VPL];
+    unsigned key[VPL];
+    float m = -INFINITY;
+#pragma unroll
+    for (int v = 0; v < VPL; ++v) {
+      const int i = v * 32 + lane;
+      z[v] = i < a.e ? load_logit(row + i) : -INFINITY;
+      m = fmaxf(m, z[v]);
+    }
+    float mx = 0.f, sum = 1.f;  // softmax: s = exp(z - mx) / sum
+    if (a.softmax) {
+      m = warp_max(m);
+      mx = m == -INFINITY ? 0.f : m;
+      float p = 0.f;
+#pragma unroll
+      for (int v = 0; v < VPL; ++v) p += expf(z[v] - mx);
+      sum = warp_sum(p);
+      if (sum == 0.f) sum = 1.f;
+    }
+    const bool by_score = a.bias != nullptr || a.top == 2;
+#pragma unroll
+    for (int v = 0; v < VPL; ++v) {
+      const int i = v * 32 + lane;
+      float c = z[v];
+      if (by_score && z[v] != -INFINITY) {
+        c = a.softmax ? expf(z[v] - mx) / sum : sigmoid_f(z[v]);
+        if (a.bias) c = __fadd_rn(c, a.bias[i]);
+      }
+      key[v] = i < a.e ? order_key(c) : 0u;
+    }
+    if (a.groups > 1) {
+      // lane g keeps the score of group g
+      unsigned gk = 0u;
+      for (int g = 0; g < a.groups; ++g) {
+        unsigned k1 = 0u, k2 = 0u;
+#pragma unroll
+        for (int v = 0; v < VPL; ++v) {
+          const int i = v * 32 + lane;
+          const unsigned k = (i >= g * per && i < (g + 1) * per) ? key[v] : 0u;
+          k2 = max(k2, min(k1, k));
+          k1 = max(k1, k);
+        }
+        const unsigned best = __reduce_max_sync(kAll, k1);
+        unsigned sc = best;
+        if (a.top == 2) {
+          const int first = __ffs(__ballot_sync(kAll, k1 == best)) - 1;
+          const unsigned second = __reduce_max_sync(kAll, lane == first ? k2 : k1);
+          if (best > kKeyNegInf && second > kKeyNegInf)
+            sc = order_key(__fadd_rn(key_value(best), key_value(second)));
+        }
+        if (lane == g) gk = sc;
+      }
+      unsigned kept = 0u;
+      for (int r = 0; r < a.keep; ++r) {
+        const unsigned best = __reduce_max_sync(kAll, gk);
+        const int g = __ffs(__ballot_sync(kAll, gk == best)) - 1;
+        kept |= 1u << g;
+        if (lane == g) gk = 0u;
+      }
+#pragma unroll
+      for (int v = 0; v < VPL; ++v) {
+        const int i = v * 32 + lane;
+        if (i < a.e && !((kept >> (i / per)) & 1u)) key[v] = 0u;
+      }
+    }
+    // k rounds: the largest key, ties to the lowest expert
+    int mine = -1;
+    float sj = 0.f;
+    unsigned lk = 0u;
+    int lv = 0;
+#pragma unroll
+    for (int v = VPL - 1; v >= 0; --v)
+      if (key[v] >= lk) { lk = key[v]; lv = v; }
+    for (int j = 0; j < a.k; ++j) {
+      const unsigned best = __reduce_max_sync(kAll, lk);
+      if (best <= kKeyNegInf) break;
+      const int i = __reduce_min_sync(kAll, lk == best ? lv * 32 + lane : 0x7fffffff);
+      if (lane == j) mine = i;
+      if ((i & 31) == lane) {
+        lk = 0u;
+#pragma unroll
+        for (int v = VPL - 1; v >= 0; --v) {
+          if (v == (i >> 5)) key[v] = 0u;
+          if (key[v] >= lk) { lk = key[v]; lv = v; }
+        }
+      }
+    }
+    if (mine >= 0) {
+      const float zj = load_logit(row + mine);
+      sj = a.softmax ? expf(zj - mx) / sum : sigmoid_f(zj);
+      atomicAdd(&s_load[mine], 1);
+    }
+    const float total = warp_sum(sj);
+    if (lane < a.k) {
+      const float d = a.renorm ? (total < kRouteTiny ? kRouteTiny : total) : 1.f;
+      a.gates[(long)t * a.k + lane] = mine >= 0 ? a.scale * sj / d : 0.f;
+      a.idx[(long)t * a.k + lane] = mine;
+    }
+  }
+  __syncthreads();
+  for (int i = threadIdx.x; i < a.e; i += blockDim.x)
+    if (s_load[i]) atomicAdd(a.load + i, s_load[i]);
+}
+
+struct RouteBwdArgs {
+  const void* logits;
+  const float* gates;
+  const int* idx;
+  const float* dgates;
+  void* dlogits;
+  int n, e, k;
+  int softmax, renorm;
+  float scale;
+};
+
+// One warp per token.  With D = max(S, tiny), S the sum of the chosen s:
+//   ds_j = scale / D (G_j - [renorm, S > tiny] sum_i G_i s_i / D)
+//   sigmoid: dz_j = ds_j s_j (1 - s_j);  softmax: dz_i = s_i (ds_i - sum_j ds_j s_j)
+template <typename T, int VPL>
+__global__ void __launch_bounds__(256) route_bwd_kernel(RouteBwdArgs a) {
+  __shared__ float s_row[8][kRouteMaxExperts];
+  const int lane = threadIdx.x & 31;
+  const int warps = (gridDim.x * blockDim.x) >> 5;
+  float* buf = s_row[threadIdx.x >> 5];
+  for (int t = (blockIdx.x * blockDim.x + threadIdx.x) >> 5; t < a.n; t += warps) {
+    const T* row = reinterpret_cast<const T*>(a.logits) + (long)t * a.e;
+    T* out = reinterpret_cast<T*>(a.dlogits) + (long)t * a.e;
+    int at = -1;
+    float G = 0.f;
+    if (lane < a.k) {
+      at = a.idx[(long)t * a.k + lane];
+      if (at < 0 || at >= a.e) at = -1;
+      if (at >= 0) G = a.dgates[(long)t * a.k + lane];
+    }
+#pragma unroll
+    for (int v = 0; v < VPL; ++v) {
+      const int i = v * 32 + lane;
+      if (i < a.e) buf[i] = 0.f;
+    }
+    __syncwarp();
+    if (!a.softmax) {
+      float ds = G, s = 0.f;
+      if (at >= 0) s = sigmoid_f(load_logit(row + at));
+      const float total = warp_sum(s);
+      if (a.renorm) {
+        const float d = total < kRouteTiny ? kRouteTiny : total;
+        const float dot = warp_sum(G * s) / d;
+        ds = (G - (total > kRouteTiny ? dot : 0.f)) / d;
+      }
+      if (at >= 0) buf[at] = a.scale * ds * s * (1.f - s);
+      __syncwarp();
+#pragma unroll
+      for (int v = 0; v < VPL; ++v) {
+        const int i = v * 32 + lane;
+        if (i < a.e) store_logit(out + i, buf[i]);
+      }
+    } else {
+      float z[VPL];
+      float m = -INFINITY, p = 0.f;
+#pragma unroll
+      for (int v = 0; v < VPL; ++v) {
+        const int i = v * 32 + lane;
+        z[v] = i < a.e ? load_logit(row + i) : -INFINITY;
+        m = fmaxf(m, z[v]);
+      }
+      m = warp_max(m);
+      if (m == -INFINITY) m = 0.f;
+#pragma unroll
+      for (int v = 0; v < VPL; ++v) {
+        z[v] = expf(z[v] - m);
+        p += z[v];
+      }
+      float sum = warp_sum(p);
+      if (sum == 0.f) sum = 1.f;
+      float s = 0.f;
+      if (at >= 0) s = expf(load_logit(row + at) - m) / sum;
+      const float total = warp_sum(s);
+      float ds = G;
+      float d = 1.f;
+      if (a.renorm) {
+        d = total < kRouteTiny ? kRouteTiny : total;
+        const float dot = warp_sum(G * s) / d;
+        ds = G - (total > kRouteTiny ? dot : 0.f);
+      }
+      ds = at >= 0 ? a.scale * ds / d : 0.f;
+      const float back = warp_sum(ds * s);
+      if (at >= 0) buf[at] = ds;
+      __syncwarp();
+#pragma unroll
+      for (int v = 0; v < VPL; ++v) {
+        const int i = v * 32 + lane;
+        if (i < a.e) store_logit(out + i, z[v] / sum * (buf[i] - back));
+      }
+    }
+    __syncwarp();
+  }
+}
+
+static int route_grid(int n) { return (int)std::max<long>(1, std::min<long>((n + 7) / 8, 148L * 8)); }
+
+// Logits [n, e] (fp32 or bf16, contiguous) -> gates fp32 [n, k], idx int32 [n, k], load int32 [e].
+std::vector<at::Tensor> route_fwd(at::Tensor logits, int64_t k, bool softmax, std::optional<at::Tensor> bias,
+                                     int64_t groups, int64_t keep, int64_t top, bool renorm, double scale) {
+  TORCH_CHECK(logits.is_cuda() && logits.dim() == 2 && logits.is_contiguous(), "route: contiguous [n, e] CUDA logits");
+  const bool f32 = logits.scalar_type() == at::kFloat;
+  TORCH_CHECK(f32 || logits.scalar_type() == at::kBFloat16, "route: fp32 or bf16 logits");
+  const long n = logits.size(0), e = logits.size(1);
+  TORCH_CHECK(e >= 1 && e <= kRouteMaxExperts, "route: 1 to ", kRouteMaxExperts, " experts, got ", e);
+  TORCH_CHECK(k >= 1 && k <= e && k <= kRouteMaxK, "route: k must be in [1, min(experts, ", kRouteMaxK, ")], got ", k);
+  TORCH_CHECK(n < (1L << 31) / 32, "route: too many rows");
+  TORCH_CHECK(groups >= 1 && groups <= 32 && e % groups == 0, "route: groups must divide the experts, at most 32");
+  TORCH_CHECK(keep >= 1 && keep <= groups && keep * (e / groups) >= k, "route: the kept groups hold fewer than k experts");
+  TORCH_CHECK(top == 1 || (top == 2 && e / groups >= 2), "route: group_top must be 1, or 2 with groups of at least 2");
+  c10::cuda::CUDAGuard guard(logits.device());
+  RouteArgs a{};
+  if (bias && bias->defined()) {
+    TORCH_CHECK(bias->is_cuda() && bias->get_device() == logits.get_device() && bias->scalar_type() == at::kFloat &&
+                    bias->numel() == e && bias->is_contiguous(),
+                "route: bias must be fp32 [experts] on the logits' device");
+    a.bias = bias->data_ptr<float>();
+  }
+  auto gates = at::empty({n, k}, logits.options().dtype(at::kFloat));
+  auto idx = at::empty({n, k}, logits.options().dtype(at::kInt));
+  auto load = at::zeros({e}, logits.options().dtype(at::kInt));
+  if (n == 0) return {gates, idx, load};
+  a.logits = logits.data_ptr();
+  a.gates = gates.data_ptr<float>();
+  a.idx = idx.data_ptr<int>();
+  a.load = load.data_ptr<int>();
+  a.n = (int)n;
+  a.e = (int)e;
+  a.k = (int)k;
+  a.groups = (int)groups;
+  a.keep = (int)keep;
+  a.top = (int)top;
+  a.softmax = softmax;
+  a.renorm = renorm;
+  a.scale = (float)scale;
+  cudaStream_t st = at::cuda::getCurrentCUDAStream();
+  const int grid = route_grid(a.n);
+#define DTB_ROUTE(V)                                              \
+  if (f32) route_fwd_kernel<float, V><<<grid, 256, 0, st>>>(a);   \
+  else route_fwd_kernel<bf16, V><<<grid, 256, 0, st>>>(a);
+  if (e <= 32) { DTB_ROUTE(1) }
+  else if (e <= 64) { DTB_ROUTE(2) }
+  else if (e <= 128) { DTB_ROUTE(4) }
+  else if (e <= 256) { DTB_ROUTE(8) }
+  else { DTB_ROUTE(16) }
+#undef DTB_ROUTE
+  count_launch();
+  C10_CUDA_KERNEL_LAUNCH_CHECK();
+  return {gates, idx, load};
+}
+
+// d(logits) in the logits' type from the gates' gradient (fp32 [n, k]).
+at::Tensor route_bwd(at::Tensor logits, at::Tensor gates, at::Tensor idx, at::Tensor dgates,
+                        bool softmax, bool renorm, double scale) {
+  TORCH_CHECK(logits.is_cuda() && logits.dim() == 2 && logits.is_contiguous(), "route_bwd: contiguous CUDA logits");
+  const bool f32 = logits.scalar_type() == at::kFloat;
+  TORCH_CHECK(f32 || logits.scalar_type() == at::kBFloat16, "route_bwd: fp32 or bf16 logits");
+  const long n = logits.size(0), e = logits.size(1);
+  TORCH_CHECK(gates.dim() == 2 && gates.size(0) == n && gates.is_contiguous() && gates.scalar_type() == at::kFloat,
+              "route_bwd: gates");
+  const long k = gates.size(1);
+  TORCH_CHECK(e <= kRouteMaxExperts && k >= 1 && k <= kRouteMaxK && k <= e, "route_bwd: sizes");
+  TORCH_CHECK(idx.sizes() == gates.sizes() && idx.scalar_type() == at::kInt && idx.is_contiguous(), "route_bwd: idx");
+  TORCH_CHECK(dgates.sizes() == gates.sizes() && dgates.scalar_type() == at::kFloat && dgates.is_contiguous(),
+              "route_bwd: dgates");
+  c10::cuda::CUDAGuard guard(logits.device());
+  auto dl = at::empty_like(logits);
+  if (n == 0) return dl;
+  RouteBwdArgs a{logits.data_ptr(), gates.data_ptr<float>(), idx.data_ptr<int>(), dgates.data_ptr<float>(),
+                 dl.data_ptr(), (int)n, (int)e, (int)k, softmax, renorm, (float)scale};
+  cudaStream_t st = at::cuda::getCurrentCUDAStream();
+  const int grid = route_grid(a.n);
+#define DTB_ROUTE(V)                                              \
+  if (f32) route_bwd_kernel<float, V><<<grid, 256, 0, st>>>(a);   \
+  else route_bwd_kernel<bf16, V><<<grid, 256, 0, st>>>(a);
+  if (e <= 32) { DTB_ROUTE(1) }
+  else if (e <= 64) { DTB_ROUTE(2) }
+  else if (e <= 128) { DTB_ROUTE(4) }
+  else if (e <= 256) { DTB_ROUTE(8) }
+  else { DTB_ROUTE(16) }
+#undef DTB_ROUTE
+  count_launch();
+  C10_CUDA_KERNEL_LAUNCH_CHECK();
+  return dl;
+}
+
+}  // namespace dtb

@@ -1,7 +1,8 @@
 """Functional ops with the reference's names and semantics (dtrain/autograd.py:199-266).
 
 ``embedding``, ``layer_norm``, ``causal_attention``, ``cross_entropy``, ``gelu``,
-``relu``, ``linear``.  Autograd is PyTorch's.  On CUDA bf16 tensors with
+``relu``, ``linear``; and, beyond the reference, a mixture of experts' ``route`` and
+``expert_mlp``.  Autograd is PyTorch's.  On CUDA bf16 tensors with
 kernel-compatible shapes each op runs the sm_100a kernels through an autograd
 Function (gradients in the inputs' dtypes); on every other input it runs the
 reference math with torch ops - explicit causal softmax, population-variance
@@ -152,6 +153,167 @@ def cross_entropy(logits, targets):
     if _fast(logits) and logits.numel() > 0:
         return _XentFn.apply(logits, targets)
     return F.cross_entropy(logits.reshape(-1, logits.shape[-1]), targets.reshape(-1))
+
+
+# ----------------------------------------------------- mixture of experts
+class _RouteFn(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, logits, k, softmax, bias, groups, keep, top, renorm, scale):
+        gates, idx, load = K.route_fwd(logits, k, softmax=softmax, bias=bias, groups=groups, keep=keep, top=top,
+                                       renorm=renorm, scale=scale)
+        ctx.save_for_backward(logits, gates, idx)
+        ctx.how = (softmax, renorm, scale)
+        ctx.mark_non_differentiable(idx, load)
+        return gates, idx, load
+
+    @staticmethod
+    def backward(ctx, dgates, _idx, _load):
+        logits, gates, idx = ctx.saved_tensors
+        softmax, renorm, scale = ctx.how
+        dz = K.route_bwd(logits, gates, idx, dgates.contiguous(), softmax=softmax, renorm=renorm, scale=scale)
+        return dz, None, None, None, None, None, None, None, None
+
+
+def _route_math(z, k, softmax, bias, groups, keep, top, renorm, scale):
+    """``route`` with torch ops (any device, fp32 or fp64 arithmetic)."""
+    z = z if z.dtype == torch.float64 else z.float()
+    n, e = z.shape
+    gone = z == -math.inf
+    if softmax:
+        s = torch.softmax(z.masked_fill(gone.all(-1, keepdim=True), 0.0), -1).masked_fill(gone, 0.0)
+    else:
+        s = torch.sigmoid(z)
+    with torch.no_grad():
+        if bias is None and top == 1:
+            c = z
+        else:
+            c = (s if bias is None else s + bias.to(s.dtype)).masked_fill(gone, -math.inf)
+        if groups > 1:
+            per = c.view(n, groups, -1)
+            best = torch.sort(per, dim=-1, descending=True).values[..., :top]
+            score = best[..., 0] + best[..., 1:].masked_fill(best[..., 1:] == -math.inf, 0.0).sum(-1)
+            order = torch.sort(score, dim=-1, descending=True, stable=True).indices
+            kept = torch.zeros_like(score, dtype=torch.bool).scatter_(1, order[:, :keep], True)
+            c = per.masked_fill(~kept[..., None], -math.inf).reshape(n, e)
+        c, idx = torch.sort(c, dim=-1, descending=True, stable=True)
+        idx, none = idx[:, :k], c[:, :k] == -math.inf
+        load = torch.bincount(idx.masked_fill(none, e).reshape(-1), minlength=e + 1)[:e].to(torch.int32)
+    sj = s.gather(1, idx).masked_fill(none, 0.0)
+    if renorm:
+        sj = sj / sj.sum(-1, keepdim=True).clamp(min=1e-20)
+    gates = scale * sj
+    return gates, idx.masked_fill(none, -1).to(torch.int32), load
+
+
+def route(logits, k: int, *, score: str = "softmax", bias=None, groups: int = 1, keep_groups: int = 1,
+          group_top: int = 1, renorm: bool = True, scale: float = 1.0):
+    """Choose ``k`` of the experts for each token: ``(gates, idx, load)``.
+
+    ``logits`` (..., experts) become scores s by ``score``: "softmax" over the experts,
+    or "sigmoid" of each.  The choice goes by the logits, or by s + ``bias`` (fp32
+    [experts]; it balances the load and takes no part in the gates) - with
+    ``group_top`` 2 always by the scores.  With ``groups`` > 1 the experts form that
+    many equal groups in a row, and only the ``keep_groups`` best ones stay: by their
+    best expert (``group_top`` 1) or the sum of their two best (2).  Ties go to the
+    lowest expert (group).  gates (..., k), fp32 and in falling order of the choice,
+    are ``scale * s``, divided by the sum of the k scores (at least 1e-20) where
+    ``renorm``.  A logit of -inf masks an expert; slots that no expert is left for have
+    idx -1 and gate 0.  A NaN counts as the largest value and shows in the gates.
+
+    idx (..., k) is int32, load int32 [experts] counts the slots of each expert.  The
+    gates are differentiable in the logits.
+    """
+    if score not in ("softmax", "sigmoid"):
+        raise ValueError(f"route: score must be 'softmax' or 'sigmoid', got {score!r}")
+    e = logits.shape[-1]
+    if not 1 <= k <= e:
+        raise ValueError(f"route: k must be in [1, {e}], got {k}")
+    if groups < 1 or e % groups or not 1 <= keep_groups <= groups or keep_groups * (e // groups) < k:
+        raise ValueError(f"route: {e} experts in {groups} groups, {keep_groups} kept, do not give {k} experts a token")
+    if group_top not in (1, 2) or group_top > e // groups:
+        raise ValueError(f"route: group_top must be 1, or 2 with groups of at least 2, got {group_top}")
+    if bias is not None and (bias.shape != (e,) or bias.device != logits.device):
+        raise ValueError(f"route: bias must be [{e}] on the logits' device")
+    softmax = score == "softmax"
+    z = logits.reshape(-1, e)
+    if z.is_cuda and z.dtype in (torch.float32, torch.bfloat16) and e <= 512 and k <= 32 and groups <= 32:
+        z = z.contiguous()
+        b = bias if bias is None else bias.detach().float().contiguous()
+        if torch.is_grad_enabled() and z.requires_grad:
+            out = _RouteFn.apply(z, k, softmax, b, groups, keep_groups, group_top, renorm, scale)
+        else:
+            out = K.route_fwd(z, k, softmax=softmax, bias=b, groups=groups, keep=keep_groups, top=group_top,
+                              renorm=renorm, scale=scale)
+    else:
+        out = _route_math(z, k, softmax, bias, groups, keep_groups, group_top, renorm, scale)
+    gates, idx, load = out
+    if logits.dim() != 2:
+        gates, idx = gates.view(*logits.shape[:-1], k), idx.view(*logits.shape[:-1], k)
+    return gates, idx, load
+
+
+class _ExpertsFn(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, w1, b1, w2, b2, idx, gates):
+        y, *saved = K.experts_fwd(x, w1, b1, w2, b2, idx, gates, save=True)
+        ctx.save_for_backward(x, w1, w2, gates, *saved)
+        ctx.biases = (b1 is not None, b2 is not None)
+        return y
+
+    @staticmethod
+    def backward(ctx, dy):
+        x, w1, w2, gates, *saved = ctx.saved_tensors
+        dw1, dw2 = torch.empty_like(w1), torch.empty_like(w2)
+        db1 = w1.new_empty(w1.shape[0], w1.shape[2]) if ctx.biases[0] else None
+        db2 = w2.new_empty(w2.shape[0], w2.shape[2]) if ctx.biases[1] else None
+        dx, dgates = K.experts_bwd(dy.contiguous(), x, w1, w2, gates, saved, dw1, db1, dw2, db2)
+        return dx, dw1, db1, dw2, db2, None, dgates
+
+
+def _experts_math(x, w1, b1, w2, b2, idx, gates):
+    """``expert_mlp`` with torch ops, expert by expert."""
+    y = x.new_zeros(x.shape[0], w2.shape[2])
+    for e in range(w1.shape[0]):
+        tok, slot = torch.nonzero(idx == e, as_tuple=True)
+        if tok.numel() == 0:
+            continue
+        h = x[tok] @ w1[e]
+        h = F.gelu(h if b1 is None else h + b1[e], approximate="tanh") @ w2[e]
+        h = h if b2 is None else h + b2[e]
+        y = y.index_add(0, tok, gates[tok, slot][:, None].to(h.dtype) * h)
+    return y
+
+
+def expert_mlp(x, w1, b1, w2, b2, idx, gates):
+    """Mixture of MLPs: ``y = sum_j gates_j (gelu(x @ w1[e] + b1[e]) @ w2[e] + b2[e])``, e = idx_j.
+
+    x (..., c); w1 [experts, c, h], w2 [experts, h, co] (in, out) as in ``linear``; b1
+    [experts, h], b2 [experts, co] or None; idx (..., k) int32 or int64, where -1 is a
+    slot without an expert; gates (..., k).  y (..., co) has x's type; gradients reach
+    x, the weights, the biases and the gates, each in its own type.  An expert that no
+    slot names gets a gradient of zeros.
+    """
+    c = x.shape[-1]
+    if w1.dim() != 3 or w2.dim() != 3 or w1.shape[1] != c or w2.shape[:2] != (w1.shape[0], w1.shape[2]):
+        raise ValueError(f"expert_mlp: x {tuple(x.shape)}, w1 {tuple(w1.shape)} and w2 {tuple(w2.shape)} do not fit")
+    if idx.shape != gates.shape or idx.shape[:-1] != x.shape[:-1]:
+        raise ValueError(f"expert_mlp: idx {tuple(idx.shape)} and gates {tuple(gates.shape)} must be x's rows by slots")
+    if idx.dtype not in (torch.int32, torch.int64):
+        raise ValueError(f"expert_mlp: idx must be int32 or int64, got {idx.dtype}")
+    co = w2.shape[2]
+    x2, idx2, gates2 = x.reshape(-1, c), idx.reshape(-1, idx.shape[-1]), gates.reshape(-1, idx.shape[-1])
+    ok = _fast(x, w1, w2) and (b1 is None or _fast(b1)) and (b2 is None or _fast(b2)) and gates.is_cuda
+    if ok and c % 8 == 0 and w1.shape[2] % 8 == 0 and co % 8 == 0 and w1.shape[0] <= 512 and idx.shape[-1] <= 32 \
+            and gates.dtype in (torch.float32, torch.bfloat16):
+        args = (x2.contiguous(), w1.contiguous(), None if b1 is None else b1.contiguous(), w2.contiguous(),
+                None if b2 is None else b2.contiguous(), idx2.contiguous(), gates2.contiguous())
+        if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (x, w1, b1, w2, b2, gates)):
+            y = _ExpertsFn.apply(*args)
+        else:
+            y = K.experts_fwd(*args)[0]
+    else:
+        y = _experts_math(x2, w1, b1, w2, b2, idx2, gates2)
+    return y if x.dim() == 2 else y.view(*x.shape[:-1], co)
 
 
 # ---------------------------------------------------------------- others

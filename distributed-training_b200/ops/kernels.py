@@ -131,6 +131,37 @@ def grad_sqnorm(g: torch.Tensor, out: torch.Tensor | None = None, scale: float =
     return out
 
 
+def route_fwd(logits: torch.Tensor, k: int, *, softmax: bool = True, bias: torch.Tensor | None = None,
+              groups: int = 1, keep: int = 1, top: int = 1, renorm: bool = True, scale: float = 1.0):
+    """Choice of ``k`` experts for each row of ``logits`` [n, e] (fp32 or bf16).
+    Returns (gates fp32 [n, k], idx int32 [n, k], load int32 [e]); see ``functional.route``."""
+    return lib().route_fwd(logits, k, softmax, bias, groups, keep, top, renorm, scale)
+
+
+def route_bwd(logits, gates, idx, dgates, *, softmax: bool = True, renorm: bool = True,
+              scale: float = 1.0) -> torch.Tensor:
+    """d(logits), in the logits' type, from the gates' gradient (fp32 [n, k])."""
+    return lib().route_bwd(logits, gates, idx, dgates, softmax, renorm, scale)
+
+
+def experts_fwd(x, w1, b1, w2, b2, idx, gates, save: bool = False):
+    """The experts' products (``functional.expert_mlp``) on bf16 rows ``x`` [n, c].
+    Returns [y], or with ``save`` [y, plan, xp, pre, act, yp]: what ``experts_bwd`` reads."""
+    return lib().experts_fwd(x, w1, b1, w2, b2, idx, gates, save)
+
+
+def experts_bwd(dy, x, w1, w2, gates, saved, dw1, db1, dw2, db2):
+    """Returns (dx, dgates); writes the parameters' gradients into ``dw1`` .. ``db2``
+    (all fp32 or all bf16; None for a bias that the layer has not)."""
+    return lib().experts_bwd(dy, x, w1, w2, gates, list(saved), dw1, db1, dw2, db2)
+
+
+def clip_grads(grads, outs, max_norm: float) -> torch.Tensor:
+    """Norm (fp32 scalar) of the CUDA tensors ``grads`` together; with ``outs`` (same
+    shapes; the gradients themselves, or others) also ``outs[i] = grads[i] * factor``."""
+    return lib().clip_grads(grads, outs, max_norm)
+
+
 def cast_f32_bf16(x: torch.Tensor, y: torch.Tensor) -> None:
     lib().cast_f32_bf16(x, y)
 

@@ -2,7 +2,8 @@
 
 API of dtrain/optim.py:7-52: ``AdamW(params, lr, betas, eps, weight_decay)`` with
 ``step(grads)``, ``state_dict()``, ``load_state_dict()``, ``state_bytes()``, and
-``clip_scale(total_sq_norm, max_norm)``.  Parameters are updated in place, so
+``clip_scale(total_sq_norm, max_norm)``; beyond the reference, ``global_norm`` and
+``clip_grads`` over a list of separate gradient tensors.  Parameters are updated in place, so
 ZeRO can run the optimizer on a shard view of the flat master buffer.
 
 Two code paths with the same formula and order of operations
@@ -26,6 +27,65 @@ def clip_scale(total_sq_norm: float, max_norm: float) -> float:
     """Factor that brings the global L2 norm down to ``max_norm`` (1.0 if already below)."""
     n = math.sqrt(float(total_sq_norm))
     return 1.0 if n <= max_norm or n == 0 else max_norm / (n + 1e-6)
+
+
+def _norm_tensors(name, grads):
+    """The gradients as a list; all on one device."""
+    ts = [g for g in grads if g is not None]
+    for g in ts:
+        if not isinstance(g, torch.Tensor) or not g.is_floating_point():
+            raise TypeError(f"{name}: floating tensors expected, got {g.dtype if isinstance(g, torch.Tensor) else type(g)}")
+    return ts
+
+
+def _cuda_list(ts) -> bool:
+    return bool(ts) and all(t.is_cuda and t.dtype in (torch.float32, torch.bfloat16, torch.float16) for t in ts)
+
+
+def global_norm(grads) -> torch.Tensor:
+    """L2 norm of all tensors together (a scalar tensor on their device; fp32 on a GPU).
+    None stands for an absent gradient.  Nothing waits on the host."""
+    ts = _norm_tensors("global_norm", grads)
+    if _cuda_list(ts):
+        from . import kernels as K
+        return K.clip_grads(ts, [], 0.0)
+    if not ts:
+        return torch.zeros(())
+    return torch.stack([g.detach().double().square().sum() for g in ts]).sum().sqrt()
+
+
+def clip_grads(grads, max_norm: float, out=None) -> torch.Tensor:
+    """Scale the gradients so that their global norm is at most ``max_norm``; returns the norm before.
+
+    The factor is ``clip_scale``'s, computed on the device, so nothing waits on the host.
+    ``grads`` may differ in size, layout and type (fp32, bf16, fp16); None stands for an
+    absent one.  They are scaled in place, or, with ``out`` (a list aligned with
+    ``grads``), written there scaled - possibly in another type, such as bf16 gradients
+    into the slices of a flat fp32 buffer - and left as they are.  A NaN or infinite
+    norm shows in the result: the gradients become NaN or 0, as with any clipping that
+    does not look at the norm on the host.
+    """
+    if not max_norm >= 0:
+        raise ValueError(f"clip_grads: max_norm must not be negative, got {max_norm}")
+    grads = list(grads)
+    ts = _norm_tensors("clip_grads", grads)
+    if out is None:
+        to = ts
+    else:
+        if len(out) != len(grads):
+            raise ValueError(f"clip_grads: {len(grads)} gradients but {len(out)} outputs")
+        to = _norm_tensors("clip_grads", [o for g, o in zip(grads, out) if g is not None])
+        if len(to) != len(ts) or any(o.shape != g.shape for g, o in zip(ts, to)):
+            raise ValueError("clip_grads: every gradient needs an output of its own shape")
+    if _cuda_list(ts) and (to is ts or _cuda_list(to)):
+        from . import kernels as K
+        return K.clip_grads(ts, to, float(max_norm))
+    norm = global_norm(ts)
+    with torch.no_grad():
+        f = torch.where((norm <= max_norm) | (norm == 0), 1.0, max_norm / (norm + 1e-6))
+        for g, o in zip(ts, to):
+            o.copy_(g * f.to(g.device))
+    return norm
 
 
 def _to_tensor(x):

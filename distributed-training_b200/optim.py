@@ -1,2 +1,2 @@
 """Reference module name ``dtrain.optim``."""
-from .ops.optim import AdamW, clip_scale  # noqa: F401
+from .ops.optim import AdamW, clip_grads, clip_scale, global_norm  # noqa: F401

@@ -1,0 +1,123 @@
+"""Routing, the experts' products and gradient clipping on the CPU: the torch paths against
+64-bit definitions and differences, and the refusals."""
+import math
+
+import pytest
+import torch
+
+from dtrain_b200 import autograd as F
+from dtrain_b200.optim import clip_grads, clip_scale, global_norm
+
+from moe_ref import experts64, gates64, route64
+
+ROUTES = [dict(), dict(renorm=False), dict(scale=2.5), dict(score="sigmoid"), dict(score="sigmoid", bias=True),
+          dict(score="softmax", bias=True), dict(groups=3, keep_groups=2), dict(groups=4, keep_groups=2, group_top=2),
+          dict(score="sigmoid", bias=True, groups=4, keep_groups=2, group_top=2, scale=2.5)]
+
+
+def _case(kw, n, e, seed=0):
+    """Logits on a grid of 1/64 (so that there are ties) with masked experts and an empty row."""
+    g = torch.Generator().manual_seed(seed)
+    z = torch.randint(-256, 257, (n, e), generator=g).float() / 64
+    z[torch.rand(n, e, generator=g) < 0.15] = -math.inf
+    z[n // 2] = -math.inf
+    kw = dict(kw)
+    if kw.get("bias"):
+        kw["bias"] = torch.randint(-8, 9, (e,), generator=g).float() / 64
+    ref = dict(softmax=kw.get("score", "softmax") == "softmax", bias=kw.get("bias"), groups=kw.get("groups", 1),
+               keep=kw.get("keep_groups", 1), top=kw.get("group_top", 1), renorm=kw.get("renorm", True),
+               scale=kw.get("scale", 1.0))
+    return z, kw, ref
+
+
+@pytest.mark.parametrize("kw", ROUTES)
+def test_route_cpu(kw):
+    z, kw, ref = _case(kw, 41, 12)
+    gates, idx, load = F.route(z.double(), 3, **kw)
+    g, i, l = route64(z, 3, **ref)
+    assert torch.equal(idx.long(), i) and torch.equal(load.long(), l)
+    torch.testing.assert_close(gates, g, rtol=1e-12, atol=1e-14)
+    # shape in front of the experts is kept
+    g3, i3, _ = F.route(z.double().view(41, 1, 12), 3, **kw)
+    assert g3.shape == (41, 1, 3) and torch.equal(i3.view(41, 3), idx)
+
+
+def test_route_gradient_cpu():
+    z = torch.randn(5, 8, dtype=torch.float64, requires_grad=True)
+    for kw in (dict(), dict(renorm=False), dict(score="sigmoid", scale=2.5)):
+        assert torch.autograd.gradcheck(lambda q: F.route(q, 3, **kw)[0], (z,))
+
+
+@pytest.mark.parametrize("bad", [dict(k=0), dict(k=9), dict(score="tanh"), dict(groups=3), dict(groups=4, keep_groups=5),
+                                 dict(groups=4, keep_groups=1), dict(group_top=3), dict(groups=8, keep_groups=8, group_top=2),
+                                 dict(bias=torch.zeros(7))])
+def test_route_refusals(bad):
+    kw = dict(k=3)
+    kw.update(bad)
+    with pytest.raises(ValueError, match="route"):
+        F.route(torch.randn(4, 8), **kw)
+
+
+def _experts(n, c, h, co, e, k, seed=0, bias=True):
+    g = torch.Generator().manual_seed(seed)
+    r = lambda *s: torch.randn(*s, generator=g, dtype=torch.float64)  # noqa: E731
+    idx = torch.stack([torch.randperm(e, generator=g)[:k] for _ in range(n)])
+    idx[n // 2] = -1
+    return (r(n, c), r(e, c, h) * 0.3, r(e, h) if bias else None, r(e, h, co) * 0.3, r(e, co) if bias else None, idx,
+            torch.rand(n, k, generator=g, dtype=torch.float64))
+
+
+@pytest.mark.parametrize("bias", [True, False])
+def test_expert_mlp_cpu(bias):
+    x, w1, b1, w2, b2, idx, gates = _experts(9, 6, 10, 5, 4, 2, bias=bias)
+    y = F.expert_mlp(x, w1, b1, w2, b2, idx, gates)
+    torch.testing.assert_close(y, experts64(x, w1, b1, w2, b2, idx, gates), rtol=1e-12, atol=1e-12)
+    assert torch.equal(y[4], torch.zeros(5, dtype=torch.float64))
+    y3 = F.expert_mlp(x.view(3, 3, 6), w1, b1, w2, b2, idx.view(3, 3, 2), gates.view(3, 3, 2))
+    assert torch.equal(y3.view(9, 5), y)
+
+
+def test_expert_mlp_gradient_cpu():
+    x, w1, b1, w2, b2, idx, gates = _experts(4, 3, 4, 3, 3, 2)
+    leaves = [t.requires_grad_() for t in (x, w1, b1, w2, b2, gates)]
+    assert torch.autograd.gradcheck(lambda x, w1, b1, w2, b2, g: F.expert_mlp(x, w1, b1, w2, b2, idx, g), leaves)
+
+
+def test_expert_mlp_refusals():
+    x, w1, b1, w2, b2, idx, gates = _experts(4, 3, 4, 3, 3, 2)
+    for bad in ((x[:, :2], w1, b1, w2, b2, idx, gates), (x, w1, b1, w2[:2], b2, idx, gates),
+                (x, w1, b1, w2, b2, idx[:3], gates), (x, w1, b1, w2, b2, idx, gates[:, :1]),
+                (x, w1, b1, w2, b2, idx.float(), gates)):
+        with pytest.raises(ValueError, match="expert_mlp"):
+            F.expert_mlp(*bad)
+
+
+@pytest.mark.parametrize("max_norm", [0.5, 1e6])
+def test_clip_cpu(max_norm):
+    g = [torch.randn(7, 3, dtype=torch.float64), None, torch.randn(5, dtype=torch.float64), torch.zeros(0)]
+    norm = math.sqrt(sum(float((t * t).sum()) for t in g if t is not None))
+    f = clip_scale(norm ** 2, max_norm)
+    want = [None if t is None else t * f for t in g]
+    out = [None if t is None else torch.empty_like(t) for t in g]
+    assert abs(float(global_norm(g)) - norm) < 1e-12 * norm
+    assert abs(float(clip_grads(g, max_norm, out=out)) - norm) < 1e-12 * norm
+    assert abs(float(clip_grads(g, max_norm)) - norm) < 1e-12 * norm
+    for a, b, w in zip(g, out, want):
+        if w is not None:
+            torch.testing.assert_close(a, w, rtol=1e-12, atol=0)
+            torch.testing.assert_close(b, w, rtol=1e-12, atol=0)
+
+
+def test_clip_refusals():
+    g = [torch.randn(3), torch.randn(4)]
+    with pytest.raises(ValueError, match="max_norm"):
+        clip_grads(g, -1.0)
+    with pytest.raises(ValueError, match="outputs"):
+        clip_grads(g, 1.0, out=g[:1])
+    with pytest.raises(ValueError, match="shape"):
+        clip_grads(g, 1.0, out=[torch.empty(3), torch.empty(3)])
+    with pytest.raises(ValueError, match="shape"):
+        clip_grads(g, 1.0, out=[torch.empty(3), None])
+    with pytest.raises(TypeError, match="floating"):
+        clip_grads([torch.zeros(3, dtype=torch.int64)], 1.0)
+    assert float(global_norm([])) == 0.0 and float(clip_grads([None], 1.0)) == 0.0

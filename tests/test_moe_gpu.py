@@ -1,0 +1,422 @@
+"""The router, the experts' products and gradient clipping on the GPU against 64-bit definitions.
+
+Tolerances.  Routing computes in fp32: a gate passes through an exponential (2 ulp, and
+2^-24 |z - max| from its rounded argument, |z - max| <= 16 here), a sum in at most 21
+steps, a division, and with renorm another sum (5 steps) and division: under 50 roundings
+of 2^-24, 3e-6.  Its gradient has two more products and sums: 1e-5 of the largest.
+A bf16 rounding is off by at most u = 2^-8 (8 significant bits), at random by about
+0.43 u in the 2-norm.  The experts round the activations and each row's product to bf16
+before they are joined and rounded, the gradients at five places at most: sqrt(5) * 0.43 u,
+1.0 u, with the tanh approximation's 2^-11 beside it; 2 u is allowed.
+The norm sums squares in fp32 eight at a time and then in fp64: 8 * 2^-24, and the fp32
+result's own 2^-24; a scaled element adds two roundings of its type.
+"""
+import math
+
+import pytest
+import torch
+
+pytestmark = pytest.mark.gpu
+
+from dtrain_b200 import autograd as F  # noqa: E402
+from dtrain_b200.ops import kernels as K  # noqa: E402
+from dtrain_b200.optim import clip_grads, clip_scale, global_norm  # noqa: E402
+
+from moe_ref import experts64, gates64, route64  # noqa: E402
+from test_moe import ROUTES, _case  # noqa: E402
+
+U = 2.0 ** -8
+
+
+@pytest.fixture(scope="module", autouse=True)
+def _dev():
+    assert torch.cuda.is_available(), "GPU tests need a CUDA device"
+    torch.manual_seed(0)
+    yield
+    assert K.device_status() == 0
+
+
+# ----------------------------------------------------------------------- routing
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("kw", ROUTES)
+@pytest.mark.parametrize("n,e,k", [(1, 12, 1), (37, 12, 4), (70, 36, 6), (33, 60, 5), (65, 132, 8), (19, 252, 8),
+                                   (9, 444, 32)])
+def test_route(kw, n, e, k, dtype):
+    z, kw, ref = _case(kw, n, e, seed=n + e)
+    z = z.to(dtype)
+    zg = z.cuda().requires_grad_()
+    if kw.get("bias") is not None:
+        kw["bias"] = kw["bias"].cuda()
+    gates, idx, load = F.route(zg, k, **kw)
+    g, i, l = route64(z, k, **ref)
+    assert gates.dtype == torch.float32 and idx.dtype == load.dtype == torch.int32
+    assert torch.equal(idx.cpu().long(), i) and torch.equal(load.cpu().long(), l)
+    torch.testing.assert_close(gates.detach().cpu().double(), g, rtol=3e-6, atol=1e-30)
+    # gradient: autograd of the fp64 definition at the same choices
+    G = torch.randn(n, k)
+    dz, = torch.autograd.grad(gates, zg, G.cuda())
+    z64 = z.double().requires_grad_()
+    opts = {k_: ref[k_] for k_ in ("softmax", "renorm", "scale")}
+    want, = torch.autograd.grad(gates64(z64, i, **opts), z64, G.double())
+    want = torch.nan_to_num(want)  # a row without experts
+    assert dz.dtype == dtype
+    tol = 1e-5 * max(1e-30, float(want.abs().max()))
+    if dtype == torch.bfloat16:
+        assert torch.all((dz.cpu().double() - want).abs() <= tol + U * want.abs())
+    else:
+        assert float((dz.cpu().double() - want).abs().max()) <= tol
+    # without a gradient: the same kernel, the same bits
+    with torch.no_grad():
+        g2, i2, l2 = F.route(zg, k, **kw)
+    assert torch.equal(g2, gates) and torch.equal(i2, idx) and torch.equal(l2, load)
+
+
+@pytest.mark.parametrize("score", ["softmax", "sigmoid"])
+@pytest.mark.parametrize("renorm", [True, False])
+def test_route_gradient_against_differences(score, renorm):
+    z = torch.randn(64, 16)
+    d, G = torch.randn(64, 16), torch.randn(64, 4)
+    zg = z.cuda().requires_grad_()
+    gates, idx, _ = F.route(zg, 4, score=score, renorm=renorm)
+    dz, = torch.autograd.grad(gates, zg, G.cuda())
+    h = 1e-6
+    at = [(gates64(z.double() + s * h * d.double(), idx.cpu().long(), softmax=score == "softmax", renorm=renorm)
+           * G.double()).sum() for s in (1, -1)]
+    num = float(at[0] - at[1]) / (2 * h)
+    ana = float((dz.cpu().double() * d.double()).sum())
+    # the difference's own error is about h^2 and 1e-16 / h times the sum's size
+    assert abs(num - ana) <= 1e-5 * float((dz.cpu().double().abs() * d.double().abs()).sum())
+
+
+def test_route_special_values():
+    z = torch.zeros(6, 8)
+    z[0, 3] = math.nan
+    z[1] = -math.inf
+    z[1, 5] = 0.0
+    z[2, 2] = 3e38
+    z[3] = -3e38
+    z[4, 0] = -0.0
+    z[5] = torch.arange(8) * 1e-38
+    for score in ("softmax", "sigmoid"):
+        gates, idx, load = F.route(z.cuda(), 2, score=score)
+        assert idx[0, 0] == 3 and math.isnan(float(gates[0, 0]))       # a NaN shows
+        assert idx[1].tolist() == [5, -1] and gates[1].tolist() == [1.0, 0.0]
+        assert idx[2, 0] == 2 and math.isfinite(float(gates[2].sum()))
+        assert idx[3].tolist() == [0, 1] and math.isfinite(float(gates[3].sum()))
+        assert idx[4].tolist() == [0, 1]                                # -0 ties with 0
+        assert idx[5].tolist() == [7, 6]                                # ordered by the logits themselves
+        assert int(load.sum()) == 11
+    # all experts masked by sigmoid scores and a bias
+    gates, idx, load = F.route(torch.full((3, 8), -math.inf).cuda(), 2, score="sigmoid", bias=torch.ones(8).cuda())
+    assert torch.all(idx == -1) and torch.all(gates == 0) and int(load.sum()) == 0
+
+
+def test_route_shapes_streams_and_sizes():
+    g, i, l = F.route(torch.empty(0, 8, device="cuda"), 2)
+    assert g.shape == (0, 2) and i.shape == (0, 2) and int(l.sum()) == 0
+    z = torch.randn(50000, 24, device="cuda")
+    s = torch.cuda.Stream()
+    s.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(s):
+        a = F.route(z[:, ::2], 3)                     # strided logits
+    s.synchronize()
+    b = F.route(z[:, ::2].contiguous().view(500, 100, 12), 3)
+    assert torch.equal(a[0], b[0].view(-1, 3)) and torch.equal(a[1], b[1].view(-1, 3)) and torch.equal(a[2], b[2])
+    assert int(a[2].sum()) == 150000
+    # beyond the kernel's 512 experts: torch ops
+    wide = torch.randn(5, 600, device="cuda")
+    assert torch.equal(F.route(wide, 2)[1].long(), wide.topk(2).indices)
+
+
+def test_route_refusals_gpu():
+    z = torch.randn(4, 8, device="cuda")
+    with pytest.raises(ValueError, match="bias"):
+        F.route(z, 2, bias=torch.zeros(8))
+    with pytest.raises(RuntimeError, match="route"):
+        K.route_fwd(z, 9)
+    with pytest.raises(RuntimeError, match="route"):
+        K.route_fwd(z.half(), 2)
+    with pytest.raises(RuntimeError, match="route"):
+        K.route_fwd(z, 4, groups=4, keep=1)
+
+
+# ----------------------------------------------------------------------- experts
+def _rel(a, b):
+    b = b.double()
+    return float((a.double() - b).norm() / b.norm().clamp(min=1e-30))
+
+
+def _inputs(n, c, h, co, e, k, bias=True, skew=0.0, gate=torch.bfloat16, idx_type=torch.int32, seed=0):
+    g = torch.Generator(device="cuda").manual_seed(seed)
+    r = lambda *s: torch.randn(*s, generator=g, device="cuda")  # noqa: E731
+    bf = torch.bfloat16
+    z = r(n, e) - skew * torch.arange(e, device="cuda")
+    idx = z.topk(k, -1).indices.to(idx_type)
+    t = dict(x=r(n, c).to(bf), w1=(r(e, c, h) / math.sqrt(c)).to(bf), b1=(0.1 * r(e, h)).to(bf) if bias else None,
+             w2=(r(e, h, co) / math.sqrt(h)).to(bf), b2=(0.1 * r(e, co)).to(bf) if bias else None, idx=idx,
+             gates=torch.softmax(r(n, k), -1).to(gate))
+    return t, r(n, co).to(bf)
+
+
+EXPERTS = [  # n, c, h, co, e, k, bias, skew
+    (1, 64, 128, 64, 4, 2, True, 0.0),
+    (1, 8, 8, 8, 1, 1, False, 0.0),
+    (3, 72, 136, 40, 5, 3, True, 0.0),
+    (17, 128, 256, 128, 8, 2, False, 0.0),
+    (64, 200, 328, 264, 7, 2, True, 3.0),       # most experts have no row
+    (129, 256, 512, 256, 2, 1, True, 0.0),
+    (257, 320, 640, 320, 3, 3, True, 0.0),
+    (700, 136, 264, 520, 40, 6, False, 0.1),
+    (2000, 512, 384, 512, 4, 2, True, 0.3),
+]
+
+
+@pytest.mark.parametrize("n,c,h,co,e,k,bias,skew", EXPERTS)
+@pytest.mark.parametrize("gate,idx_type", [(torch.bfloat16, torch.int32), (torch.float32, torch.int64)])
+def test_expert_mlp(n, c, h, co, e, k, bias, skew, gate, idx_type):
+    t, dy = _inputs(n, c, h, co, e, k, bias, skew, gate, idx_type)
+    if n > 2:
+        t["idx"][n // 2] = -1                       # a token without an expert
+        t["idx"][0, k - 1] = -1
+    names = [m for m in ("x", "w1", "b1", "w2", "b2", "gates") if t[m] is not None]
+    for m in names:
+        t[m].requires_grad_()
+    y = F.expert_mlp(**t)
+    grads = torch.autograd.grad(y, [t[m] for m in names], dy)
+    d = {m: v.detach().double().requires_grad_(m in names) if v is not None and v.is_floating_point() else v
+         for m, v in t.items()}
+    ref = experts64(**d)
+    want = torch.autograd.grad(ref, [d[m] for m in names], dy.double())
+    assert y.dtype == torch.bfloat16 and _rel(y, ref) <= 2 * U
+    if n > 2:
+        assert torch.all(y[n // 2] == 0)
+    for m, a, b in zip(names, grads, want):
+        assert a.dtype == t[m].dtype and a.shape == t[m].shape
+        assert _rel(a, b) <= 2 * U, m
+        if m[0] in "wb":                            # every expert by itself; unused ones exactly zero
+            for q in range(e):
+                if torch.any(t["idx"] == q):
+                    assert _rel(a[q], b[q]) <= 2 * U, (m, q)
+                else:
+                    assert torch.all(a[q] == 0), (m, q)
+    with torch.no_grad():
+        y2 = F.expert_mlp(**t)
+    assert _rel(y2, ref) <= 2 * U
+    grads2 = torch.autograd.grad(F.expert_mlp(**t), [t[m] for m in names], dy)
+    assert all(torch.equal(a, b) for a, b in zip(grads, grads2)), "fixed orders of summation"
+
+
+def test_expert_mlp_gradient_against_differences():
+    t, dy = _inputs(40, 64, 96, 64, 4, 2, gate=torch.float32)
+    names = ("x", "w1", "b1", "w2", "b2", "gates")
+    for m in names:
+        t[m].requires_grad_()
+    grads = torch.autograd.grad(F.expert_mlp(**t), [t[m] for m in names], dy)
+    d = {m: v.detach().double() if v.is_floating_point() else v for m, v in t.items()}
+    for m, a in zip(names, grads):
+        step = torch.randn_like(d[m])
+        h = 1e-5
+        at = [(experts64(**{**d, m: d[m] + s * h * step}) * dy.double()).sum() for s in (1, -1)]
+        num = float(at[0] - at[1]) / (2 * h)
+        # the sum over entries of (gradient x step): errors of 2 u an entry, at random
+        noise = 2 * U * float((a.double() * step).norm()) * 4
+        assert abs(num - float((a.double() * step).sum())) <= noise, m
+
+
+def test_expert_mlp_repeated_expert_and_bad_index():
+    # the same expert twice for a token counts twice
+    t, _ = _inputs(5, 64, 64, 64, 3, 2)
+    t["idx"][:, 1] = t["idx"][:, 0]
+    y = F.expert_mlp(**t)
+    ref = experts64(**{m: v.double() if v.is_floating_point() else v for m, v in t.items()})
+    assert _rel(y, ref) <= 2 * U
+    # an index past the experts is skipped and reported
+    t["idx"][2, 1] = 3
+    K.device_status()
+    y = F.expert_mlp(**t)
+    assert K.device_status() != 0
+    t["idx"][2, 1] = -1
+    assert torch.equal(y, F.expert_mlp(**t)) and K.device_status() == 0
+
+
+def test_expert_mlp_shapes_and_streams():
+    t, _ = _inputs(24, 64, 128, 64, 4, 2)
+    y = F.expert_mlp(**t)
+    s = torch.cuda.Stream()
+    s.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(s):
+        v = dict(t, x=t["x"].view(2, 12, 64), idx=t["idx"].view(2, 12, 2), gates=t["gates"].view(2, 12, 2))
+        y3 = F.expert_mlp(**v)
+    s.synchronize()
+    assert torch.equal(y3.view(24, 64), y)
+    # strided inputs
+    wide = torch.zeros(24, 128, device="cuda", dtype=torch.bfloat16)
+    wide[:, ::2] = t["x"]
+    assert torch.equal(F.expert_mlp(**dict(t, x=wide[:, ::2])), y)
+    w1t = t["w1"].transpose(1, 2).contiguous().transpose(1, 2)
+    assert torch.equal(F.expert_mlp(**dict(t, w1=w1t)), y)
+    # no tokens
+    e = F.expert_mlp(**dict(t, x=t["x"][:0].requires_grad_(), idx=t["idx"][:0], gates=t["gates"][:0]))
+    assert e.shape == (0, 64)
+    e.sum().backward()
+    # widths that are not multiples of 8, and fp32: torch ops
+    q, _ = _inputs(6, 12, 20, 12, 3, 2)
+    assert _rel(F.expert_mlp(**q), experts64(**{m: v.double() if v.is_floating_point() else v for m, v in q.items()})) < 2 * U
+
+
+def test_expert_mlp_inf_and_nan_stay_in_their_rows():
+    t, _ = _inputs(40, 64, 64, 64, 4, 1)
+    t["x"][7] = math.nan
+    t["x"][9, 3] = math.inf
+    y = F.expert_mlp(**t)
+    assert torch.isnan(y[7]).all() and not torch.isfinite(y[9]).all()
+    rest = [i for i in range(40) if i not in (7, 9)]
+    assert torch.isfinite(y[rest]).all()
+    # an expert that no token names may hold anything
+    t, dy = _inputs(40, 64, 64, 64, 4, 1)
+    t["idx"].clamp_(max=2)
+    t["w1"][3] = math.nan
+    t["w2"][3] = math.inf
+    t["x"].requires_grad_()
+    y = F.expert_mlp(**t)
+    y.backward(dy)
+    assert torch.isfinite(y).all() and torch.isfinite(t["x"].grad).all()
+
+
+def test_experts_kernel_refusals():
+    t, dy = _inputs(8, 64, 64, 64, 4, 2)
+    ok = [t[m] for m in ("x", "w1", "b1", "w2", "b2", "idx", "gates")]
+    for at, bad in ((0, t["x"].float()), (0, t["x"][:, :56]), (1, t["w1"].cpu()), (2, t["b1"][:2]), (3, t["w2"][:, :, :60]),
+                    (5, t["idx"].short()), (5, t["idx"][:4]), (6, t["gates"].half())):
+        args = list(ok)
+        args[at] = bad
+        with pytest.raises(RuntimeError, match="experts"):
+            K.experts_fwd(*args)
+    y, *saved = K.experts_fwd(*ok, save=True)
+    g = [torch.empty_like(t[m]) for m in ("w1", "b1", "w2", "b2")]
+    with pytest.raises(RuntimeError, match="experts_bwd"):
+        K.experts_bwd(dy[:, :32].contiguous(), t["x"], t["w1"], t["w2"], t["gates"], saved, *g)
+    with pytest.raises(RuntimeError, match="experts_bwd"):
+        K.experts_bwd(dy, t["x"], t["w1"], t["w2"], t["gates"], saved, g[0].float(), *g[1:])
+    with pytest.raises(RuntimeError, match="experts_bwd"):
+        K.experts_bwd(dy, t["x"], t["w1"], t["w2"], t["gates"], saved[:3], *g)
+
+
+def test_experts_bwd_fp32_weight_gradients():
+    t, dy = _inputs(300, 136, 264, 72, 5, 2)
+    y, *saved = K.experts_fwd(**t, save=True)
+    b = [torch.empty_like(t[m]) for m in ("w1", "b1", "w2", "b2")]
+    f = [torch.empty_like(v, dtype=torch.float32) for v in b]
+    a = K.experts_bwd(dy, t["x"], t["w1"], t["w2"], t["gates"], saved, *b)
+    c = K.experts_bwd(dy, t["x"], t["w1"], t["w2"], t["gates"], saved, *f)
+    assert all(torch.equal(p, q) for p, q in zip(a, c))
+    assert all(torch.equal(p, q.to(torch.bfloat16)) for p, q in zip(b, f))
+
+
+# ----------------------------------------------------------------------- clipping
+def _clip_check(grads, max_norm, outs=None):
+    want = [g.double().clone() for g in grads]
+    norm = math.sqrt(sum(float((w * w).sum()) for w in want))
+    got = float(global_norm(grads))
+    eps = 9 * 2.0 ** -24
+    assert abs(got - norm) <= eps * norm
+    ret = clip_grads(grads, max_norm, out=outs)
+    assert ret.dtype == torch.float32 and ret.dim() == 0 and float(ret) == got
+    f = clip_scale(norm ** 2, max_norm)
+    for g, o, w in zip(grads, grads if outs is None else outs, want):
+        ulp = {torch.float32: 2.0 ** -23, torch.bfloat16: 2.0 ** -8, torch.float16: 2.0 ** -11}[o.dtype]
+        tiny = {torch.float32: 1e-44, torch.bfloat16: 1e-38, torch.float16: 6e-8}[o.dtype]
+        assert torch.all((o.double() - w * f).abs() <= (w * f).abs() * (ulp + 2 * eps) * 1.01 + tiny)
+        if outs is not None:
+            assert torch.equal(g.double(), w)
+
+
+@pytest.mark.parametrize("max_norm", [0.5, 1e9])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16, torch.float16])
+def test_clip_sizes(dtype, max_norm):
+    sizes = [(), (1,), (3,), (0,), (7, 9), (8192,), (8193,), (16391,), (257, 129), (64, 33, 5)]
+    _clip_check([torch.randn(s, device="cuda").to(dtype) for s in sizes], max_norm)
+
+
+@pytest.mark.parametrize("out_type", [torch.float32, torch.bfloat16, torch.float16])
+def test_clip_into_other_types_and_unaligned_slices(out_type):
+    grads, n = [], 0
+    for i, dt in enumerate([torch.float32, torch.bfloat16, torch.float16] * 5):
+        size = 1 + 613 * i
+        grads.append(torch.randn(size + 7, device="cuda").to(dt)[i % 7:i % 7 + size])   # unaligned starts
+        n += size
+    flat = torch.empty(n + 1, device="cuda", dtype=out_type)
+    outs, off = [], 1
+    for g in grads:
+        outs.append(flat[off:off + g.numel()])
+        off += g.numel()
+    _clip_check(grads, 2.0, outs)
+
+
+def test_clip_layouts():
+    a = torch.randn(40, 50, device="cuda")
+    grads = [a[:, ::2], torch.randn(33, 21, device="cuda").t(), torch.randn(4, 6, 5, 7, device="cuda").permute(2, 0, 3, 1),
+             torch.randn(3, 10, 12, device="cuda")[:, 2:9, 1::3], torch.randn(16, device="cuda")]
+    rest = a[:, 1::2].clone()
+    outs = [torch.empty(g.shape, device="cuda") for g in grads]
+    _clip_check(grads, 1.0, outs)
+    _clip_check(grads, 1.0)
+    assert torch.equal(a[:, 1::2], rest)                                # what lies between is left alone
+    assert abs(float(global_norm([torch.full((1,), 3.0, device="cuda").expand(16)])) - 12.0) < 1e-5
+
+
+def test_clip_many_tensors_and_determinism():
+    g = torch.Generator(device="cuda").manual_seed(3)
+    grads = [torch.randn(1 + (37 * i) % 301, device="cuda", generator=g) for i in range(2300)]
+    first = [x.clone() for x in grads]
+    second = [x.clone() for x in grads]
+    _clip_check(grads, 1.0)
+    n1, n2 = clip_grads(first, 1.0), clip_grads(second, 1.0)
+    assert torch.equal(n1, n2) and all(torch.equal(p, q) for p, q in zip(first, second))
+
+
+def test_clip_large_small_and_nonfinite():
+    _clip_check([torch.full((5000,), 1e30, device="cuda"), torch.ones(3, device="cuda")], 1.0)
+    _clip_check([torch.full((5000,), 1e-30, device="cuda")], 1.0)
+    _clip_check([torch.full((5000,), 1e-30, device="cuda")], 1e-30)
+    _clip_check([torch.zeros(100, device="cuda")], 1.0)
+    x = [torch.ones(100, device="cuda"), torch.ones(9, device="cuda")]
+    x[1][4] = math.nan
+    assert math.isnan(float(clip_grads(x, 1.0))) and torch.isnan(x[0]).all()
+    x = [torch.ones(100, device="cuda"), torch.ones(9, device="cuda")]
+    x[1][4] = math.inf
+    assert math.isinf(float(clip_grads(x, 1.0))) and torch.all(x[0] == 0) and torch.isnan(x[1][4])
+
+
+def test_clip_graph_and_stream():
+    grads = [torch.randn(1000, device="cuda"), torch.randn(77, device="cuda").bfloat16()]
+    outs = [torch.empty_like(g, dtype=torch.float32) for g in grads]
+    clip_grads(grads, 1.0, out=outs)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        norm = clip_grads(grads, 1.0, out=outs)
+    for g in grads:
+        g.mul_(3.0)
+    graph.replay()
+    torch.cuda.synchronize()
+    want = math.sqrt(sum(float(g.double().square().sum()) for g in grads))
+    assert abs(float(norm) - want) < 1e-6 * want
+    torch.testing.assert_close(outs[0], grads[0] * clip_scale(want ** 2, 1.0), rtol=1e-6, atol=0)
+
+
+def test_clip_refusals_gpu():
+    a = torch.randn(100, device="cuda")
+    with pytest.raises(RuntimeError, match="overlap"):
+        clip_grads([a, a], 1.0)
+    with pytest.raises(RuntimeError, match="overlap"):
+        clip_grads([a[:60], a[50:]], 1.0)
+    with pytest.raises(RuntimeError, match="overlap"):
+        clip_grads([a[:50], torch.randn(50, device="cuda")], 1.0, out=[torch.empty(50, device="cuda"), a[20:70]])
+    with pytest.raises(RuntimeError, match="overlap"):
+        clip_grads([torch.randn(1, device="cuda").expand(5)], 1.0)
+    with pytest.raises(RuntimeError, match="overlays"):
+        clip_grads([a], 1.0, out=[a.view(torch.bfloat16)[:100]])
+    with pytest.raises(RuntimeError, match="max_norm"):
+        K.clip_grads([a], [a], -1.0)
+    with pytest.raises(RuntimeError, match="fp32"):
+        K.clip_grads([a.double()], [], 1.0)
