@@ -59,8 +59,15 @@ std::vector<torch::Tensor> experts_bwd(torch::Tensor dy, torch::Tensor x, torch:
                                        torch::Tensor gates, std::vector<torch::Tensor> saved, torch::Tensor dw1,
                                        c10::optional<torch::Tensor> db1, torch::Tensor dw2,
                                        c10::optional<torch::Tensor> db2);
+// autograd_ops.cpp
+std::vector<torch::Tensor> route_autograd(torch::Tensor logits, int64_t k, bool softmax,
+                                          c10::optional<torch::Tensor> bias, int64_t groups, int64_t keep, int64_t top,
+                                          bool renorm, double scale);
+torch::Tensor experts_autograd(torch::Tensor x, torch::Tensor w1, c10::optional<torch::Tensor> b1, torch::Tensor w2,
+                               c10::optional<torch::Tensor> b2, torch::Tensor idx, torch::Tensor gates);
 // clip.cu
-torch::Tensor clip_grads(std::vector<torch::Tensor> in, std::vector<torch::Tensor> out, double max_norm);
+torch::Tensor clip_grads(std::vector<c10::optional<torch::Tensor>> in,
+                         c10::optional<std::vector<c10::optional<torch::Tensor>>> out, double max_norm, bool scale);
 // comm.cu
 std::tuple<int64_t, torch::Tensor> symm_alloc(int64_t nbytes);
 int64_t symm_open(torch::Tensor handle);
@@ -174,7 +181,9 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
         py::arg("idx"), py::arg("gates"), py::arg("save"));
   m.def("experts_bwd", &experts_bwd, py::arg("dy"), py::arg("x"), py::arg("w1"), py::arg("w2"), py::arg("gates"),
         py::arg("saved"), py::arg("dw1"), py::arg("db1"), py::arg("dw2"), py::arg("db2"));
-  m.def("clip_grads", &clip_grads);
+  m.def("route", &route_autograd);
+  m.def("experts", &experts_autograd);
+  m.def("clip_grads", &clip_grads, py::arg("grads"), py::arg("out"), py::arg("max_norm"), py::arg("scale"));
   m.def("symm_alloc", &symm_alloc);
   m.def("symm_open", &symm_open);
   m.def("symm_close", &symm_close);

@@ -419,48 +419,67 @@ static void launch_lists(const std::vector<ClipDesc>& all, size_t at, size_t cou
   C10_CUDA_KERNEL_LAUNCH_CHECK();
 }
 
-// The norm (fp32 scalar) of the tensors `in` together; with `out` (as many tensors, of the
-// same shapes) also out[i] = in[i] * factor.  out[i] may be in[i].
-at::Tensor clip_grads(std::vector<at::Tensor> in, std::vector<at::Tensor> out, double max_norm) {
-  TORCH_CHECK(!in.empty(), "clip_grads: an empty list has no device");
-  TORCH_CHECK(out.empty() || out.size() == in.size(), "clip_grads: ", in.size(), " gradients but ", out.size(), " outputs");
-  TORCH_CHECK(max_norm >= 0.0, "clip_grads: max_norm must not be negative");
-  const auto dev = in[0].device();
+// The norm (fp32 scalar) of the tensors `in` together (those that are there); with `scale`
+// also in[i] *= factor or, with `out` (aligned with `in`, of the same shapes),
+// out[i] = in[i] * factor.  out[i] may be in[i].
+at::Tensor clip_grads(std::vector<std::optional<at::Tensor>> in,
+                      std::optional<std::vector<std::optional<at::Tensor>>> out, double max_norm, bool scale) {
+  TORCH_CHECK_VALUE(max_norm >= 0.0, "clip_grads: max_norm must not be negative, got ", max_norm);
+  TORCH_CHECK_VALUE(!out || out->size() == in.size(), "clip_grads: ", in.size(), " gradients but ",
+                    out ? out->size() : 0, " outputs");
+  const at::Tensor* head = nullptr;
+  for (const auto& t : in)
+    if (t) {
+      head = &*t;
+      break;
+    }
+  TORCH_CHECK_VALUE(head, "clip_grads: an empty list has no device");
+  const auto dev = head->device();
   TORCH_CHECK(dev.is_cuda(), "clip_grads: CUDA tensors expected");
   c10::cuda::CUDAGuard guard(dev);
   std::vector<ClipDesc> dense;
   std::vector<ClipStrided> strided;
   std::vector<ClipRange> ranges;
   dense.reserve(in.size());
-  ranges.reserve(out.empty() ? 0 : 2 * in.size());
+  if (scale) ranges.reserve(out ? 2 * in.size() : in.size());
   for (size_t i = 0; i < in.size(); ++i) {
-    const at::Tensor& a = in[i];
-    const at::Tensor* b = out.empty() ? nullptr : &out[i];
+    if (!in[i]) continue;
+    const at::Tensor& a = *in[i];
+    TORCH_CHECK_VALUE(!scale || !out || (*out)[i], "clip_grads: every gradient needs an output of its own shape");
+    const at::Tensor* b = !scale ? nullptr : out ? &*(*out)[i] : &a;
     TORCH_CHECK(a.device() == dev && (!b || b->device() == dev), "clip_grads: tensor ", i, " is on another device");
-    const short ta = clip_type(a), tb = b ? clip_type(*b) : 0;
-    TORCH_CHECK(!b || b->sizes() == a.sizes(), "clip_grads: output ", i, " has another shape than its gradient");
-    if (a.numel() == 0) continue;
-    const bool same = b && b->data_ptr() == a.data_ptr();
+    const short ta = clip_type(a), tb = !b ? 0 : b == &a ? ta : clip_type(*b);
+    TORCH_CHECK_VALUE(!b || b == &a || b->sizes() == a.sizes(), "clip_grads: output ", i,
+                      " has another shape than its gradient");
+    const long numel = a.numel();
+    if (numel == 0) continue;
+    const void* pa = a.const_data_ptr();
+    void* pb = b ? b->mutable_data_ptr() : nullptr;
+    const bool same = pa == pb;
     TORCH_CHECK(!same || (ta == tb && same_order(a, *b)), "clip_grads: output ", i, " overlays its gradient differently");
-    const bool flat = a.is_non_overlapping_and_dense() &&
-                      (!b || same || (b->is_non_overlapping_and_dense() && same_order(a, *b)));
+    const bool dense_a = a.is_non_overlapping_and_dense();
+    const bool dense_b = b && (b == &a ? dense_a : b->is_non_overlapping_and_dense());
+    const bool flat = dense_a && (!b || same || (dense_b && same_order(a, *b)));
     if (b) {
-      TORCH_CHECK(at::has_internal_overlap(*b) != at::MemOverlap::Yes, "clip_grads: output ", i, " overlaps itself");
-      const auto range = [&](const at::Tensor& t, bool o) {
-        long last = 0;
-        for (int64_t k = 0; k < t.dim(); ++k) last += (t.size(k) - 1) * t.stride(k);
-        const uintptr_t lo = reinterpret_cast<uintptr_t>(t.data_ptr());
-        ranges.push_back({lo, lo + (last + 1) * t.element_size(), (int)i, o});
-      };
-      if (flat || b->is_non_overlapping_and_dense()) {
+      TORCH_CHECK(dense_b || at::has_internal_overlap(*b) != at::MemOverlap::Yes, "clip_grads: output ", i,
+                  " overlaps itself");
+      if (flat) {
+        const uintptr_t lo = reinterpret_cast<uintptr_t>(pa), lb = reinterpret_cast<uintptr_t>(pb);
+        if (!same) ranges.push_back({lo, lo + numel * a.element_size(), (int)i, false});
+        ranges.push_back({lb, lb + numel * b->element_size(), (int)i, true});
+      } else if (dense_b) {
+        const auto range = [&](const at::Tensor& t, bool o) {
+          long last = 0;
+          for (int64_t k = 0; k < t.dim(); ++k) last += (t.size(k) - 1) * t.stride(k);
+          const uintptr_t lo = reinterpret_cast<uintptr_t>(t.const_data_ptr());
+          ranges.push_back({lo, lo + (last + 1) * t.element_size(), (int)i, o});
+        };
         if (!same) range(a, false);
         range(*b, true);
       }
     }
-    if (flat)
-      dense.push_back({a.data_ptr(), b ? b->data_ptr() : nullptr, (long)a.numel(), 0, ta, tb});
-    else
-      strided.push_back(strided_desc(a, b));
+    if (flat) dense.push_back({pa, pb, numel, 0, ta, tb});
+    else strided.push_back(strided_desc(a, b));
   }
   check_ranges(ranges);
 
@@ -485,20 +504,20 @@ at::Tensor clip_grads(std::vector<at::Tensor> in, std::vector<at::Tensor> out, d
   }
   const size_t nlists = (strided.size() + kClipStridedMax - 1) / kClipStridedMax;
   np += (int)nlists * kClipGrid;
-  auto norm = at::empty({}, in[0].options().dtype(at::kFloat));
-  auto part = at::empty({std::max(np, 1)}, in[0].options().dtype(at::kDouble));
+  auto norm = at::empty({}, head->options().dtype(at::kFloat));
+  auto part = at::empty({std::max(np, 1)}, head->options().dtype(at::kDouble));
   double* pp = part.data_ptr<double>();
   float* nn = norm.data_ptr<float>();
   cudaStream_t st = at::cuda::getCurrentCUDAStream();
-  for (int scale = 0; scale < (out.empty() ? 1 : 2); ++scale) {
+  for (int pass = 0; pass < (scale ? 2 : 1); ++pass) {
     double* to = pp;
     bool first = true;
     for (const auto& p : parts) {
-      double* q = scale ? pp : to;
-      float* wr = scale && first ? nn : nullptr;
-      if (p.count <= 32) launch_lists<32>(dense, p.at, p.count, p.grid, scale, q, np, (float)max_norm, wr, st);
-      else if (p.count <= 256) launch_lists<256>(dense, p.at, p.count, p.grid, scale, q, np, (float)max_norm, wr, st);
-      else launch_lists<960>(dense, p.at, p.count, p.grid, scale, q, np, (float)max_norm, wr, st);
+      double* q = pass ? pp : to;
+      float* wr = pass && first ? nn : nullptr;
+      if (p.count <= 32) launch_lists<32>(dense, p.at, p.count, p.grid, pass, q, np, (float)max_norm, wr, st);
+      else if (p.count <= 256) launch_lists<256>(dense, p.at, p.count, p.grid, pass, q, np, (float)max_norm, wr, st);
+      else launch_lists<960>(dense, p.at, p.count, p.grid, pass, q, np, (float)max_norm, wr, st);
       to += p.grid;
       first = false;
     }
@@ -506,14 +525,14 @@ at::Tensor clip_grads(std::vector<at::Tensor> in, std::vector<at::Tensor> out, d
       ClipStridedList l;
       l.count = (int)std::min<size_t>(kClipStridedMax, strided.size() - s * kClipStridedMax);
       std::copy_n(strided.begin() + s * kClipStridedMax, l.count, l.d);
-      if (scale) clip_scale_strided_kernel<<<kClipGrid, kClipThreads, 0, st>>>(l, pp, np, (float)max_norm);
+      if (pass) clip_scale_strided_kernel<<<kClipGrid, kClipThreads, 0, st>>>(l, pp, np, (float)max_norm);
       else clip_norm_strided_kernel<<<kClipGrid, kClipThreads, 0, st>>>(l, to);
       to += kClipGrid;
       count_launch();
       C10_CUDA_KERNEL_LAUNCH_CHECK();
     }
   }
-  if (out.empty() || parts.empty()) {
+  if (!scale || parts.empty()) {
     clip_finish_kernel<<<1, kClipThreads, 0, st>>>(pp, np, nn);
     count_launch();
     C10_CUDA_KERNEL_LAUNCH_CHECK();

@@ -14,9 +14,9 @@
 #include <ATen/core/Tensor.h>
 #include <ATen/ops/empty.h>
 #include <ATen/ops/empty_like.h>
-#include <ATen/ops/zeros.h>
 #include <ATen/cuda/CUDAContext.h>
 #include <c10/cuda/CUDAGuard.h>
+#include <c10/cuda/CUDAException.h>
 
 #include "common.cuh"
 
@@ -36,6 +36,9 @@ struct RouteArgs {
   int n, e, k;
   int groups, keep, top;
   int softmax, renorm;
+  int lanes;     // route_fwd_kernel: lanes of a group
+  int vec;       // its lanes' values start at 16-byte boundaries
+  int need_sum;  // the softmax's sum takes part: not when the gates are renormalised over the row's largest
   float scale;
 };
 
@@ -67,12 +70,207 @@ __device__ __forceinline__ float warp_max(float v) {
   for (int o = 16; o; o >>= 1) v = fmaxf(v, __shfl_xor_sync(kAll, v, o));
   return v;
 }
-__device__ __forceinline__ float sigmoid_f(float z) { return 1.f / (1.f + expf(-z)); }
+__device__ __forceinline__ float sigmoid_f(float z) { return __frcp_rn(1.f + expf(-z)); }
 
-// One warp per token; lane l holds experts l, l + 32, ...
-template <typename T, int VPL>
+// The gates of the chosen experts (lane j: slot j).
+template <typename T>
+__device__ __forceinline__ void route_finish(const RouteArgs& a, const T* row, int t, int lane, int mine, float mx,
+                                             float sum, int* s_load) {
+  float sj = 0.f;
+  if (mine >= 0) {
+    const float zj = load_logit(row + mine);
+    sj = a.softmax ? expf(zj - mx) / sum : sigmoid_f(zj);
+    atomicAdd(&s_load[mine], 1);
+  }
+  float d = 1.f;
+  if (a.renorm) {
+    const float total = warp_sum(sj);
+    d = total < kRouteTiny ? kRouteTiny : total;
+  }
+  if (lane < a.k) {
+    a.gates[(long)t * a.k + lane] = mine >= 0 ? a.scale * sj / d : 0.f;
+    a.idx[(long)t * a.k + lane] = mine;
+  }
+}
+__device__ __forceinline__ void route_counts(const RouteArgs& a, const int* s_load) {
+  __syncthreads();
+  for (int i = threadIdx.x; i < a.e; i += blockDim.x) {
+    if (gridDim.x == 1) a.load[i] = s_load[i];
+    else if (s_load[i]) atomicAdd(a.load + i, s_load[i]);
+  }
+}
+
+// V values of a row from `p` on, of which the first `valid` are there (vec: all, 16-byte aligned).
+template <typename T, int V>
+__device__ __forceinline__ void load_logits(const T* p, int valid, bool vec, float* z) {
+  constexpr int PER16 = 16 / (int)sizeof(T);
+  if constexpr (V % PER16 == 0) {
+    if (vec) {
+#pragma unroll
+      for (int i = 0; i < V / PER16; ++i) {
+        const uint4 u = *(reinterpret_cast<const uint4*>(p) + i);  // p: global or shared memory
+        const unsigned w[4] = {u.x, u.y, u.z, u.w};
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          if constexpr (sizeof(T) == 4) {
+            z[i * 4 + j] = __uint_as_float(w[j]);
+          } else {
+            z[i * 8 + 2 * j] = __uint_as_float(w[j] << 16);
+            z[i * 8 + 2 * j + 1] = __uint_as_float(w[j] & 0xffff0000u);
+          }
+        }
+      }
+      return;
+    }
+  }
+#pragma unroll
+  for (int v = 0; v < V; ++v) z[v] = v < valid ? load_logit(p + v) : -INFINITY;
+}
+template <typename T, int V>
+__device__ __forceinline__ void store_logits(T* p, int valid, bool vec, const float* z) {
+  constexpr int PER16 = 16 / (int)sizeof(T);
+  if constexpr (V % PER16 == 0) {
+    if (vec) {
+#pragma unroll
+      for (int i = 0; i < V / PER16; ++i) {
+        uint4 u;
+        if constexpr (sizeof(T) == 4)
+          u = make_uint4(__float_as_uint(z[4 * i]), __float_as_uint(z[4 * i + 1]), __float_as_uint(z[4 * i + 2]),
+                         __float_as_uint(z[4 * i + 3]));
+        else
+          u = make_uint4(pack_bf16x2(z[8 * i], z[8 * i + 1]), pack_bf16x2(z[8 * i + 2], z[8 * i + 3]),
+                         pack_bf16x2(z[8 * i + 4], z[8 * i + 5]), pack_bf16x2(z[8 * i + 6], z[8 * i + 7]));
+        *(reinterpret_cast<uint4*>(p) + i) = u;
+      }
+      return;
+    }
+  }
+#pragma unroll
+  for (int v = 0; v < V; ++v)
+    if (v < valid) store_logit(p + v, z[v]);
+}
+
+// One warp per token.  The lanes are split evenly over the groups (their number rounded up
+// to a power of two), and each lane holds V experts in a row of its group, sorted once by
+// a stable exchange of neighbours; lanes stand in the experts' order, so the lowest lane
+// that holds a largest key holds the lowest such expert.  A group's two best come from the
+// heads of its lanes' lists by xor-shuffles, all groups at once, and each of the k rounds
+// takes the largest head of the warp (redux) and pops it.
+//
+// Bound by instruction issue: per token about 25 V for the scores, 5 V (V - 1) / 2 for the
+// sort and 18 a round.  The form that keeps the values unsorted and rescans V values a
+// round (route_fwd_wide_kernel) costs 7 V a round and 10 V a group: it serves V > 8, where
+// the sort would cost more.
+template <typename T, int V>
 __global__ void __launch_bounds__(256) route_fwd_kernel(RouteArgs a) {
-  __shared__ int s_load[kRouteMaxExperts];
+  extern __shared__ int s_load[];
+  for (int i = threadIdx.x; i < a.e; i += blockDim.x) s_load[i] = 0;
+  __syncthreads();
+  const int lane = threadIdx.x & 31;
+  const int warps = (gridDim.x * blockDim.x) >> 5;
+  const int per = a.e / a.groups;
+  const int group = lane / a.lanes, part = lane % a.lanes;  // lanes: of a group, a power of two
+  const int base = group * per + part * V;
+  const int valid = group < a.groups ? max(0, min(V, per - part * V)) : 0;
+  const bool by_score = a.bias != nullptr || a.top == 2;
+  float bias[V];
+#pragma unroll
+  for (int v = 0; v < V; ++v) bias[v] = a.bias != nullptr && v < valid ? a.bias[base + v] : 0.f;
+  for (int t = (blockIdx.x * blockDim.x + threadIdx.x) >> 5; t < a.n; t += warps) {
+    const T* row = reinterpret_cast<const T*>(a.logits) + (long)t * a.e;
+    float z[V];
+    load_logits<T, V>(row + base, valid, a.vec && valid == V, z);
+    float mx = 0.f, sum = 1.f;  // softmax: s = exp(z - mx) / sum
+    if (a.softmax) {
+      float m = z[0];
+#pragma unroll
+      for (int v = 1; v < V; ++v) m = fmaxf(m, z[v]);
+      m = warp_max(m);
+      mx = m == -INFINITY ? 0.f : m;
+      if (a.need_sum) {
+        float p = 0.f;
+#pragma unroll
+        for (int v = 0; v < V; ++v) p += expf(z[v] - mx);
+        sum = warp_sum(p);
+        if (sum == 0.f) sum = 1.f;
+      }
+    }
+    unsigned key[V];
+    int at[V];
+#pragma unroll
+    for (int v = 0; v < V; ++v) {
+      float c = z[v];
+      if (by_score) {
+        c = a.softmax ? expf(z[v] - mx) / sum : sigmoid_f(z[v]);
+        if (a.bias != nullptr) c = __fadd_rn(c, bias[v]);
+        if (z[v] == -INFINITY) c = -INFINITY;
+      }
+      key[v] = v < valid ? order_key(c) : 0u;
+      at[v] = v;
+    }
+#pragma unroll
+    for (int i = 0; i < V - 1; ++i)
+#pragma unroll
+      for (int j = 0; j < V - 1 - i; ++j)
+        if (key[j + 1] > key[j]) {
+          const unsigned k0 = key[j];
+          const int a0 = at[j];
+          key[j] = key[j + 1];
+          at[j] = at[j + 1];
+          key[j + 1] = k0;
+          at[j + 1] = a0;
+        }
+    unsigned where = 0u;  // the list's experts, four bits each
+#pragma unroll
+    for (int v = 0; v < V; ++v) where |= (unsigned)at[v] << (4 * v);
+    if (a.groups > 1) {
+      unsigned k1 = key[0], k2 = 0u;
+      if constexpr (V > 1) k2 = key[1];
+      for (int o = 1; o < a.lanes; o <<= 1) {
+        const unsigned b1 = __shfl_xor_sync(kAll, k1, o), b2 = __shfl_xor_sync(kAll, k2, o);
+        k2 = max(min(k1, b1), max(k2, b2));
+        k1 = max(k1, b1);
+      }
+      unsigned score = k1;
+      if (a.top == 2 && k1 > kKeyNegInf && k2 > kKeyNegInf)
+        score = order_key(__fadd_rn(key_value(k1), key_value(k2)));
+      if (part != 0 || group >= a.groups) score = 0u;  // one lane a group
+      unsigned kept = 0u;
+      for (int r = 0; r < a.keep; ++r) {
+        const unsigned best = __reduce_max_sync(kAll, score);
+        const int l = __ffs(__ballot_sync(kAll, score == best && part == 0 && group < a.groups &&
+                                                    !((kept >> group) & 1u))) - 1;
+        kept |= 1u << (l / a.lanes);
+        if (lane == l) score = 0u;
+      }
+      if (!((kept >> group) & 1u)) {
+#pragma unroll
+        for (int v = 0; v < V; ++v) key[v] = 0u;
+      }
+    }
+    int mine = -1;
+    for (int j = 0; j < a.k; ++j) {
+      const unsigned best = __reduce_max_sync(kAll, key[0]);
+      if (best <= kKeyNegInf) break;
+      const int l = __ffs(__ballot_sync(kAll, key[0] == best)) - 1;
+      const int i = __shfl_sync(kAll, base + (int)(where & 15u), l);
+      if (lane == j) mine = i;
+      if (lane == l) {
+#pragma unroll
+        for (int v = 0; v < V - 1; ++v) key[v] = key[v + 1];
+        key[V - 1] = 0u;
+        where >>= 4;
+      }
+    }
+    route_finish(a, row, t, lane, mine, mx, sum, s_load);
+  }
+  route_counts(a, s_load);
+}
+
+// One warp per token; lane l holds experts l, l + 32, ... unsorted: any groups and sizes.
+template <typename T, int VPL>
+__global__ void __launch_bounds__(256) route_fwd_wide_kernel(RouteArgs a) {
+  extern __shared__ int s_load[];
   for (int i = threadIdx.x; i < a.e; i += blockDim.x) s_load[i] = 0;
   __syncthreads();
   const int lane = threadIdx.x & 31;
@@ -147,7 +345,6 @@ __global__ void __launch_bounds__(256) route_fwd_kernel(RouteArgs a) {
     }
     // k rounds: the largest key, ties to the lowest expert
     int mine = -1;
-    float sj = 0.f;
     unsigned lk = 0u;
     int lv = 0;
 #pragma unroll
@@ -167,21 +364,9 @@ __global__ void __launch_bounds__(256) route_fwd_kernel(RouteArgs a) {
         }
       }
     }
-    if (mine >= 0) {
-      const float zj = load_logit(row + mine);
-      sj = a.softmax ? expf(zj - mx) / sum : sigmoid_f(zj);
-      atomicAdd(&s_load[mine], 1);
-    }
-    const float total = warp_sum(sj);
-    if (lane < a.k) {
-      const float d = a.renorm ? (total < kRouteTiny ? kRouteTiny : total) : 1.f;
-      a.gates[(long)t * a.k + lane] = mine >= 0 ? a.scale * sj / d : 0.f;
-      a.idx[(long)t * a.k + lane] = mine;
-    }
+    route_finish(a, row, t, lane, mine, mx, sum, s_load);
   }
-  __syncthreads();
-  for (int i = threadIdx.x; i < a.e; i += blockDim.x)
-    if (s_load[i]) atomicAdd(a.load + i, s_load[i]);
+  route_counts(a, s_load);
 }
 
 struct RouteBwdArgs {
@@ -192,92 +377,85 @@ struct RouteBwdArgs {
   void* dlogits;
   int n, e, k;
   int softmax, renorm;
+  int vec;  // the lanes' values start at 16-byte boundaries
   float scale;
 };
 
 // One warp per token.  With D = max(S, tiny), S the sum of the chosen s:
 //   ds_j = scale / D (G_j - [renorm, S > tiny] sum_i G_i s_i / D)
 //   sigmoid: dz_j = ds_j s_j (1 - s_j);  softmax: dz_i = s_i (ds_i - sum_j ds_j s_j)
-template <typename T, int VPL>
+// The row is put together in shared memory (each lane owns V experts in a row) and
+// written with 16-byte stores.  Bound by memory: the sigmoid reads the chosen logits
+// only, the softmax the row; both write the row.
+template <typename T, int V>
 __global__ void __launch_bounds__(256) route_bwd_kernel(RouteBwdArgs a) {
-  __shared__ float s_row[8][kRouteMaxExperts];
+  extern __shared__ __align__(16) float s_row[];
   const int lane = threadIdx.x & 31;
   const int warps = (gridDim.x * blockDim.x) >> 5;
-  float* buf = s_row[threadIdx.x >> 5];
+  float* buf = s_row + (threadIdx.x >> 5) * (32 * V);
+  const int base = lane * V;
+  const int valid = max(0, min(V, a.e - base));
+  const bool vec = a.vec && valid == V;
   for (int t = (blockIdx.x * blockDim.x + threadIdx.x) >> 5; t < a.n; t += warps) {
     const T* row = reinterpret_cast<const T*>(a.logits) + (long)t * a.e;
     T* out = reinterpret_cast<T*>(a.dlogits) + (long)t * a.e;
     int at = -1;
-    float G = 0.f;
+    float G = 0.f, zj = 0.f;
     if (lane < a.k) {
       at = a.idx[(long)t * a.k + lane];
-      if (at < 0 || at >= a.e) at = -1;
-      if (at >= 0) G = a.dgates[(long)t * a.k + lane];
+      if (at >= a.e) at = -1;
+      if (at >= 0) {
+        G = a.dgates[(long)t * a.k + lane];
+        zj = load_logit(row + at);
+      }
     }
+    float w[V];
 #pragma unroll
-    for (int v = 0; v < VPL; ++v) {
-      const int i = v * 32 + lane;
-      if (i < a.e) buf[i] = 0.f;
-    }
-    __syncwarp();
-    if (!a.softmax) {
-      float ds = G, s = 0.f;
-      if (at >= 0) s = sigmoid_f(load_logit(row + at));
-      const float total = warp_sum(s);
-      if (a.renorm) {
-        const float d = total < kRouteTiny ? kRouteTiny : total;
-        const float dot = warp_sum(G * s) / d;
-        ds = (G - (total > kRouteTiny ? dot : 0.f)) / d;
-      }
-      if (at >= 0) buf[at] = a.scale * ds * s * (1.f - s);
-      __syncwarp();
+    for (int v = 0; v < V; ++v) w[v] = 0.f;
+    store_logits<float, V>(buf + base, V, true, w);
+    float m = 0.f, sum = 1.f;
+    if (a.softmax) {
+      load_logits<T, V>(row + base, valid, vec, w);
+      m = w[0];
 #pragma unroll
-      for (int v = 0; v < VPL; ++v) {
-        const int i = v * 32 + lane;
-        if (i < a.e) store_logit(out + i, buf[i]);
-      }
-    } else {
-      float z[VPL];
-      float m = -INFINITY, p = 0.f;
-#pragma unroll
-      for (int v = 0; v < VPL; ++v) {
-        const int i = v * 32 + lane;
-        z[v] = i < a.e ? load_logit(row + i) : -INFINITY;
-        m = fmaxf(m, z[v]);
-      }
+      for (int v = 1; v < V; ++v) m = fmaxf(m, w[v]);
       m = warp_max(m);
       if (m == -INFINITY) m = 0.f;
+      float p = 0.f;
 #pragma unroll
-      for (int v = 0; v < VPL; ++v) {
-        z[v] = expf(z[v] - m);
-        p += z[v];
+      for (int v = 0; v < V; ++v) {
+        w[v] = expf(w[v] - m);
+        p += w[v];
       }
-      float sum = warp_sum(p);
+      sum = warp_sum(p);
       if (sum == 0.f) sum = 1.f;
-      float s = 0.f;
-      if (at >= 0) s = expf(load_logit(row + at) - m) / sum;
-      const float total = warp_sum(s);
-      float ds = G;
-      float d = 1.f;
-      if (a.renorm) {
-        d = total < kRouteTiny ? kRouteTiny : total;
-        const float dot = warp_sum(G * s) / d;
-        ds = G - (total > kRouteTiny ? dot : 0.f);
-      }
-      ds = at >= 0 ? a.scale * ds / d : 0.f;
-      const float back = warp_sum(ds * s);
-      if (at >= 0) buf[at] = ds;
-      __syncwarp();
-#pragma unroll
-      for (int v = 0; v < VPL; ++v) {
-        const int i = v * 32 + lane;
-        if (i < a.e) store_logit(out + i, z[v] / sum * (buf[i] - back));
-      }
     }
+    float s = 0.f;
+    if (at >= 0) s = a.softmax ? expf(zj - m) / sum : sigmoid_f(zj);
+    float ds = G;
+    if (a.renorm) {
+      const float total = warp_sum(s);
+      const float d = total < kRouteTiny ? kRouteTiny : total;
+      const float dot = warp_sum(G * s) / d;
+      ds = (G - (total > kRouteTiny ? dot : 0.f)) / d;
+    }
+    ds = at >= 0 ? a.scale * ds : 0.f;
+    const float back = a.softmax ? warp_sum(ds * s) : 0.f;
+    __syncwarp();
+    if (at >= 0) buf[at] = a.softmax ? ds : ds * s * (1.f - s);
+    __syncwarp();
+    float b[V];
+    load_logits<float, V>(buf + base, V, true, b);
+    if (a.softmax) {
+#pragma unroll
+      for (int v = 0; v < V; ++v) b[v] = w[v] / sum * (b[v] - back);
+    }
+    store_logits<T, V>(out + base, valid, vec, b);
     __syncwarp();
   }
 }
 
+// Eight warps a CTA, one token each at a time.
 static int route_grid(int n) { return (int)std::max<long>(1, std::min<long>((n + 7) / 8, 148L * 8)); }
 
 // Logits [n, e] (fp32 or bf16, contiguous) -> gates fp32 [n, k], idx int32 [n, k], load int32 [e].
@@ -303,7 +481,10 @@ std::vector<at::Tensor> route_fwd(at::Tensor logits, int64_t k, bool softmax, st
   }
   auto gates = at::empty({n, k}, logits.options().dtype(at::kFloat));
   auto idx = at::empty({n, k}, logits.options().dtype(at::kInt));
-  auto load = at::zeros({e}, logits.options().dtype(at::kInt));
+  auto load = at::empty({e}, logits.options().dtype(at::kInt));
+  cudaStream_t st = at::cuda::getCurrentCUDAStream();
+  const int grid = route_grid((int)n);
+  if (grid > 1 || n == 0) C10_CUDA_CHECK(cudaMemsetAsync(load.data_ptr(), 0, e * 4, st));  // one CTA writes its counts
   if (n == 0) return {gates, idx, load};
   a.logits = logits.data_ptr();
   a.gates = gates.data_ptr<float>();
@@ -318,16 +499,24 @@ std::vector<at::Tensor> route_fwd(at::Tensor logits, int64_t k, bool softmax, st
   a.softmax = softmax;
   a.renorm = renorm;
   a.scale = (float)scale;
-  cudaStream_t st = at::cuda::getCurrentCUDAStream();
-  const int grid = route_grid(a.n);
-#define DTB_ROUTE(V)                                              \
-  if (f32) route_fwd_kernel<float, V><<<grid, 256, 0, st>>>(a);   \
-  else route_fwd_kernel<bf16, V><<<grid, 256, 0, st>>>(a);
-  if (e <= 32) { DTB_ROUTE(1) }
-  else if (e <= 64) { DTB_ROUTE(2) }
-  else if (e <= 128) { DTB_ROUTE(4) }
-  else if (e <= 256) { DTB_ROUTE(8) }
-  else { DTB_ROUTE(16) }
+  a.need_sum = !(renorm && !a.bias && groups == 1 && top == 1);
+  int pow2 = 1;
+  while (pow2 < groups) pow2 *= 2;
+  a.lanes = 32 / pow2;
+  const long per = e / groups, v = (per + a.lanes - 1) / a.lanes;
+  const int V = v <= 1 ? 1 : v <= 2 ? 2 : v <= 4 ? 4 : 8;
+  const int es = f32 ? 4 : 2;
+  a.vec = per % V == 0 && (V * es) % 16 == 0 && (e * es) % 16 == 0 &&
+          (reinterpret_cast<uintptr_t>(a.logits) & 15) == 0;
+#define DTB_ROUTE(KERN, V)                                              \
+  if (f32) KERN<float, V><<<grid, 256, e * 4, st>>>(a);                 \
+  else KERN<bf16, V><<<grid, 256, e * 4, st>>>(a);
+  if (v <= 1) { DTB_ROUTE(route_fwd_kernel, 1) }
+  else if (v <= 2) { DTB_ROUTE(route_fwd_kernel, 2) }
+  else if (v <= 4) { DTB_ROUTE(route_fwd_kernel, 4) }
+  else if (v <= 8) { DTB_ROUTE(route_fwd_kernel, 8) }
+  else if (e <= 256) { DTB_ROUTE(route_fwd_wide_kernel, 8) }
+  else { DTB_ROUTE(route_fwd_wide_kernel, 16) }
 #undef DTB_ROUTE
   count_launch();
   C10_CUDA_KERNEL_LAUNCH_CHECK();
@@ -352,16 +541,20 @@ at::Tensor route_bwd(at::Tensor logits, at::Tensor gates, at::Tensor idx, at::Te
   auto dl = at::empty_like(logits);
   if (n == 0) return dl;
   RouteBwdArgs a{logits.data_ptr(), gates.data_ptr<float>(), idx.data_ptr<int>(), dgates.data_ptr<float>(),
-                 dl.data_ptr(), (int)n, (int)e, (int)k, softmax, renorm, (float)scale};
+                 dl.data_ptr(), (int)n, (int)e, (int)k, softmax, renorm, 0, (float)scale};
+  const int V = e <= 32 ? 1 : e <= 64 ? 2 : e <= 128 ? 4 : e <= 256 ? 8 : 16;
+  const int es = f32 ? 4 : 2;
+  a.vec = (V * es) % 16 == 0 && (e * es) % 16 == 0 &&
+          ((reinterpret_cast<uintptr_t>(a.logits) | reinterpret_cast<uintptr_t>(a.dlogits)) & 15) == 0;
   cudaStream_t st = at::cuda::getCurrentCUDAStream();
   const int grid = route_grid(a.n);
-#define DTB_ROUTE(V)                                              \
-  if (f32) route_bwd_kernel<float, V><<<grid, 256, 0, st>>>(a);   \
-  else route_bwd_kernel<bf16, V><<<grid, 256, 0, st>>>(a);
-  if (e <= 32) { DTB_ROUTE(1) }
-  else if (e <= 64) { DTB_ROUTE(2) }
-  else if (e <= 128) { DTB_ROUTE(4) }
-  else if (e <= 256) { DTB_ROUTE(8) }
+#define DTB_ROUTE(V)                                                             \
+  if (f32) route_bwd_kernel<float, V><<<grid, 256, 8 * 32 * V * 4, st>>>(a);     \
+  else route_bwd_kernel<bf16, V><<<grid, 256, 8 * 32 * V * 4, st>>>(a);
+  if (V == 1) { DTB_ROUTE(1) }
+  else if (V == 2) { DTB_ROUTE(2) }
+  else if (V == 4) { DTB_ROUTE(4) }
+  else if (V == 8) { DTB_ROUTE(8) }
   else { DTB_ROUTE(16) }
 #undef DTB_ROUTE
   count_launch();

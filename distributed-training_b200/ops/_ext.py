@@ -23,7 +23,7 @@ BUILD_DIR = PKG_DIR / "_build"
 NAME = "dtb_C"
 
 SOURCES = ["bindings.cpp", "gemm.cu", "layernorm.cu", "embed_xent.cu", "optim.cu", "attention.cu", "attention_tc.cu", "comm.cu",
-           "vmm.cpp", "route.cu", "moe.cu", "clip.cu"]
+           "vmm.cpp", "route.cu", "moe.cu", "clip.cu", "autograd_ops.cpp"]
 
 CUDA_FLAGS = [
     "-gencode", "arch=compute_100a,code=sm_100a",

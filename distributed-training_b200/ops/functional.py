@@ -156,24 +156,6 @@ def cross_entropy(logits, targets):
 
 
 # ----------------------------------------------------- mixture of experts
-class _RouteFn(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, logits, k, softmax, bias, groups, keep, top, renorm, scale):
-        gates, idx, load = K.route_fwd(logits, k, softmax=softmax, bias=bias, groups=groups, keep=keep, top=top,
-                                       renorm=renorm, scale=scale)
-        ctx.save_for_backward(logits, gates, idx)
-        ctx.how = (softmax, renorm, scale)
-        ctx.mark_non_differentiable(idx, load)
-        return gates, idx, load
-
-    @staticmethod
-    def backward(ctx, dgates, _idx, _load):
-        logits, gates, idx = ctx.saved_tensors
-        softmax, renorm, scale = ctx.how
-        dz = K.route_bwd(logits, gates, idx, dgates.contiguous(), softmax=softmax, renorm=renorm, scale=scale)
-        return dz, None, None, None, None, None, None, None, None
-
-
 def _route_math(z, k, softmax, bias, groups, keep, top, renorm, scale):
     """``route`` with torch ops (any device, fp32 or fp64 arithmetic)."""
     z = z if z.dtype == torch.float64 else z.float()
@@ -239,35 +221,13 @@ def route(logits, k: int, *, score: str = "softmax", bias=None, groups: int = 1,
     if z.is_cuda and z.dtype in (torch.float32, torch.bfloat16) and e <= 512 and k <= 32 and groups <= 32:
         z = z.contiguous()
         b = bias if bias is None else bias.detach().float().contiguous()
-        if torch.is_grad_enabled() and z.requires_grad:
-            out = _RouteFn.apply(z, k, softmax, b, groups, keep_groups, group_top, renorm, scale)
-        else:
-            out = K.route_fwd(z, k, softmax=softmax, bias=b, groups=groups, keep=keep_groups, top=group_top,
-                              renorm=renorm, scale=scale)
+        out = K.route(z, k, softmax, b, groups, keep_groups, group_top, renorm, scale)
     else:
         out = _route_math(z, k, softmax, bias, groups, keep_groups, group_top, renorm, scale)
     gates, idx, load = out
     if logits.dim() != 2:
         gates, idx = gates.view(*logits.shape[:-1], k), idx.view(*logits.shape[:-1], k)
     return gates, idx, load
-
-
-class _ExpertsFn(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, x, w1, b1, w2, b2, idx, gates):
-        y, *saved = K.experts_fwd(x, w1, b1, w2, b2, idx, gates, save=True)
-        ctx.save_for_backward(x, w1, w2, gates, *saved)
-        ctx.biases = (b1 is not None, b2 is not None)
-        return y
-
-    @staticmethod
-    def backward(ctx, dy):
-        x, w1, w2, gates, *saved = ctx.saved_tensors
-        dw1, dw2 = torch.empty_like(w1), torch.empty_like(w2)
-        db1 = w1.new_empty(w1.shape[0], w1.shape[2]) if ctx.biases[0] else None
-        db2 = w2.new_empty(w2.shape[0], w2.shape[2]) if ctx.biases[1] else None
-        dx, dgates = K.experts_bwd(dy.contiguous(), x, w1, w2, gates, saved, dw1, db1, dw2, db2)
-        return dx, dw1, db1, dw2, db2, None, dgates
 
 
 def _experts_math(x, w1, b1, w2, b2, idx, gates):
@@ -305,12 +265,8 @@ def expert_mlp(x, w1, b1, w2, b2, idx, gates):
     ok = _fast(x, w1, w2) and (b1 is None or _fast(b1)) and (b2 is None or _fast(b2)) and gates.is_cuda
     if ok and c % 8 == 0 and w1.shape[2] % 8 == 0 and co % 8 == 0 and w1.shape[0] <= 512 and idx.shape[-1] <= 32 \
             and gates.dtype in (torch.float32, torch.bfloat16):
-        args = (x2.contiguous(), w1.contiguous(), None if b1 is None else b1.contiguous(), w2.contiguous(),
-                None if b2 is None else b2.contiguous(), idx2.contiguous(), gates2.contiguous())
-        if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (x, w1, b1, w2, b2, gates)):
-            y = _ExpertsFn.apply(*args)
-        else:
-            y = K.experts_fwd(*args)[0]
+        y = K.experts(x2.contiguous(), w1.contiguous(), None if b1 is None else b1.contiguous(), w2.contiguous(),
+                      None if b2 is None else b2.contiguous(), idx2.contiguous(), gates2.contiguous())
     else:
         y = _experts_math(x2, w1, b1, w2, b2, idx2, gates2)
     return y if x.dim() == 2 else y.view(*x.shape[:-1], co)

@@ -144,6 +144,16 @@ def route_bwd(logits, gates, idx, dgates, *, softmax: bool = True, renorm: bool 
     return lib().route_bwd(logits, gates, idx, dgates, softmax, renorm, scale)
 
 
+def route(logits, k, softmax, bias, groups, keep, top, renorm, scale):
+    """``route_fwd`` with autograd (csrc/autograd_ops.cpp): the gates are differentiable in the logits."""
+    return lib().route(logits, k, softmax, bias, groups, keep, top, renorm, scale)
+
+
+def experts(x, w1, b1, w2, b2, idx, gates) -> torch.Tensor:
+    """The experts' products with autograd (csrc/autograd_ops.cpp); gradients in the tensors' own types."""
+    return lib().experts(x, w1, b1, w2, b2, idx, gates)
+
+
 def experts_fwd(x, w1, b1, w2, b2, idx, gates, save: bool = False):
     """The experts' products (``functional.expert_mlp``) on bf16 rows ``x`` [n, c].
     Returns [y], or with ``save`` [y, plan, xp, pre, act, yp]: what ``experts_bwd`` reads."""
@@ -156,10 +166,10 @@ def experts_bwd(dy, x, w1, w2, gates, saved, dw1, db1, dw2, db2):
     return lib().experts_bwd(dy, x, w1, w2, gates, list(saved), dw1, db1, dw2, db2)
 
 
-def clip_grads(grads, outs, max_norm: float) -> torch.Tensor:
-    """Norm (fp32 scalar) of the CUDA tensors ``grads`` together; with ``outs`` (same
-    shapes; the gradients themselves, or others) also ``outs[i] = grads[i] * factor``."""
-    return lib().clip_grads(grads, outs, max_norm)
+def clip_grads(grads, out, max_norm: float, scale: bool = True) -> torch.Tensor:
+    """Norm (fp32 scalar) of the CUDA tensors ``grads`` together (None: absent); with
+    ``scale`` also ``grads[i] *= factor`` or, with ``out``, ``out[i] = grads[i] * factor``."""
+    return lib().clip_grads(grads, out, max_norm, scale)
 
 
 def cast_f32_bf16(x: torch.Tensor, y: torch.Tensor) -> None:

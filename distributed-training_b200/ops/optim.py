@@ -29,8 +29,13 @@ def clip_scale(total_sq_norm: float, max_norm: float) -> float:
     return 1.0 if n <= max_norm or n == 0 else max_norm / (n + 1e-6)
 
 
-def _norm_tensors(name, grads):
-    """The gradients as a list; all on one device."""
+def _on_gpu(grads) -> bool:
+    """Whether the kernels take the list: its first tensor decides, the others must be like it."""
+    g = next((g for g in grads if g is not None), None)
+    return isinstance(g, torch.Tensor) and g.is_cuda and g.dtype in (torch.float32, torch.bfloat16, torch.float16)
+
+
+def _floating(name, grads):
     ts = [g for g in grads if g is not None]
     for g in ts:
         if not isinstance(g, torch.Tensor) or not g.is_floating_point():
@@ -38,17 +43,14 @@ def _norm_tensors(name, grads):
     return ts
 
 
-def _cuda_list(ts) -> bool:
-    return bool(ts) and all(t.is_cuda and t.dtype in (torch.float32, torch.bfloat16, torch.float16) for t in ts)
-
-
 def global_norm(grads) -> torch.Tensor:
     """L2 norm of all tensors together (a scalar tensor on their device; fp32 on a GPU).
     None stands for an absent gradient.  Nothing waits on the host."""
-    ts = _norm_tensors("global_norm", grads)
-    if _cuda_list(ts):
+    grads = list(grads)
+    if _on_gpu(grads):
         from . import kernels as K
-        return K.clip_grads(ts, [], 0.0)
+        return K.clip_grads(grads, None, 0.0, scale=False)
+    ts = _floating("global_norm", grads)
     if not ts:
         return torch.zeros(())
     return torch.stack([g.detach().double().square().sum() for g in ts]).sum().sqrt()
@@ -65,21 +67,18 @@ def clip_grads(grads, max_norm: float, out=None) -> torch.Tensor:
     norm shows in the result: the gradients become NaN or 0, as with any clipping that
     does not look at the norm on the host.
     """
+    grads = list(grads)
+    if _on_gpu(grads):
+        from . import kernels as K
+        return K.clip_grads(grads, out, float(max_norm))
     if not max_norm >= 0:
         raise ValueError(f"clip_grads: max_norm must not be negative, got {max_norm}")
-    grads = list(grads)
-    ts = _norm_tensors("clip_grads", grads)
-    if out is None:
-        to = ts
-    else:
-        if len(out) != len(grads):
-            raise ValueError(f"clip_grads: {len(grads)} gradients but {len(out)} outputs")
-        to = _norm_tensors("clip_grads", [o for g, o in zip(grads, out) if g is not None])
-        if len(to) != len(ts) or any(o.shape != g.shape for g, o in zip(ts, to)):
-            raise ValueError("clip_grads: every gradient needs an output of its own shape")
-    if _cuda_list(ts) and (to is ts or _cuda_list(to)):
-        from . import kernels as K
-        return K.clip_grads(ts, to, float(max_norm))
+    if out is not None and len(out) != len(grads):
+        raise ValueError(f"clip_grads: {len(grads)} gradients but {len(out)} outputs")
+    ts = _floating("clip_grads", grads)
+    to = ts if out is None else _floating("clip_grads", [o for g, o in zip(grads, out) if g is not None])
+    if len(to) != len(ts) or any(o.shape != g.shape for g, o in zip(ts, to)):
+        raise ValueError("clip_grads: every gradient needs an output of its own shape")
     norm = global_norm(ts)
     with torch.no_grad():
         f = torch.where((norm <= max_norm) | (norm == 0), 1.0, max_norm / (norm + 1e-6))

@@ -416,7 +416,16 @@ def test_clip_refusals_gpu():
         clip_grads([torch.randn(1, device="cuda").expand(5)], 1.0)
     with pytest.raises(RuntimeError, match="overlays"):
         clip_grads([a], 1.0, out=[a.view(torch.bfloat16)[:100]])
-    with pytest.raises(RuntimeError, match="max_norm"):
-        K.clip_grads([a], [a], -1.0)
+    with pytest.raises(ValueError, match="max_norm"):
+        clip_grads([a], -1.0)
+    with pytest.raises(ValueError, match="outputs"):
+        clip_grads([a], 1.0, out=[])
+    with pytest.raises(ValueError, match="shape"):
+        clip_grads([a], 1.0, out=[a[:50]])
+    with pytest.raises(ValueError, match="shape"):
+        clip_grads([a], 1.0, out=[None])
     with pytest.raises(RuntimeError, match="fp32"):
-        K.clip_grads([a.double()], [], 1.0)
+        clip_grads([a, a.double()], 1.0)
+    with pytest.raises(RuntimeError, match="device"):
+        clip_grads([a, torch.zeros(3)], 1.0)
+    assert float(global_norm([None, torch.full((4,), 2.0, device="cuda"), None])) == 4.0
