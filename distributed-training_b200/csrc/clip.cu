@@ -271,9 +271,9 @@ __device__ __forceinline__ void clip_chunk_scale(const ClipDesc& d, int chunk, f
   const uint4* p = reinterpret_cast<const uint4*>(base + s.head * S);
   char* o = out + s.head * SO;
   const bool wide = (reinterpret_cast<uintptr_t>(o) & (4 * SO - 1)) == 0;  // four outputs at a time
-  for (int i = threadIdx.x; i < s.vecs; i += kClipThreads) {
+  const auto put = [&](int i, const uint4& u) {
     float v[N];
-    ClipVec<T>::get(p[i], v);
+    ClipVec<T>::get(u, v);
 #pragma unroll
     for (int j = 0; j < N; ++j) v[j] *= f;
     if (wide) {
@@ -283,7 +283,17 @@ __device__ __forceinline__ void clip_chunk_scale(const ClipDesc& d, int chunk, f
 #pragma unroll
       for (int j = 0; j < N; ++j) clip_store(o, TO, (long)i * N + j, v[j]);
     }
+  };
+  constexpr int U = 4;
+  int i = threadIdx.x;
+  for (; i + (U - 1) * kClipThreads < s.vecs; i += U * kClipThreads) {
+    uint4 u[U];
+#pragma unroll
+    for (int j = 0; j < U; ++j) u[j] = __ldcs(p + i + j * kClipThreads);
+#pragma unroll
+    for (int j = 0; j < U; ++j) put(i + j * kClipThreads, u[j]);
   }
+  for (; i < s.vecs; i += kClipThreads) put(i, __ldcs(p + i));
   for (int e = threadIdx.x; e < s.len - s.vecs * N; e += kClipThreads) {
     const int at = e < s.head ? e : e + s.vecs * N;
     clip_store(out, TO, at, clip_load(base, T, at) * f);
@@ -302,7 +312,8 @@ __global__ void __launch_bounds__(kClipThreads)
     clip_scale_kernel(const __grid_constant__ ClipList<CAP> l, const double* __restrict__ part, int np, float max_norm,
                       float* norm) {
   const float f = clip_total(part, np, max_norm, norm);
-  for (int c = blockIdx.x; c < l.chunks; c += gridDim.x) {
+  // from the last chunk to the first: the norm has read the last ones last, so they are still in L2
+  for (int c = l.chunks - 1 - (int)blockIdx.x; c >= 0; c -= gridDim.x) {
     const ClipDesc& d = l.d[clip_find(l, c)];
     if (d.out == nullptr || (f == 1.f && d.in == d.out)) continue;
     if (d.in_t == CLIP_F32) clip_chunk_scale_to<CLIP_F32>(d, c, f);

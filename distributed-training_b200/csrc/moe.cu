@@ -13,7 +13,7 @@
 //   moe_grad_rows     u[r] = gate dy[token of r],  dgate = dy . yp[r]
 //   grouped GEMMs     dpre = (u W2^T) gelu'(pre) ; dxp = dpre W1^T
 //   grouped GEMMs     dW2_e = act_e^T u_e ; dW1_e = xp_e^T dpre_e   (over the expert's rows)
-//   moe_col_sums      db2_e, db1_e
+//   moe_join_sums     db2_e, db1_e from sums over blocks of rows that moe_grad_rows and the dpre GEMM leave
 //
 // The number of rows of each expert stays on the device: grids are sized by the most
 // tiles that the slots can fill, and the kernels read the real counts from the plan.
@@ -35,8 +35,9 @@ constexpr int kRowPad = 64;
 
 // The plan (int32), sized by the most rows and tiles that P slots and E experts can have.
 struct MoePlan {
-  int4* tile;  // row tiles of 128 in expert order: {expert, first row, end of the expert's rows, 0}
-  int* ntile;  // [1], padded to 4
+  int4* tile;   // row tiles of 128 in expert order: {expert, first row, end of the expert's rows, 0}
+  int4* tile2;  // the same of 256 rows
+  int* ntile;   // [2] their numbers, padded to 4
   int* off;    // [E + 1] first row of each expert, a multiple of 64
   int* count;  // [E] rows of each expert, without the padding
   int* inv;    // [P] row of a slot, -1: none
@@ -51,12 +52,13 @@ constexpr int kPlanThreads = 256;
 constexpr int kPlanChunk = 2048;  // slots a block sorts: 8 warps x 256
 static long plan_blocks(long P) { return std::max<long>(1, (P + kPlanChunk - 1) / kPlanChunk); }
 static long plan_ints(long P, long E) {
-  return 4 * moe_max_tiles(P, E) + 4 + (E + 1) + E + P + moe_max_rows(P, E) + plan_blocks(P) * E;
+  return 8 * moe_max_tiles(P, E) + 4 + (E + 1) + E + P + moe_max_rows(P, E) + plan_blocks(P) * E;
 }
 static MoePlan plan_views(int* p, long P, long E) {
   MoePlan v;
   v.tile = reinterpret_cast<int4*>(p);
-  v.ntile = p + 4 * moe_max_tiles(P, E);
+  v.tile2 = v.tile + moe_max_tiles(P, E);
+  v.ntile = p + 8 * moe_max_tiles(P, E);
   v.off = v.ntile + 4;
   v.count = v.off + E + 1;
   v.inv = v.count + E;
@@ -86,41 +88,114 @@ __global__ void __launch_bounds__(kPlanThreads) moe_hist_kernel(const I* __restr
   for (int i = threadIdx.x; i < E; i += blockDim.x) pl.hist[(long)blockIdx.x * E + i] = s_h[i];
 }
 
+// Inclusive sums over the block's 512 threads of (a, b, c); every thread calls it.
+__device__ __forceinline__ void plan_scan(int& a, int& b, int& c) {
+  __shared__ int s_t[3][kMoeMaxExperts / 32];
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const int x = __shfl_up_sync(0xffffffffu, a, o), y = __shfl_up_sync(0xffffffffu, b, o),
+              z = __shfl_up_sync(0xffffffffu, c, o);
+    if (lane >= o) { a += x; b += y; c += z; }
+  }
+  if (lane == 31) { s_t[0][warp] = a; s_t[1][warp] = b; s_t[2][warp] = c; }
+  __syncthreads();
+  for (int w = 0; w < warp; ++w) { a += s_t[0][w]; b += s_t[1][w]; c += s_t[2][w]; }
+}
+
+// Thread e of 512: expert e's offsets and tiles from its number of rows; returns its first row.
+__device__ __forceinline__ int plan_expert(const MoePlan& pl, int e, int E, int total) {
+  const int padded = (total + kRowPad - 1) / kRowPad * kRowPad;
+  const int t1 = (padded + kBM - 1) / kBM, t2 = (padded + 2 * kBM - 1) / (2 * kBM);
+  int end = padded, n1 = t1, n2 = t2;
+  plan_scan(end, n1, n2);
+  const int start = end - padded;
+  if (e < E) {
+    pl.count[e] = total;
+    pl.off[e + 1] = end;
+    if (e == 0) pl.off[0] = 0;
+    for (int t = 0; t < t1; ++t) pl.tile[n1 - t1 + t] = make_int4(e, start + t * kBM, end, 0);
+    for (int t = 0; t < t2; ++t) pl.tile2[n2 - t2 + t] = make_int4(e, start + t * 2 * kBM, end, 0);
+    if (e == E - 1) {
+      pl.ntile[0] = n1;
+      pl.ntile[1] = n2;
+    }
+    for (int r = start + total; r < end; ++r) pl.src[r] = -1;
+  }
+  return start;
+}
+
 // One block of 512 threads (one per expert): totals, offsets, and each block's start in its experts' rows.
 __global__ void __launch_bounds__(kMoeMaxExperts) moe_offsets_kernel(int nb, int E, MoePlan pl) {
-  __shared__ int s_a[kMoeMaxExperts], s_b[kMoeMaxExperts];
   const int e = threadIdx.x;
   int total = 0;
   if (e < E)
     for (int b = 0; b < nb; ++b) total += pl.hist[(long)b * E + e];
-  const int padded = (total + kRowPad - 1) / kRowPad * kRowPad;
-  s_a[e] = e < E ? padded : 0;
-  s_b[e] = e < E ? (padded + kBM - 1) / kBM : 0;
-  __syncthreads();
-  for (int o = 1; o < kMoeMaxExperts; o <<= 1) {
-    const int a = e >= o ? s_a[e - o] : 0, b = e >= o ? s_b[e - o] : 0;
-    __syncthreads();
-    s_a[e] += a;
-    s_b[e] += b;
-    __syncthreads();
-  }
-  if (e < E) {
-    const int start = s_a[e] - padded;
-    pl.count[e] = total;
-    pl.off[e + 1] = s_a[e];
-    const int tiles = (padded + kBM - 1) / kBM;
-    for (int t = 0; t < tiles; ++t) pl.tile[s_b[e] - tiles + t] = make_int4(e, start + t * kBM, s_a[e], 0);
-    if (e == E - 1) pl.ntile[0] = s_b[e];
-    int at = start;
+  int at = plan_expert(pl, e, E, total);
+  if (e < E)
     for (int b = 0; b < nb; ++b) {
       const long h = (long)b * E + e;
       const int c = pl.hist[h];
       pl.hist[h] = at;
       at += c;
     }
-    for (int r = start + total; r < start + padded; ++r) pl.src[r] = -1;
+}
+
+// A warp gives the slots [base, base + count) their rows, in order; `next` holds its experts' next rows.
+template <typename I>
+__device__ __forceinline__ void place_slots(const I* idx, long base, int count, long P, int E, int* next,
+                                            const MoePlan& pl) {
+  const int lane = threadIdx.x & 31;
+  for (int i = lane; i < count; i += 32) {
+    const long s = base + i;
+    const int e = s < P ? slot_expert(idx, s, E) : -1;
+    const unsigned same = __match_any_sync(0xffffffffu, e);
+    const int rank = __popc(same & ((1u << lane) - 1u));
+    int row = -1;
+    if (e >= 0) row = next[e] + rank;
+    __syncwarp();
+    if (e >= 0 && rank == 0) next[e] += __popc(same);
+    __syncwarp();
+    if (s < P) {
+      pl.inv[s] = row;
+      if (row >= 0) pl.src[row] = (int)s;
+    }
   }
-  if (e == 0) pl.off[0] = 0;
+}
+
+// The whole plan in one block, for up to kPlanSmall slots: 16 warps count and place a sixteenth each.
+// (2.6 us where the three kernels take 7.4, at 96 slots.)
+constexpr int kPlanSmall = 4096;
+template <typename I>
+__global__ void __launch_bounds__(kMoeMaxExperts) moe_plan_kernel(const I* __restrict__ idx, int P, int E, MoePlan pl) {
+  extern __shared__ int s_w[];  // [16][E]
+  constexpr int W = kMoeMaxExperts / 32;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int per = ((P + W - 1) / W + 31) / 32 * 32;
+  for (int i = threadIdx.x; i < W * E; i += blockDim.x) s_w[i] = 0;
+  __syncthreads();
+  for (int i = lane; i < per; i += 32) {
+    const int s = warp * per + i;
+    if (s < P) {
+      const int e = slot_expert(idx, s, E);
+      if (e >= 0) atomicAdd(&s_w[warp * E + e], 1);
+      else if (idx[s] >= (I)E) set_status(kStatusBadArgument);
+    }
+  }
+  __syncthreads();
+  const int e = threadIdx.x;
+  int total = 0;
+  if (e < E)
+    for (int w = 0; w < W; ++w) total += s_w[w * E + e];
+  int at = plan_expert(pl, e, E, total);
+  if (e < E)
+    for (int w = 0; w < W; ++w) {
+      const int c = s_w[w * E + e];
+      s_w[w * E + e] = at;
+      at += c;
+    }
+  __syncthreads();
+  place_slots(idx, (long)warp * per, per, P, E, s_w + warp * E, pl);
 }
 
 // Each warp places 256 slots in a row: first it counts its experts, then (after the
@@ -148,21 +223,7 @@ __global__ void __launch_bounds__(kPlanThreads) moe_place_kernel(const I* __rest
     }
   }
   __syncthreads();
-  for (int i = lane; i < PER; i += 32) {
-    const long s = base + i;
-    const int e = s < P ? slot_expert(idx, s, E) : -1;
-    const unsigned same = __match_any_sync(0xffffffffu, e);
-    const int rank = __popc(same & ((1u << lane) - 1u));
-    int row = -1;
-    if (e >= 0) row = mine[e] + rank;
-    __syncwarp();
-    if (e >= 0 && rank == 0) mine[e] += __popc(same);
-    __syncwarp();
-    if (s < P) {
-      pl.inv[s] = row;
-      if (row >= 0) pl.src[row] = (int)s;
-    }
-  }
+  place_slots(idx, base, PER, P, E, mine, pl);
 }
 
 // ---------------------------------------------------------------- rows in and out
@@ -200,89 +261,150 @@ __global__ void __launch_bounds__(256)
 }
 
 // One warp per token: y = sum over its slots of gate * yp[row] (gates null: of yp[row]).
+// The rows are read once, four slots' loads in flight a lane; bound by memory.
 template <typename G>
 __global__ void __launch_bounds__(256)
     moe_combine_kernel(const bf16* __restrict__ yp, const G* __restrict__ gates, bf16* __restrict__ y, MoePlan pl,
                        int n, int C, int k) {
   const int lane = threadIdx.x & 31;
   for (int t = (blockIdx.x * blockDim.x + threadIdx.x) >> 5; t < n; t += (gridDim.x * blockDim.x) >> 5) {
-    for (int c = lane; c < C / 8; c += 32) {
+    int row = -1;
+    float gate = 1.f;
+    if (lane < k) {
+      row = pl.inv[(long)t * k + lane];
+      if (gates) gate = load_gate(gates, (long)t * k + lane);
+    }
+    for (int c0 = 0; c0 < C / 8; c0 += 32) {
+      const int c = c0 + lane;
       float acc[8] = {};
-      for (int j = 0; j < k; ++j) {
-        const long s = (long)t * k + j;
-        const int r = pl.inv[s];
-        if (r < 0) continue;
-        const float g = gates ? load_gate(gates, s) : 1.f;
-        float v[8];
-        unpack8(*reinterpret_cast<const uint4*>(yp + (long)r * C + c * 8), v);
+      for (int j = 0; j < k; j += 4) {
+        uint4 u[4];
+        float g[4];
 #pragma unroll
-        for (int i = 0; i < 8; ++i) acc[i] = fmaf(g, v[i], acc[i]);
+        for (int q = 0; q < 4; ++q) {
+          const int r = __shfl_sync(0xffffffffu, row, (j + q) & 31);
+          g[q] = __shfl_sync(0xffffffffu, gate, (j + q) & 31);
+          const bool there = j + q < k && r >= 0 && c < C / 8;
+          if (!there) g[q] = 0.f;
+          u[q] = there ? __ldcs(reinterpret_cast<const uint4*>(yp + (long)r * C) + c) : make_uint4(0, 0, 0, 0);
+        }
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+          float v[8];
+          unpack8(u[q], v);
+#pragma unroll
+          for (int i = 0; i < 8; ++i) acc[i] = fmaf(g[q], v[i], acc[i]);
+        }
       }
-      *reinterpret_cast<uint4*>(y + (long)t * C + c * 8) = pack8(acc);
+      if (c < C / 8) *(reinterpret_cast<uint4*>(y + (long)t * C) + c) = pack8(acc);
     }
   }
 }
 
-// One warp per row: u = gate * dy[token], d(gate) = dy[token] . yp[row].  u is rounded to
-// bf16: it is the tensor cores' operand in three products.
+// A block of 64 rows (one expert's) per CTA, 8 rows a warp: u = gate * dy[token],
+// d(gate) = dy[token] . yp[row], and the block's column sums of u (as rounded), from one
+// pass over the rows.  u is rounded to bf16: it is the tensor cores' operand in two products.
+constexpr int kGradCols = 1024;  // columns at a time: 4 x 16 bytes a lane
 template <typename G>
 __global__ void __launch_bounds__(256)
     moe_grad_rows_kernel(const bf16* __restrict__ dy, const bf16* __restrict__ yp, const G* __restrict__ gates,
-                         bf16* __restrict__ u, G* __restrict__ dgates, MoePlan pl, int E, int C, int k) {
-  const int lane = threadIdx.x & 31;
-  const int rows = pl.off[E];
-  for (int r = (blockIdx.x * blockDim.x + threadIdx.x) >> 5; r < rows; r += (gridDim.x * blockDim.x) >> 5) {
-    const int s = pl.src[r];
-    uint4* dst = reinterpret_cast<uint4*>(u + (long)r * C);
-    if (s < 0) {
-      for (int c = lane; c < C / 8; c += 32) dst[c] = make_uint4(0, 0, 0, 0);
-      continue;
-    }
-    const float g = load_gate(gates, s);
-    const uint4* d = reinterpret_cast<const uint4*>(dy + (long)(s / k) * C);
-    const uint4* o = reinterpret_cast<const uint4*>(yp + (long)r * C);
-    float dot = 0.f;
-    for (int c = lane; c < C / 8; c += 32) {
-      float a[8], b[8];
-      unpack8(d[c], a);
-      unpack8(o[c], b);
-#pragma unroll
+                         bf16* __restrict__ u, G* __restrict__ dgates, float* __restrict__ sums, MoePlan pl, int E,
+                         int C, int k) {
+  __shared__ float s_sum[8][kGradCols];
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int blocks = pl.off[E] / kRowPad;
+  for (int b = blockIdx.x; b < blocks; b += gridDim.x) {
+    const int r0 = b * kRowPad + warp * 8;
+    const int slot = lane < 8 ? pl.src[r0 + lane] : -1;
+    const float gate = slot >= 0 ? load_gate(gates, slot) : 0.f;
+    float dot = 0.f;  // lane i: row i's
+    for (int c0 = 0; c0 < C; c0 += kGradCols) {
+      float acc[4][8] = {};
+#pragma unroll 2
       for (int i = 0; i < 8; ++i) {
-        dot = fmaf(a[i], b[i], dot);
-        a[i] *= g;
-      }
-      dst[c] = pack8(a);
-    }
+        const int s = __shfl_sync(0xffffffffu, slot, i);
+        const float g = __shfl_sync(0xffffffffu, gate, i);
+        const uint4* d = reinterpret_cast<const uint4*>(dy + (long)(max(s, 0) / k) * C + c0);
+        const uint4* o = reinterpret_cast<const uint4*>(yp + (long)(r0 + i) * C + c0);
+        uint4* dst = reinterpret_cast<uint4*>(u + (long)(r0 + i) * C + c0);
+        uint4 dv[4], ov[4];
 #pragma unroll
-    for (int o2 = 16; o2; o2 >>= 1) dot += __shfl_xor_sync(0xffffffffu, dot, o2);
-    if (lane == 0) store_gate(dgates, s, dot);
+        for (int q = 0; q < 4; ++q) {
+          const int c = lane + 32 * q;
+          const bool there = s >= 0 && c0 + c * 8 < C;
+          dv[q] = there ? d[c] : make_uint4(0, 0, 0, 0);
+          ov[q] = there ? __ldcs(o + c) : make_uint4(0, 0, 0, 0);
+        }
+        float p = 0.f;
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+          const int c = lane + 32 * q;
+          float a[8], w[8];
+          unpack8(dv[q], a);
+          unpack8(ov[q], w);
+#pragma unroll
+          for (int x = 0; x < 8; ++x) {
+            p = fmaf(a[x], w[x], p);
+            a[x] *= g;
+          }
+          if (s < 0) {
+#pragma unroll
+            for (int x = 0; x < 8; ++x) a[x] = 0.f;
+          }
+          const uint4 packed = pack8(a);
+          if (c0 + c * 8 < C) dst[c] = packed;
+          unpack8(packed, a);
+#pragma unroll
+          for (int x = 0; x < 8; ++x) acc[q][x] += a[x];
+        }
+#pragma unroll
+        for (int o2 = 16; o2; o2 >>= 1) p += __shfl_xor_sync(0xffffffffu, p, o2);
+        if (lane == i) dot += p;
+      }
+      if (sums != nullptr) {
+#pragma unroll
+        for (int q = 0; q < 4; ++q)
+#pragma unroll
+          for (int x = 0; x < 8; x += 4)
+            *reinterpret_cast<float4*>(&s_sum[warp][(lane + 32 * q) * 8 + x]) =
+                make_float4(acc[q][x], acc[q][x + 1], acc[q][x + 2], acc[q][x + 3]);
+        __syncthreads();
+        for (int c = threadIdx.x; c < kGradCols && c0 + c < C; c += 256) {
+          float t = 0.f;
+#pragma unroll
+          for (int w = 0; w < 8; ++w) t += s_sum[w][c];
+          sums[(long)b * C + c0 + c] = t;
+        }
+        __syncthreads();
+      }
+    }
+    if (lane < 8 && slot >= 0) store_gate(dgates, slot, dot);
   }
 }
 
-// out[e, c] = sum over the expert's rows of g[r, c]: one block per expert and 64 columns,
-// 32 row lanes x 8 column vectors, joined in a fixed order.
+// out[e, c] = sum of the partial column sums of the expert's blocks of `rows` rows: one CTA per expert and
+// 64 columns, 16 block lanes x 16 column vectors, joined in a fixed order.
 template <typename O>
 __global__ void __launch_bounds__(256)
-    moe_col_sums_kernel(const bf16* __restrict__ g, O* __restrict__ out, MoePlan pl, int N) {
-  __shared__ float s_sum[32][65];
+    moe_join_sums_kernel(const float* __restrict__ part, O* __restrict__ out, MoePlan pl, int N, int rows) {
+  __shared__ float s_sum[16][68];
   const int e = blockIdx.y, c0 = blockIdx.x * 64;
-  const int tx = threadIdx.x & 7, ty = threadIdx.x >> 3;
-  const int lo = pl.off[e], hi = lo + pl.count[e];
-  const int c = c0 + tx * 8;
-  float acc[8] = {};
+  const int tx = threadIdx.x & 15, ty = threadIdx.x >> 4;
+  const int lo = pl.off[e] / rows, hi = pl.off[e + 1] / rows;
+  const int c = c0 + tx * 4;
+  float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
   if (c < N)
-    for (int r = lo + ty; r < hi; r += 32) {
-      float v[8];
-      unpack8(*reinterpret_cast<const uint4*>(g + (long)r * N + c), v);
-#pragma unroll
-      for (int i = 0; i < 8; ++i) acc[i] += v[i];
+#pragma unroll 4
+    for (int r = lo + ty; r < hi; r += 16) {
+      const float4 v = *reinterpret_cast<const float4*>(part + (long)r * N + c);
+      acc.x += v.x; acc.y += v.y; acc.z += v.z; acc.w += v.w;
     }
-#pragma unroll
-  for (int i = 0; i < 8; ++i) s_sum[ty][tx * 8 + i] = acc[i];
+  *reinterpret_cast<float4*>(&s_sum[ty][tx * 4]) = acc;
   __syncthreads();
   if (threadIdx.x < 64 && c0 + threadIdx.x < N) {
     float s = 0.f;
-    for (int r = 0; r < 32; ++r) s += s_sum[r][threadIdx.x];
+#pragma unroll
+    for (int r = 0; r < 16; ++r) s += s_sum[r][threadIdx.x];
     store_gate(out, (long)e * N + c0 + threadIdx.x, s);
   }
 }
@@ -308,6 +430,7 @@ struct MoeGemmArgs {
   const bf16* bias;    // [E, N] or null
   const bf16* aux_in;  // [R, N]
   int save_aux;
+  float* sums;         // MOE_DGELU: [R / 32, N] column sums of each 32 rows of the output, or null
 };
 
 // Where unit u of the grid lies: expert, first row and column of the tile, end of its rows, first row
@@ -374,6 +497,22 @@ __device__ __forceinline__ void moe_epi_chunk(const MoeGemmArgs& a, const CUtens
   }
   fence_proxy_async_smem();
   __syncwarp();
+  if (a.epi == MOE_DGELU && a.sums != nullptr) {
+    // lane: two columns of every other row, from the slab (as rounded); the two row halves meet in lanes 0-15
+    const int cp = lane & 15, h = lane >> 4;
+    float s0 = 0.f, s1 = 0.f;
+#pragma unroll
+    for (int i = 0; i < 16; ++i) {
+      const int r = 2 * i + h;
+      const uint32_t w = *reinterpret_cast<const uint32_t*>(slab + r * 64 + slab_unit_bf16(r, cp >> 2) * 16 + (cp & 3) * 4);
+      s0 += __uint_as_float(w << 16);
+      s1 += __uint_as_float(w & 0xffff0000u);
+    }
+    s0 += __shfl_xor_sync(0xffffffffu, s0, 16);
+    s1 += __shfl_xor_sync(0xffffffffu, s1, 16);
+    if (h == 0 && col + 2 * cp < a.N)
+      *reinterpret_cast<float2*>(a.sums + (long)(row0 >> 5) * a.N + col + 2 * cp) = make_float2(s0, s1);
+  }
   if (lane == 0) {
     if (dw) {
       tma_store_3d(tmOut, slab, col, row0, e);
@@ -566,6 +705,225 @@ __global__ void __maxnreg__(DTB_CORESIDENT_MAXNREG)
   }
 }
 
+// -------------------------------------------------------------------------
+// 2-SM variant: a cluster of two CTAs computes a 256x256 tile (tcgen05 cta_group::2).
+// CTA r loads its 128 rows of A and its 128 columns of B (32 KB a k-block where the 1-SM
+// 128x256 tile loads 48 KB, for half the output), the leader issues the MMAs of both.
+// Barriers as in the dense pair GEMM (gemm.cu): full (leader; both CTAs' bytes), empty and
+// tile-full (both, by the leader's commit), tile-empty (leader; both epilogues), done.
+// No load is multicast.
+__device__ __forceinline__ void tma_load_3d_pair(const CUtensorMap* map, void* dst, uint32_t leader_bar, int x, int y,
+                                                 int z) {
+  asm volatile(
+      "cp.async.bulk.tensor.3d.cta_group::2.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5}], [%2];"
+      ::"r"(smem_u32(dst)), "l"(reinterpret_cast<uint64_t>(map)), "r"(leader_bar), "r"(x), "r"(y), "r"(z)
+      : "memory");
+}
+
+struct MoePairCfg {
+  static constexpr int A_BYTES = kBM * kBK * 2;
+  static constexpr int B_BYTES = 128 * kBK * 2;
+  static constexpr int STAGE_BYTES = A_BYTES + B_BYTES;
+  static constexpr int STAGES = 5;
+  static constexpr int TMEM_COLS = 512;
+  static constexpr int EPI_BYTES = kEpiWarps * 2 * kEpiSlab;
+  static constexpr int SMEM_BYTES = STAGES * STAGE_BYTES + EPI_BYTES + 1024 /*align*/ + 256 /*barriers*/;
+};
+
+template <int MODE>
+__global__ void __maxnreg__(DTB_CORESIDENT_MAXNREG)
+    moe_gemm2_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmB,
+                     const __grid_constant__ CUtensorMap tmOut, const __grid_constant__ CUtensorMap tmAux,
+                     MoeGemmArgs args) {
+  using Cfg = MoePairCfg;
+  constexpr bool A_MN = MODE == MOE_DW, B_MN = MODE != MOE_DX;
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  uint8_t* epi_smem = smem + Cfg::STAGES * Cfg::STAGE_BYTES;
+  uint64_t* full_bar = reinterpret_cast<uint64_t*>(epi_smem + Cfg::EPI_BYTES);
+  uint64_t* empty_bar = full_bar + Cfg::STAGES;
+  uint64_t* tfull_bar = empty_bar + Cfg::STAGES;  // [2]
+  uint64_t* tempty_bar = tfull_bar + 2;           // [2]
+  uint64_t* done_bar = tempty_bar + 2;
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(done_bar + 1);
+  volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
+
+  const int warp = threadIdx.x >> 5;
+  const int lane = threadIdx.x & 31;
+  const uint32_t rank = cluster_ctarank();
+  const bool leader = rank == 0;
+
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < Cfg::STAGES; ++s) {
+      mbar_init(&full_bar[s], 1);
+      mbar_init(&empty_bar[s], 1);
+    }
+    for (int b = 0; b < 2; ++b) {
+      mbar_init(&tfull_bar[b], 1);
+      mbar_init(&tempty_bar[b], 2 * kEpiWarps);
+    }
+    mbar_init(done_bar, 1);
+    *abort_flag = 0;
+    fence_barrier_init_cluster();
+    tma_prefetch_desc(&tmA);
+    tma_prefetch_desc(&tmB);
+  }
+  if (warp == 1) tmem_alloc_pair(tmem_slot, Cfg::TMEM_COLS);
+  tc_fence_before();
+  cluster_sync_all();  // both CTAs' barriers initialised and TMEM allocated
+  tc_fence_after();
+  const uint32_t tmem_base = *tmem_slot;
+
+  const int nt = (args.N + 255) / 256;
+  const int mt = MODE == MOE_DW ? (args.M + 255) / 256 : __ldg(args.ntile);
+  const int units = MODE == MOE_DW ? args.E * mt * nt : mt * nt;
+  const int pair = blockIdx.x >> 1, npairs = gridDim.x >> 1;
+
+  if (warp == 0) {
+    if (lane == 0) {
+      // ------------------------------------------------------------ TMA producer (both CTAs)
+      const uint32_t lead_full0 = mapa_shared(&full_bar[0], 0);
+      int stage = 0;
+      uint32_t phase = 0;
+      bool ok = true;
+      for (int u = pair; u < units && ok; u += npairs) {
+        const MoeUnit q = moe_unit<MODE, 256, 256>(args, u, mt, nt);
+        const int m0 = q.m0 + (int)rank * 128, n0 = q.n0 + (int)rank * 128;
+        for (int kb = 0; kb < q.kb; ++kb) {
+          if (!mbar_wait(&empty_bar[stage], phase ^ 1, abort_flag)) { ok = false; break; }
+          uint8_t* sA = smem + stage * Cfg::STAGE_BYTES;
+          uint8_t* sB = sA + Cfg::A_BYTES;
+          const uint32_t fb = lead_full0 + (uint32_t)(stage * sizeof(uint64_t));
+          if (leader) mbar_arrive_expect_tx(&full_bar[stage], 2 * Cfg::STAGE_BYTES);
+          if (MODE == MOE_DW) {
+            const int r0 = q.r0 + kb * kBK;
+            tma_load_2d_pair(&tmA, sA, fb, m0, r0);
+            tma_load_2d_pair(&tmA, sA + 8192, fb, m0 + 64, r0);
+            tma_load_2d_pair(&tmB, sB, fb, n0, r0);
+            tma_load_2d_pair(&tmB, sB + 8192, fb, n0 + 64, r0);
+          } else {
+            const int k0 = kb * kBK;
+            tma_load_2d_pair(&tmA, sA, fb, k0, m0);
+            if (MODE == MOE_DX) {
+              tma_load_3d_pair(&tmB, sB, fb, k0, n0, q.e);
+            } else {
+              tma_load_3d_pair(&tmB, sB, fb, n0, k0, q.e);
+              tma_load_3d_pair(&tmB, sB + 8192, fb, n0 + 64, k0, q.e);
+            }
+          }
+          if (++stage == Cfg::STAGES) { stage = 0; phase ^= 1; }
+        }
+      }
+    }
+  } else if (warp == 1) {
+    if (lane == 0 && leader) {
+      // ------------------------------------------------------------ MMA issuer (leader only)
+      constexpr uint32_t idesc = make_idesc_bf16(256, 256, A_MN, B_MN);
+      int stage = 0;
+      uint32_t phase = 0;
+      int ab = 0;
+      uint32_t aphase = 0;
+      bool ok = true;
+      for (int u = pair; u < units && ok; u += npairs) {
+        const MoeUnit q = moe_unit<MODE, 256, 256>(args, u, mt, nt);
+        if (q.kb == 0) continue;  // an expert without rows: the epilogue writes zeros
+        if (!mbar_wait(&tempty_bar[ab], aphase ^ 1, abort_flag)) break;
+        tc_fence_after();
+        const uint32_t d_tmem = tmem_base + (uint32_t)(ab * 256);
+        for (int kb = 0; kb < q.kb; ++kb) {
+          if (!mbar_wait(&full_bar[stage], phase, abort_flag)) { ok = false; break; }
+          tc_fence_after();
+          const uint32_t aBase = smem_u32(smem + stage * Cfg::STAGE_BYTES);
+          const uint32_t bBase = aBase + Cfg::A_BYTES;
+#pragma unroll
+          for (int kk = 0; kk < kBK / 16; ++kk) {
+            const uint64_t ad = A_MN ? make_sw128_desc(aBase + kk * 2048, 8192, 1024)
+                                     : make_sw128_desc(aBase + kk * 32, 16, 1024);
+            const uint64_t bd = B_MN ? make_sw128_desc(bBase + kk * 2048, 8192, 1024)
+                                     : make_sw128_desc(bBase + kk * 32, 16, 1024);
+            tc_mma_f16_pair(d_tmem, ad, bd, idesc, (kb > 0 || kk > 0) ? 1u : 0u);
+          }
+          tc_commit_pair(&empty_bar[stage], 0x3);
+          if (++stage == Cfg::STAGES) { stage = 0; phase ^= 1; }
+        }
+        if (!ok) break;
+        tc_commit_pair(&tfull_bar[ab], 0x3);
+        if (++ab == 2) { ab = 0; aphase ^= 1; }
+      }
+    }
+  } else {
+    // -------------------------------------------------------------- epilogue (both CTAs)
+    const int ew = warp - 2;
+    const int q4 = warp & 3;
+    const int half = ew >> 2;
+    uint8_t* slab = epi_smem + ew * 2 * kEpiSlab;
+    const uint32_t lead_tempty0 = mapa_shared(&tempty_bar[0], 0);
+    uint32_t ck = 0;
+    int ab = 0;
+    uint32_t aphase = 0;
+    for (int u = pair; u < units; u += npairs) {
+      const MoeUnit q = moe_unit<MODE, 256, 256>(args, u, mt, nt);
+      if (q.kb > 0) {
+        if (!mbar_wait(&tfull_bar[ab], aphase, abort_flag)) break;
+        tc_fence_after();
+      }
+      const int row0 = q.m0 + (int)rank * 128 + q4 * 32;
+      const uint32_t tbase = tmem_base + ((uint32_t)(q4 * 32) << 16) + (uint32_t)(ab * 256);
+      const int c_begin = half * 128, c_end = c_begin + 128;
+      if (row0 < q.row_end) {
+#pragma unroll 1
+        for (int c = c_begin; c < c_end; c += 64) {
+          if (q.n0 + c >= args.N) break;  // warp-uniform
+          uint32_t r0[32], r1[32];
+          if (q.kb > 0) {
+            tmem_ld32_issue(tbase + c, r0);
+            tmem_ld32_issue(tbase + c + 32, r1);
+            tmem_wait_ld();
+          } else {
+#pragma unroll
+            for (int j = 0; j < 32; ++j) r0[j] = r1[j] = 0u;
+          }
+          float v[32];
+#pragma unroll
+          for (int j = 0; j < 32; ++j) v[j] = __uint_as_float(r0[j]);
+          epi_slab_acquire(lane, true);
+          moe_epi_chunk(args, &tmOut, &tmAux, slab + (ck & 1) * kEpiSlab, lane, row0, q.n0 + c, q.e, MODE == MOE_DW, v);
+          ++ck;
+          if (q.n0 + c + 32 < args.N) {
+#pragma unroll
+            for (int j = 0; j < 32; ++j) v[j] = __uint_as_float(r1[j]);
+            epi_slab_acquire(lane, true);
+            moe_epi_chunk(args, &tmOut, &tmAux, slab + (ck & 1) * kEpiSlab, lane, row0, q.n0 + c + 32, q.e,
+                          MODE == MOE_DW, v);
+            ++ck;
+          }
+        }
+      }
+      if (q.kb > 0) {
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive_cluster(lead_tempty0 + (uint32_t)(ab * sizeof(uint64_t)));
+        if (++ab == 2) { ab = 0; aphase ^= 1; }
+      }
+    }
+    if (lane == 0) bulk_wait0();
+    __syncwarp();
+  }
+
+  // Neither CTA releases the pair's TMEM before the other has finished with it.
+  tc_fence_before();
+  __syncthreads();
+  if (threadIdx.x == 0) {
+    mbar_arrive_cluster(mapa_shared(done_bar, rank ^ 1));
+    mbar_wait(done_bar, 0, abort_flag);
+  }
+  __syncthreads();
+  if (warp == 1) {
+    tc_fence_after();
+    tmem_dealloc_pair(tmem_base, Cfg::TMEM_COLS);
+  }
+}
+
 // ------------------------------------------------------------------ host
 // 3-D bf16 operand map over [depth, rows, cols], 128B swizzle: a box never leaves its expert's matrix
 // (rows and columns past its end read as zeros).
@@ -597,17 +955,69 @@ static void launch_moe(const CUtensorMap& ta, const CUtensorMap& tb, const CUten
   C10_CUDA_KERNEL_LAUNCH_CHECK();
 }
 
+// Pairs that can be resident at once.
+static int moe_max_pairs() {
+  static int n = -1;
+  if (n < 0) {
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(2 * (num_sms() / 2), 1, 1);
+    cfg.blockDim = dim3(kThreads, 1, 1);
+    cfg.dynamicSmemBytes = MoePairCfg::SMEM_BYTES;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim.x = 2;
+    attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    cudaFuncSetAttribute(moe_gemm2_kernel<MOE_FWD>, cudaFuncAttributeMaxDynamicSharedMemorySize, MoePairCfg::SMEM_BYTES);
+    int c = 0;
+    if (cudaOccupancyMaxActiveClusters(&c, moe_gemm2_kernel<MOE_FWD>, &cfg) != cudaSuccess || c <= 0) {
+      cudaGetLastError();
+      c = num_sms() / 2;
+    }
+    n = c;
+  }
+  return n;
+}
+
+template <int MODE>
+static void launch_moe2(const CUtensorMap& ta, const CUtensorMap& tb, const CUtensorMap& to, const CUtensorMap& tx,
+                        const MoeGemmArgs& a, long units, cudaStream_t st) {
+  static bool attr_set = false;
+  auto kern = moe_gemm2_kernel<MODE>;
+  if (!attr_set) {
+    cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, MoePairCfg::SMEM_BYTES);
+    attr_set = true;
+  }
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(2 * (unsigned)std::min<long>(units, moe_max_pairs()), 1, 1);
+  cfg.blockDim = dim3(kThreads, 1, 1);
+  cfg.dynamicSmemBytes = MoePairCfg::SMEM_BYTES;
+  cfg.stream = st;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = 2;
+  attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  C10_CUDA_CHECK(cudaLaunchKernelEx(&cfg, kern, ta, tb, to, tx, a));
+  count_launch();
+}
+
 struct MoeSizes {
   long n, k, P, E, R;  // tokens, slots a token, slots, experts, most padded rows
 };
 
 // rows [R, N] = rows [R, K] . W_e (MOE_FWD, w [E, K, N]) or . W_e^T (MOE_DX, w [E, N, K])
 static void moe_rows_gemm(int mode, const bf16* a, const bf16* w, bf16* out, int N, int K, int epi, const bf16* bias,
-                          bf16* aux, const MoePlan& pl, const MoeSizes& z, cudaStream_t st) {
+                          bf16* aux, float* sums, const MoePlan& pl, const MoeSizes& z, cudaStream_t st) {
+  // 256-row pair tiles once the experts have 256 rows on average (below, half of a tile is padding)
+  const bool pair = N > 128 && z.P >= 256 * z.E;
   MoeGemmArgs g{};
   g.off = pl.off;
-  g.tile = pl.tile;
-  g.ntile = pl.ntile;
+  g.tile = pair ? pl.tile2 : pl.tile;
+  g.ntile = pl.ntile + (pair ? 1 : 0);
+  g.sums = sums;
   g.E = (int)z.E;
   g.N = N;
   g.K = K;
@@ -618,10 +1028,15 @@ static void moe_rows_gemm(int mode, const bf16* a, const bf16* w, bf16* out, int
   g.save_aux = epi == MOE_GELU && aux != nullptr;
   const int bn = N <= 128 ? 128 : 256;
   const CUtensorMap ta = make_map(a, z.R, K, K, 64, kBM);
-  const CUtensorMap tb = mode == MOE_FWD ? make_map3(w, z.E, K, N, 64, 64) : make_map3(w, z.E, N, K, 64, bn);
+  const CUtensorMap tb = mode == MOE_FWD ? make_map3(w, z.E, K, N, 64, 64) : make_map3(w, z.E, N, K, 64, pair ? 128 : bn);
   const CUtensorMap to = make_store_map(out, false, z.R, N, N);
   const CUtensorMap tx = g.save_aux ? make_store_map(aux, false, z.R, N, N) : to;
   const long units = moe_max_tiles(z.P, z.E) * ((N + bn - 1) / bn);
+  if (pair) {
+    if (mode == MOE_FWD) launch_moe2<MOE_FWD>(ta, tb, to, tx, g, units, st);
+    else launch_moe2<MOE_DX>(ta, tb, to, tx, g, units, st);
+    return;
+  }
   if (mode == MOE_FWD) {
     if (bn == 256) launch_moe<256, MOE_FWD>(ta, tb, to, tx, g, units, st);
     else launch_moe<128, MOE_FWD>(ta, tb, to, tx, g, units, st);
@@ -645,6 +1060,10 @@ static void moe_weight_gemm(const bf16* a, const bf16* b, at::Tensor& out, int M
   const CUtensorMap ta = make_map(a, z.R, M, M, 64, 64);
   const CUtensorMap tb = make_map(b, z.R, N, N, 64, 64);
   const CUtensorMap to = make_store_map(out.data_ptr(), f32, M, N, N, z.E);
+  if (M > 128 && N > 128) {
+    launch_moe2<MOE_DW>(ta, tb, to, to, g, z.E * ((M + 255) / 256) * ((N + 255) / 256), st);
+    return;
+  }
   const long units = z.E * ((M + kBM - 1) / kBM) * ((N + bn - 1) / bn);
   if (bn == 256) launch_moe<256, MOE_DW>(ta, tb, to, to, g, units, st);
   else launch_moe<128, MOE_DW>(ta, tb, to, to, g, units, st);
@@ -652,20 +1071,23 @@ static void moe_weight_gemm(const bf16* a, const bf16* b, at::Tensor& out, int M
 
 static int warp_grid(long rows) { return (int)std::max<long>(1, std::min<long>((rows + 7) / 8, 148L * 8)); }
 
-static void moe_build_plan(const at::Tensor& idx, const MoePlan& pl, const MoeSizes& z, cudaStream_t st) {
+template <typename I>
+static void moe_build_plan_of(const I* idx, const MoePlan& pl, const MoeSizes& z, cudaStream_t st) {
   const int nb = (int)plan_blocks(z.P), E = (int)z.E;
-  if (idx.scalar_type() == at::kInt) {
-    moe_hist_kernel<int><<<nb, kPlanThreads, E * 4, st>>>(idx.data_ptr<int>(), z.P, E, pl);
-    moe_offsets_kernel<<<1, kMoeMaxExperts, 0, st>>>(nb, E, pl);
-    moe_place_kernel<int><<<nb, kPlanThreads, 8 * E * 4, st>>>(idx.data_ptr<int>(), z.P, E, pl);
+  if (z.P <= kPlanSmall) {
+    moe_plan_kernel<I><<<1, kMoeMaxExperts, kMoeMaxExperts / 32 * E * 4, st>>>(idx, (int)z.P, E, pl);
+    count_launch();
   } else {
-    const long* p = reinterpret_cast<const long*>(idx.data_ptr<int64_t>());
-    moe_hist_kernel<long><<<nb, kPlanThreads, E * 4, st>>>(p, z.P, E, pl);
+    moe_hist_kernel<I><<<nb, kPlanThreads, E * 4, st>>>(idx, z.P, E, pl);
     moe_offsets_kernel<<<1, kMoeMaxExperts, 0, st>>>(nb, E, pl);
-    moe_place_kernel<long><<<nb, kPlanThreads, 8 * E * 4, st>>>(p, z.P, E, pl);
+    moe_place_kernel<I><<<nb, kPlanThreads, 8 * E * 4, st>>>(idx, z.P, E, pl);
+    count_launch(3);
   }
-  count_launch(3);
   C10_CUDA_KERNEL_LAUNCH_CHECK();
+}
+static void moe_build_plan(const at::Tensor& idx, const MoePlan& pl, const MoeSizes& z, cudaStream_t st) {
+  if (idx.scalar_type() == at::kInt) moe_build_plan_of(idx.data_ptr<int>(), pl, z, st);
+  else moe_build_plan_of(reinterpret_cast<const long*>(idx.data_ptr<int64_t>()), pl, z, st);
 }
 
 static const bf16* bptr(const at::Tensor& t) { return reinterpret_cast<const bf16*>(t.data_ptr()); }
@@ -745,9 +1167,9 @@ std::vector<at::Tensor> experts_fwd(at::Tensor x, at::Tensor w1, std::optional<a
   if (save) pre = at::empty({z.R, H}, x.options());
   auto yp = at::empty({z.R, Co}, x.options());
   moe_rows_gemm(MOE_FWD, bptr(xp), bptr(w1), bptr_mut(act), (int)H, (int)C, MOE_GELU, bptr_opt(b1),
-                save ? bptr_mut(pre) : nullptr, pl, z, st);
-  moe_rows_gemm(MOE_FWD, bptr(act), bptr(w2), bptr_mut(yp), (int)Co, (int)H, MOE_PLAIN, bptr_opt(b2), nullptr, pl, z,
-                st);
+                save ? bptr_mut(pre) : nullptr, nullptr, pl, z, st);
+  moe_rows_gemm(MOE_FWD, bptr(act), bptr(w2), bptr_mut(yp), (int)Co, (int)H, MOE_PLAIN, bptr_opt(b2), nullptr, nullptr, pl,
+                z, st);
   if (gates.scalar_type() == at::kFloat)
     moe_combine_kernel<float><<<warp_grid(z.n), 256, 0, st>>>(bptr(yp), gates.data_ptr<float>(), bptr_mut(y), pl,
                                                              (int)z.n, (int)Co, (int)z.k);
@@ -802,30 +1224,36 @@ std::vector<at::Tensor> experts_bwd(at::Tensor dy, at::Tensor x, at::Tensor w1, 
   const MoePlan pl = plan_views(plan.data_ptr<int>(), z.P, z.E);
   const bool gf = gates.scalar_type() == at::kFloat;
   auto u = at::empty({z.R, Co}, x.options());
+  const bool has1 = db1 && db1->defined(), has2 = db2 && db2->defined();
+  at::Tensor s1, s2;  // column sums of blocks of rows
+  if (has1) s1 = at::empty({z.R / 32, H}, x.options().dtype(at::kFloat));
+  if (has2) s2 = at::empty({z.R / kRowPad, Co}, x.options().dtype(at::kFloat));
+  float* p1 = has1 ? s1.data_ptr<float>() : nullptr;
+  float* p2 = has2 ? s2.data_ptr<float>() : nullptr;
+  const int gr = (int)std::min<long>(z.R / kRowPad, 148L * 4);
   if (gf)
-    moe_grad_rows_kernel<float><<<warp_grid(z.R), 256, 0, st>>>(bptr(dy), bptr(yp), gates.data_ptr<float>(),
-                                                               bptr_mut(u), dgates.data_ptr<float>(), pl, (int)z.E,
-                                                               (int)Co, (int)z.k);
+    moe_grad_rows_kernel<float><<<gr, 256, 0, st>>>(bptr(dy), bptr(yp), gates.data_ptr<float>(), bptr_mut(u),
+                                                   dgates.data_ptr<float>(), p2, pl, (int)z.E, (int)Co, (int)z.k);
   else
-    moe_grad_rows_kernel<bf16><<<warp_grid(z.R), 256, 0, st>>>(bptr(dy), bptr(yp), bptr(gates), bptr_mut(u),
-                                                              bptr_mut(dgates), pl, (int)z.E, (int)Co, (int)z.k);
+    moe_grad_rows_kernel<bf16><<<gr, 256, 0, st>>>(bptr(dy), bptr(yp), bptr(gates), bptr_mut(u), bptr_mut(dgates), p2,
+                                                  pl, (int)z.E, (int)Co, (int)z.k);
   count_launch();
-  const auto col_sums = [&](const at::Tensor& g, const std::optional<at::Tensor>& out, long N) {
-    if (!out || !out->defined()) return;
+  const auto join = [&](const float* part, const at::Tensor& out, long N, int rows) {
     const dim3 grid((unsigned)((N + 63) / 64), (unsigned)z.E);
-    if (wt == at::kFloat) moe_col_sums_kernel<float><<<grid, 256, 0, st>>>(bptr(g), out->data_ptr<float>(), pl, (int)N);
-    else moe_col_sums_kernel<bf16><<<grid, 256, 0, st>>>(bptr(g), bptr_mut(*out), pl, (int)N);
+    if (wt == at::kFloat) moe_join_sums_kernel<float><<<grid, 256, 0, st>>>(part, out.data_ptr<float>(), pl, (int)N, rows);
+    else moe_join_sums_kernel<bf16><<<grid, 256, 0, st>>>(part, bptr_mut(out), pl, (int)N, rows);
     count_launch();
   };
   auto dpre = at::empty({z.R, H}, x.options());
-  moe_rows_gemm(MOE_DX, bptr(u), bptr(w2), bptr_mut(dpre), (int)H, (int)Co, MOE_DGELU, nullptr, bptr_mut(pre), pl, z,
-                st);
+  moe_rows_gemm(MOE_DX, bptr(u), bptr(w2), bptr_mut(dpre), (int)H, (int)Co, MOE_DGELU, nullptr, bptr_mut(pre), p1, pl,
+                z, st);
   moe_weight_gemm(bptr(act), bptr(u), dw2, (int)H, (int)Co, pl, z, st);
-  col_sums(u, db2, Co);
+  if (has2) join(p2, *db2, Co, kRowPad);
   auto dxp = at::empty({z.R, C}, x.options());
-  moe_rows_gemm(MOE_DX, bptr(dpre), bptr(w1), bptr_mut(dxp), (int)C, (int)H, MOE_PLAIN, nullptr, nullptr, pl, z, st);
+  moe_rows_gemm(MOE_DX, bptr(dpre), bptr(w1), bptr_mut(dxp), (int)C, (int)H, MOE_PLAIN, nullptr, nullptr, nullptr, pl,
+                z, st);
   moe_weight_gemm(bptr(xp), bptr(dpre), dw1, (int)C, (int)H, pl, z, st);
-  col_sums(dpre, db1, H);
+  if (has1) join(p1, *db1, H, 32);
   moe_combine_kernel<float><<<warp_grid(z.n), 256, 0, st>>>(bptr(dxp), nullptr, bptr_mut(dx), pl, (int)z.n, (int)C,
                                                            (int)z.k);
   count_launch();
