@@ -304,22 +304,25 @@ __global__ void __launch_bounds__(256)
 // A block of 64 rows (one expert's) per CTA, 8 rows a warp: u = gate * dy[token],
 // d(gate) = dy[token] . yp[row], and the block's column sums of u (as rounded), from one
 // pass over the rows.  u is rounded to bf16: it is the tensor cores' operand in two products.
-constexpr int kGradCols = 1024;  // columns at a time: 4 x 16 bytes a lane
-template <typename G>
+// Q x 16 bytes a lane at a time, 256 Q columns.
+template <typename G, int Q>
 __global__ void __launch_bounds__(256)
     moe_grad_rows_kernel(const bf16* __restrict__ dy, const bf16* __restrict__ yp, const G* __restrict__ gates,
                          bf16* __restrict__ u, G* __restrict__ dgates, float* __restrict__ sums, MoePlan pl, int E,
-                         int C, int k) {
+                         int C, int k, long P) {
+  constexpr int kGradCols = 256 * Q;
   __shared__ float s_sum[8][kGradCols];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int blocks = pl.off[E] / kRowPad;
+  for (long s = (long)blockIdx.x * blockDim.x + threadIdx.x; s < P; s += (long)gridDim.x * blockDim.x)
+    if (pl.inv[s] < 0) store_gate(dgates, s, 0.f);
   for (int b = blockIdx.x; b < blocks; b += gridDim.x) {
     const int r0 = b * kRowPad + warp * 8;
     const int slot = lane < 8 ? pl.src[r0 + lane] : -1;
     const float gate = slot >= 0 ? load_gate(gates, slot) : 0.f;
     float dot = 0.f;  // lane i: row i's
     for (int c0 = 0; c0 < C; c0 += kGradCols) {
-      float acc[4][8] = {};
+      float acc[Q][8] = {};
 #pragma unroll 2
       for (int i = 0; i < 8; ++i) {
         const int s = __shfl_sync(0xffffffffu, slot, i);
@@ -327,9 +330,9 @@ __global__ void __launch_bounds__(256)
         const uint4* d = reinterpret_cast<const uint4*>(dy + (long)(max(s, 0) / k) * C + c0);
         const uint4* o = reinterpret_cast<const uint4*>(yp + (long)(r0 + i) * C + c0);
         uint4* dst = reinterpret_cast<uint4*>(u + (long)(r0 + i) * C + c0);
-        uint4 dv[4], ov[4];
+        uint4 dv[Q], ov[Q];
 #pragma unroll
-        for (int q = 0; q < 4; ++q) {
+        for (int q = 0; q < Q; ++q) {
           const int c = lane + 32 * q;
           const bool there = s >= 0 && c0 + c * 8 < C;
           dv[q] = there ? d[c] : make_uint4(0, 0, 0, 0);
@@ -337,7 +340,7 @@ __global__ void __launch_bounds__(256)
         }
         float p = 0.f;
 #pragma unroll
-        for (int q = 0; q < 4; ++q) {
+        for (int q = 0; q < Q; ++q) {
           const int c = lane + 32 * q;
           float a[8], w[8];
           unpack8(dv[q], a);
@@ -363,7 +366,7 @@ __global__ void __launch_bounds__(256)
       }
       if (sums != nullptr) {
 #pragma unroll
-        for (int q = 0; q < 4; ++q)
+        for (int q = 0; q < Q; ++q)
 #pragma unroll
           for (int x = 0; x < 8; x += 4)
             *reinterpret_cast<float4*>(&s_sum[warp][(lane + 32 * q) * 8 + x]) =
@@ -384,11 +387,22 @@ __global__ void __launch_bounds__(256)
 
 // out[e, c] = sum of the partial column sums of the expert's blocks of `rows` rows: one CTA per expert and
 // 64 columns, 16 block lanes x 16 column vectors, joined in a fixed order.
+// Grid z: the layer's first bias, then its second (where it has them).
 template <typename O>
-__global__ void __launch_bounds__(256)
-    moe_join_sums_kernel(const float* __restrict__ part, O* __restrict__ out, MoePlan pl, int N, int rows) {
+struct JoinArgs {
+  const float* part;
+  O* out;
+  int N, rows;
+};
+template <typename O>
+__global__ void __launch_bounds__(256) moe_join_sums_kernel(JoinArgs<O> first, JoinArgs<O> second, MoePlan pl) {
   __shared__ float s_sum[16][68];
+  const JoinArgs<O> a = blockIdx.z == 0 ? first : second;
+  const float* __restrict__ part = a.part;
+  O* __restrict__ out = a.out;
+  const int N = a.N, rows = a.rows;
   const int e = blockIdx.y, c0 = blockIdx.x * 64;
+  if (c0 >= N) return;
   const int tx = threadIdx.x & 15, ty = threadIdx.x >> 4;
   const int lo = pl.off[e] / rows, hi = pl.off[e + 1] / rows;
   const int c = c0 + tx * 4;
@@ -407,6 +421,160 @@ __global__ void __launch_bounds__(256)
     for (int r = 0; r < 16; ++r) s += s_sum[r][threadIdx.x];
     store_gate(out, (long)e * N + c0 + threadIdx.x, s);
   }
+}
+
+// ---------------------------------------------------------------- a few slots (generation)
+// For a token or a few the weights of the chosen experts are the whole work: they are
+// streamed once by all SMs, without a plan, in two launches.
+//   up    h[slot] = gelu(x W1_e + b1_e), fp32: a CTA per slot and 8 L columns, its threads in
+//         256 / L rows of W1 by L 16-byte column vectors
+//   down  y[n] = sum_j gate_j (h W2_e + b2_e): a cluster of 8 CTAs per token and 8 L columns;
+//         each sums an eighth of the token's k H rows of W2, and the leader adds the eight
+//         up in order through distributed shared memory
+// `down` is launched while `up` runs (programmatic dependent launch) and asks for its weights
+// in L2 before it waits for h, so both matrices stream at once.  L is 4, 8 or 16 by
+// how many CTAs that makes.
+constexpr int kFewCluster = 8;
+constexpr int kFewThreads = 256;
+
+__device__ __forceinline__ void pdl_wait() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
+__device__ __forceinline__ void pdl_launch() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
+__device__ __forceinline__ void prefetch_l2(const void* p) { asm volatile("prefetch.global.L2 [%0];" ::"l"(p)); }
+
+// acc (8 columns a thread) summed over the CTA's 256 / L row lanes: s_out[0 .. 8 L), valid after the
+// __syncthreads that the caller does.
+template <int L>
+__device__ __forceinline__ void few_reduce(float* acc, float (*s_part)[8 * L], float* s_out) {
+#pragma unroll
+  for (int i = 0; i < 8; ++i)
+#pragma unroll
+    for (int o = L; o < 32; o <<= 1) acc[i] += __shfl_xor_sync(0xffffffffu, acc[i], o);
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  if (lane < L) {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) s_part[warp][lane * 8 + i] = acc[i];
+  }
+  __syncthreads();
+  if (threadIdx.x < 8 * L) {
+    float s = 0.f;
+#pragma unroll
+    for (int w = 0; w < kFewThreads / 32; ++w) s += s_part[w][threadIdx.x];
+    s_out[threadIdx.x] = s;
+  }
+}
+
+__device__ __forceinline__ void few_fma(float* acc, const uint4& u, float x) {
+  float w[8];
+  unpack8(u, w);
+#pragma unroll
+  for (int i = 0; i < 8; ++i) acc[i] = fmaf(x, w[i], acc[i]);
+}
+
+template <typename I, int L>
+__global__ void __launch_bounds__(kFewThreads)
+    moe_few_up_kernel(const bf16* __restrict__ x, const bf16* __restrict__ w1, const bf16* __restrict__ b1,
+                      const I* __restrict__ idx, float* __restrict__ h, int E, int C, int H, int k) {
+  __shared__ float s_part[kFewThreads / 32][8 * L];
+  __shared__ float s_out[8 * L];
+  extern __shared__ float s_x[];
+  pdl_launch();
+  const int slot = blockIdx.y;
+  const int e = slot_expert(idx, slot, E);
+  if (e < 0) {
+    if (idx[slot] >= (I)E && threadIdx.x == 0) set_status(kStatusBadArgument);
+    return;
+  }
+  const bf16* xr = x + (long)(slot / k) * C;
+  for (int c = threadIdx.x; c < C / 8; c += kFewThreads) unpack8(*(reinterpret_cast<const uint4*>(xr) + c), s_x + c * 8);
+  constexpr int R = kFewThreads / L;
+  const int r = threadIdx.x / L, col = blockIdx.x * 8 * L + (threadIdx.x % L) * 8;
+  __syncthreads();
+  float acc[8] = {};
+  if (col < H) {
+    const uint4* w = reinterpret_cast<const uint4*>(w1 + (long)e * C * H + col);
+    const long step = H / 8;
+    constexpr int U = 8;
+    int c = r;
+    for (; c + (U - 1) * R < C; c += U * R) {
+      uint4 u[U];
+#pragma unroll
+      for (int j = 0; j < U; ++j) u[j] = __ldg(w + (c + j * R) * step);
+#pragma unroll
+      for (int j = 0; j < U; ++j) few_fma(acc, u[j], s_x[c + j * R]);
+    }
+    for (; c < C; c += R) few_fma(acc, __ldg(w + c * step), s_x[c]);
+  }
+  few_reduce<L>(acc, s_part, s_out);
+  const int oc = blockIdx.x * 8 * L + threadIdx.x;
+  if (threadIdx.x < 8 * L && oc < H) {
+    const float v = s_out[threadIdx.x] + (b1 ? bf2f(b1[(long)e * H + oc]) : 0.f);
+    h[(long)slot * H + oc] = gelu_fast(v);
+  }
+}
+
+template <typename I, typename G, int L>
+__global__ void __cluster_dims__(kFewCluster, 1, 1) __launch_bounds__(kFewThreads)
+    moe_few_down_kernel(const float* __restrict__ h, const bf16* __restrict__ w2, const bf16* __restrict__ b2,
+                        const I* __restrict__ idx, const G* __restrict__ gates, bf16* __restrict__ y, int E, int H,
+                        int Co, int k) {
+  __shared__ float s_part[kFewThreads / 32][8 * L];
+  __shared__ float s_out[8 * L];
+  const int part = blockIdx.x;  // of the cluster
+  const long n = blockIdx.z;
+  constexpr int R = kFewThreads / L;
+  const int r = threadIdx.x / L, col = blockIdx.y * 8 * L + (threadIdx.x % L) * 8;
+  // each slot's rows [lo, hi) of this part
+  const int lo = (int)((long)H * part / kFewCluster), hi = (int)((long)H * (part + 1) / kFewCluster);
+  const long step = Co / 8;
+  if (col < Co && (threadIdx.x % L) % 4 == 0)
+    for (int j = 0; j < k; ++j) {
+      const int e = slot_expert(idx, n * k + j, E);
+      if (e < 0) continue;
+      const uint4* w = reinterpret_cast<const uint4*>(w2 + (long)e * H * Co + col);
+      for (int c = lo + r; c < hi; c += R) prefetch_l2(w + c * step);
+    }
+  pdl_wait();
+  float acc[8] = {};
+  for (int j = 0; j < k; ++j) {
+    const int e = slot_expert(idx, n * k + j, E);
+    if (e < 0 || col >= Co) continue;
+    const float g = load_gate(gates, n * k + j);
+    const uint4* w = reinterpret_cast<const uint4*>(w2 + (long)e * H * Co + col);
+    const float* hr = h + (n * k + j) * H;
+    constexpr int U = 8;
+    int c = lo + r;
+    for (; c + (U - 1) * R < hi; c += U * R) {
+      uint4 u[U];
+      float a[U];
+#pragma unroll
+      for (int q = 0; q < U; ++q) {
+        u[q] = __ldg(w + (c + q * R) * step);
+        a[q] = __ldcg(hr + c + q * R);
+      }
+#pragma unroll
+      for (int q = 0; q < U; ++q) few_fma(acc, u[q], g * a[q]);
+    }
+    for (; c < hi; c += R) few_fma(acc, __ldg(w + c * step), g * __ldcg(hr + c));
+  }
+  few_reduce<L>(acc, s_part, s_out);
+  cluster_sync_all();
+  const int oc = blockIdx.y * 8 * L + threadIdx.x;
+  if (part == 0 && threadIdx.x < 8 * L && oc < Co) {
+    float v = 0.f;
+#pragma unroll
+    for (int p = 0; p < kFewCluster; ++p) {
+      float t;
+      asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(t) : "r"(mapa_shared(&s_out[threadIdx.x], p)));
+      v += t;
+    }
+    if (b2)
+      for (int j = 0; j < k; ++j) {
+        const int e = slot_expert(idx, n * k + j, E);
+        if (e >= 0) v = fmaf(load_gate(gates, n * k + j), bf2f(b2[(long)e * Co + oc]), v);
+      }
+    y[n * Co + oc] = f2bf(v);
+  }
+  cluster_sync_all();  // the leader has read the others' sums
 }
 
 // ---------------------------------------------------------------- grouped GEMM
@@ -462,9 +630,18 @@ __device__ __forceinline__ MoeUnit moe_unit(const MoeGemmArgs& a, int u, int mt,
   return q;
 }
 
-// One 32x32 chunk: this lane's row of 32 accumulators -> slab -> TMA store.
+// Unpack this lane's 64-byte row of a slab to fp32.
+__device__ __forceinline__ void slab_get_bf16(const uint8_t* slab, int lane, float* v) {
+  const uint4* src = reinterpret_cast<const uint4*>(slab + lane * 64);
+#pragma unroll
+  for (int j = 0; j < 4; ++j) unpack8(src[slab_unit_bf16(lane, j)], v + 8 * j);
+}
+
+// One 32x32 chunk: this lane's row of 32 accumulators -> slab -> TMA store.  `staged` (MOE_DGELU): the chunk's
+// pre-activations, already in shared memory; null: read from global memory.
 __device__ __forceinline__ void moe_epi_chunk(const MoeGemmArgs& a, const CUtensorMap* tmOut, const CUtensorMap* tmAux,
-                                              uint8_t* slab, int lane, int row0, int col, int e, bool dw, float* v) {
+                                              uint8_t* slab, int lane, int row0, int col, int e, bool dw, float* v,
+                                              const uint8_t* staged = nullptr) {
   switch (a.epi) {
     case MOE_PLAIN:
     case MOE_GELU: {
@@ -484,7 +661,8 @@ __device__ __forceinline__ void moe_epi_chunk(const MoeGemmArgs& a, const CUtens
     }
     case MOE_DGELU: {
       float h[32];
-      load_row32(a.aux_in + (long)(row0 + lane) * a.N, col, a.N, h);
+      if (staged) slab_get_bf16(staged, lane, h);
+      else load_row32(a.aux_in + (long)(row0 + lane) * a.N, col, a.N, h);
 #pragma unroll
       for (int j = 0; j < 32; ++j) v[j] *= gelu_grad_fast(h[j]);
       slab_put_bf16(slab, lane, v);
@@ -727,7 +905,8 @@ struct MoePairCfg {
   static constexpr int STAGES = 5;
   static constexpr int TMEM_COLS = 512;
   static constexpr int EPI_BYTES = kEpiWarps * 2 * kEpiSlab;
-  static constexpr int SMEM_BYTES = STAGES * STAGE_BYTES + EPI_BYTES + 1024 /*align*/ + 256 /*barriers*/;
+  static constexpr int SMEM_BYTES = STAGES * STAGE_BYTES + EPI_BYTES + 1024 /*align*/ + 256 /*barriers: 15 + 16, and two words*/;
+  static_assert((2 * STAGES + 5 + 2 * kEpiWarps) * 8 + 8 <= 256, "barriers");
 };
 
 template <int MODE>
@@ -745,7 +924,8 @@ __global__ void __maxnreg__(DTB_CORESIDENT_MAXNREG)
   uint64_t* tfull_bar = empty_bar + Cfg::STAGES;  // [2]
   uint64_t* tempty_bar = tfull_bar + 2;           // [2]
   uint64_t* done_bar = tempty_bar + 2;
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(done_bar + 1);
+  uint64_t* aux_bar = done_bar + 1;  // [epilogue warps][2]
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(aux_bar + 2 * kEpiWarps);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
 
   const int warp = threadIdx.x >> 5;
@@ -763,6 +943,7 @@ __global__ void __maxnreg__(DTB_CORESIDENT_MAXNREG)
       mbar_init(&tempty_bar[b], 2 * kEpiWarps);
     }
     mbar_init(done_bar, 1);
+    for (int b = 0; b < 2 * kEpiWarps; ++b) mbar_init(&aux_bar[b], 1);
     *abort_flag = 0;
     fence_barrier_init_cluster();
     tma_prefetch_desc(&tmA);
@@ -857,47 +1038,59 @@ __global__ void __maxnreg__(DTB_CORESIDENT_MAXNREG)
     const int q4 = warp & 3;
     const int half = ew >> 2;
     uint8_t* slab = epi_smem + ew * 2 * kEpiSlab;
+    uint64_t* abar = aux_bar + ew * 2;
     const uint32_t lead_tempty0 = mapa_shared(&tempty_bar[0], 0);
+    // MOE_DGELU: a chunk's pre-activations come by TMA into the second half of its slab, two chunks ahead and
+    // the tile's first two before its products are done.  (Read by the lanes themselves, a row each, they cost
+    // the dpre GEMM of 65536 rows x 1536 columns, K 768, 224 us.)
+    const bool stage_aux = MODE == MOE_DX && args.epi == MOE_DGELU;
     uint32_t ck = 0;
     int ab = 0;
     uint32_t aphase = 0;
     for (int u = pair; u < units; u += npairs) {
       const MoeUnit q = moe_unit<MODE, 256, 256>(args, u, mt, nt);
+      const int row0 = q.m0 + (int)rank * 128 + q4 * 32;
+      const int c0 = q.n0 + half * 128;
+      // chunks of 32 columns that this warp has to do (none where its rows are not this tile's)
+      const int chunks = row0 < q.row_end ? max(0, min(4, (args.N - c0 + 31) / 32)) : 0;
+      if (stage_aux && lane == 0) {
+        fence_proxy_async_smem();
+        for (int i = 0; i < min(2, chunks); ++i) {
+          const uint32_t b = (ck + i) & 1;
+          mbar_arrive_expect_tx(&abar[b], 2048);
+          tma_load_2d(&tmAux, slab + b * kEpiSlab + 2048, &abar[b], c0 + 32 * i, row0);
+        }
+      }
       if (q.kb > 0) {
-        if (!mbar_wait(&tfull_bar[ab], aphase, abort_flag)) break;
+        if (!mbar_wait(&tfull_bar[ab], aphase, abort_flag)) {
+          if (stage_aux) {  // leave no copy in flight
+            volatile int never = 0;
+            for (int i = 0; i < min(2, chunks); ++i) mbar_wait(&abar[(ck + i) & 1], ((ck + i) >> 1) & 1, &never);
+          }
+          break;
+        }
         tc_fence_after();
       }
-      const int row0 = q.m0 + (int)rank * 128 + q4 * 32;
-      const uint32_t tbase = tmem_base + ((uint32_t)(q4 * 32) << 16) + (uint32_t)(ab * 256);
-      const int c_begin = half * 128, c_end = c_begin + 128;
-      if (row0 < q.row_end) {
+      const uint32_t tbase = tmem_base + ((uint32_t)(q4 * 32) << 16) + (uint32_t)(ab * 256 + half * 128);
 #pragma unroll 1
-        for (int c = c_begin; c < c_end; c += 64) {
-          if (q.n0 + c >= args.N) break;  // warp-uniform
-          uint32_t r0[32], r1[32];
-          if (q.kb > 0) {
-            tmem_ld32_issue(tbase + c, r0);
-            tmem_ld32_issue(tbase + c + 32, r1);
-            tmem_wait_ld();
-          } else {
+      for (int i = 0; i < chunks; ++i) {
+        uint8_t* sl = slab + (ck & 1) * kEpiSlab;
+        float v[32];
+        if (q.kb > 0) {
+          tmem_ld32(tbase + 32 * i, v);
+        } else {
 #pragma unroll
-            for (int j = 0; j < 32; ++j) r0[j] = r1[j] = 0u;
-          }
-          float v[32];
-#pragma unroll
-          for (int j = 0; j < 32; ++j) v[j] = __uint_as_float(r0[j]);
-          epi_slab_acquire(lane, true);
-          moe_epi_chunk(args, &tmOut, &tmAux, slab + (ck & 1) * kEpiSlab, lane, row0, q.n0 + c, q.e, MODE == MOE_DW, v);
-          ++ck;
-          if (q.n0 + c + 32 < args.N) {
-#pragma unroll
-            for (int j = 0; j < 32; ++j) v[j] = __uint_as_float(r1[j]);
-            epi_slab_acquire(lane, true);
-            moe_epi_chunk(args, &tmOut, &tmAux, slab + (ck & 1) * kEpiSlab, lane, row0, q.n0 + c + 32, q.e,
-                          MODE == MOE_DW, v);
-            ++ck;
-          }
+          for (int j = 0; j < 32; ++j) v[j] = 0.f;
         }
+        epi_slab_acquire(lane, true);
+        if (stage_aux) mbar_wait(&abar[ck & 1], (ck >> 1) & 1, abort_flag);
+        moe_epi_chunk(args, &tmOut, &tmAux, sl, lane, row0, c0 + 32 * i, q.e, MODE == MOE_DW, v,
+                      stage_aux ? sl + 2048 : nullptr);
+        if (stage_aux && i + 2 < chunks && lane == 0) {  // every lane has read the buffer (moe_epi_chunk synchronises)
+          mbar_arrive_expect_tx(&abar[ck & 1], 2048);
+          tma_load_2d(&tmAux, sl + 2048, &abar[ck & 1], c0 + 32 * (i + 2), row0);
+        }
+        ++ck;
       }
       if (q.kb > 0) {
         tc_fence_before();
@@ -1030,7 +1223,7 @@ static void moe_rows_gemm(int mode, const bf16* a, const bf16* w, bf16* out, int
   const CUtensorMap ta = make_map(a, z.R, K, K, 64, kBM);
   const CUtensorMap tb = mode == MOE_FWD ? make_map3(w, z.E, K, N, 64, 64) : make_map3(w, z.E, N, K, 64, pair ? 128 : bn);
   const CUtensorMap to = make_store_map(out, false, z.R, N, N);
-  const CUtensorMap tx = g.save_aux ? make_store_map(aux, false, z.R, N, N) : to;
+  const CUtensorMap tx = aux ? make_store_map(aux, false, z.R, N, N) : to;
   const long units = moe_max_tiles(z.P, z.E) * ((N + bn - 1) / bn);
   if (pair) {
     if (mode == MOE_FWD) launch_moe2<MOE_FWD>(ta, tb, to, tx, g, units, st);
@@ -1138,10 +1331,89 @@ static MoeSizes check_experts(const at::Tensor& x, const at::Tensor& w1, const s
   return z;
 }
 
-// Forward.  Returns [y] or, with `save`, [y, plan, xp, pre, act, yp] for experts_bwd.
-std::vector<at::Tensor> experts_fwd(at::Tensor x, at::Tensor w1, std::optional<at::Tensor> b1,
-                                       at::Tensor w2, std::optional<at::Tensor> b2, at::Tensor idx,
-                                       at::Tensor gates, bool save) {
+// Up to this many slots go the streaming way: each slot reads its expert's weights, so it loses once many
+// slots share experts.
+constexpr long kFewSlots = 16;
+
+template <typename I, typename G>
+static void moe_few_launch(const bf16* x, const bf16* w1, const bf16* b1, const bf16* w2, const bf16* b2, const I* idx,
+                           const G* gates, float* h, bf16* y, int C, int H, int Co, const MoeSizes& z, cudaStream_t st) {
+  const int E = (int)z.E, k = (int)z.k;
+  // the fewest column vectors a row that still leave two CTAs an SM or fewer
+  const auto lanes = [](long cols, long per) {
+    for (int l = 16; l > 4; l /= 2)
+      if ((cols + 8 * l - 1) / (8 * l) * per >= 148) return l;
+    return 4;
+  };
+  const int l1 = lanes(H, z.P), l2 = lanes(Co, z.n * kFewCluster);
+#define DTB_FEW_UP(L)                                                                                              \
+  moe_few_up_kernel<I, L><<<dim3((H + 8 * L - 1) / (8 * L), (unsigned)z.P), kFewThreads, C * 4, st>>>(x, w1, b1, idx, h, E, \
+                                                                                                     C, H, k)
+  if (l1 == 16) DTB_FEW_UP(16);
+  else if (l1 == 8) DTB_FEW_UP(8);
+  else DTB_FEW_UP(4);
+#undef DTB_FEW_UP
+  C10_CUDA_KERNEL_LAUNCH_CHECK();
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(kFewCluster, (unsigned)((Co + 8 * l2 - 1) / (8 * l2)), (unsigned)z.n);
+  cfg.blockDim = dim3(kFewThreads, 1, 1);
+  cfg.stream = st;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+#define DTB_FEW_DOWN(L)                                                                                              \
+  C10_CUDA_CHECK(cudaLaunchKernelEx(&cfg, moe_few_down_kernel<I, G, L>, (const float*)h, w2, b2, idx, gates, y, E, H, Co, k))
+  if (l2 == 16) DTB_FEW_DOWN(16);
+  else if (l2 == 8) DTB_FEW_DOWN(8);
+  else DTB_FEW_DOWN(4);
+#undef DTB_FEW_DOWN
+  count_launch(2);
+}
+
+static void moe_few(const at::Tensor& x, const at::Tensor& w1, const bf16* b1, const at::Tensor& w2, const bf16* b2,
+                    const at::Tensor& idx, const at::Tensor& gates, const at::Tensor& y, const MoeSizes& z,
+                    cudaStream_t st) {
+  const int C = (int)w1.size(1), H = (int)w1.size(2), Co = (int)w2.size(2);
+  auto h = at::empty({z.P, H}, x.options().dtype(at::kFloat));
+  const auto go = [&](auto* i, auto* g) {
+    moe_few_launch(bptr(x), bptr(w1), b1, bptr(w2), b2, i, g, h.data_ptr<float>(), bptr_mut(y), C, H, Co, z, st);
+  };
+  const bool i32 = idx.scalar_type() == at::kInt, f32 = gates.scalar_type() == at::kFloat;
+  const int* pi = i32 ? idx.const_data_ptr<int>() : nullptr;
+  const long* pl = i32 ? nullptr : reinterpret_cast<const long*>(idx.const_data_ptr<int64_t>());
+  if (i32 && f32) go(pi, gates.const_data_ptr<float>());
+  else if (i32) go(pi, bptr(gates));
+  else if (f32) go(pl, gates.const_data_ptr<float>());
+  else go(pl, bptr(gates));
+}
+
+// What the backward reads of the forward, in one bf16 buffer.
+struct MoeSaved {
+  bf16 *xp, *pre, *act, *yp;
+};
+static long saved_numel(const MoeSizes& z, long C, long H, long Co) { return z.R * (C + 2 * H + Co); }
+static MoeSaved saved_views(const at::Tensor& t, const MoeSizes& z, long C, long H) {
+  MoeSaved v;
+  v.xp = bptr_mut(t);
+  v.pre = v.xp + z.R * C;
+  v.act = v.pre + z.R * H;
+  v.yp = v.act + z.R * H;
+  return v;
+}
+
+template <typename G>
+static void moe_combine(const bf16* rows, const G* gates, const at::Tensor& y, long C, const MoePlan& pl,
+                        const MoeSizes& z, cudaStream_t st) {
+  moe_combine_kernel<G><<<warp_grid(z.n), 256, 0, st>>>(rows, gates, bptr_mut(y), pl, (int)z.n, (int)C, (int)z.k);
+  count_launch();
+  C10_CUDA_KERNEL_LAUNCH_CHECK();
+}
+
+// Forward.  Returns [y] or, with `save`, [y, plan, rows] for experts_bwd.
+std::vector<at::Tensor> experts_fwd(at::Tensor x, at::Tensor w1, std::optional<at::Tensor> b1, at::Tensor w2,
+                                    std::optional<at::Tensor> b2, at::Tensor idx, at::Tensor gates, bool save) {
   const MoeSizes z = check_experts(x, w1, b1, w2, b2, gates);
   TORCH_CHECK(idx.is_cuda() && idx.get_device() == x.get_device() && idx.sizes() == gates.sizes() &&
                   idx.is_contiguous() && (idx.scalar_type() == at::kInt || idx.scalar_type() == at::kLong),
@@ -1154,45 +1426,42 @@ std::vector<at::Tensor> experts_fwd(at::Tensor x, at::Tensor w1, std::optional<a
   if (z.n == 0) {
     if (!save) return {y};
     auto none = at::empty({0}, x.options());
-    return {y, none, none, none, none, none};
+    return {y, none, none};
+  }
+  if (!save && z.P <= kFewSlots && C <= 8192) {  // x's row in shared memory
+    moe_few(x, w1, bptr_opt(b1), w2, bptr_opt(b2), idx, gates, y, z, st);
+    return {y};
   }
   auto plan = at::empty({plan_ints(z.P, z.E)}, x.options().dtype(at::kInt));
   const MoePlan pl = plan_views(plan.data_ptr<int>(), z.P, z.E);
   moe_build_plan(idx, pl, z, st);
-  auto xp = at::empty({z.R, C}, x.options());
-  moe_gather_kernel<<<warp_grid(z.R), 256, 0, st>>>(bptr(x), bptr_mut(xp), pl, (int)z.E, (int)C, (int)z.k);
+  auto rows = at::empty({saved_numel(z, C, H, Co) - (save ? 0 : z.R * H)}, x.options());
+  MoeSaved v = saved_views(rows, z, C, H);
+  if (!save) {  // no pre-activations
+    v.act = v.pre;
+    v.pre = nullptr;
+    v.yp = v.act + z.R * H;
+  }
+  moe_gather_kernel<<<warp_grid(z.R), 256, 0, st>>>(bptr(x), v.xp, pl, (int)z.E, (int)C, (int)z.k);
   count_launch();
-  auto act = at::empty({z.R, H}, x.options());
-  at::Tensor pre;
-  if (save) pre = at::empty({z.R, H}, x.options());
-  auto yp = at::empty({z.R, Co}, x.options());
-  moe_rows_gemm(MOE_FWD, bptr(xp), bptr(w1), bptr_mut(act), (int)H, (int)C, MOE_GELU, bptr_opt(b1),
-                save ? bptr_mut(pre) : nullptr, nullptr, pl, z, st);
-  moe_rows_gemm(MOE_FWD, bptr(act), bptr(w2), bptr_mut(yp), (int)Co, (int)H, MOE_PLAIN, bptr_opt(b2), nullptr, nullptr, pl,
-                z, st);
-  if (gates.scalar_type() == at::kFloat)
-    moe_combine_kernel<float><<<warp_grid(z.n), 256, 0, st>>>(bptr(yp), gates.data_ptr<float>(), bptr_mut(y), pl,
-                                                             (int)z.n, (int)Co, (int)z.k);
-  else
-    moe_combine_kernel<bf16><<<warp_grid(z.n), 256, 0, st>>>(bptr(yp), bptr(gates), bptr_mut(y), pl, (int)z.n, (int)Co,
-                                                            (int)z.k);
-  count_launch();
-  C10_CUDA_KERNEL_LAUNCH_CHECK();
+  moe_rows_gemm(MOE_FWD, v.xp, bptr(w1), v.act, (int)H, (int)C, MOE_GELU, bptr_opt(b1), v.pre, nullptr, pl, z, st);
+  moe_rows_gemm(MOE_FWD, v.act, bptr(w2), v.yp, (int)Co, (int)H, MOE_PLAIN, bptr_opt(b2), nullptr, nullptr, pl, z, st);
+  if (gates.scalar_type() == at::kFloat) moe_combine(v.yp, gates.data_ptr<float>(), y, Co, pl, z, st);
+  else moe_combine(v.yp, bptr(gates), y, Co, pl, z, st);
   if (!save) return {y};
-  return {y, plan, xp, pre, act, yp};
+  return {y, plan, rows};
 }
 
 // Backward: returns [dx, dgates]; the weights' and biases' gradients are written to dw1, db1, dw2, db2
 // (all bf16 or all fp32; db1 / db2 only where the layer has the bias).
-std::vector<at::Tensor> experts_bwd(at::Tensor dy, at::Tensor x, at::Tensor w1, at::Tensor w2,
-                                       at::Tensor gates, std::vector<at::Tensor> saved, at::Tensor dw1,
-                                       std::optional<at::Tensor> db1, at::Tensor dw2,
-                                       std::optional<at::Tensor> db2) {
+std::vector<at::Tensor> experts_bwd(at::Tensor dy, at::Tensor x, at::Tensor w1, at::Tensor w2, at::Tensor gates,
+                                    std::vector<at::Tensor> saved, at::Tensor dw1, std::optional<at::Tensor> db1,
+                                    at::Tensor dw2, std::optional<at::Tensor> db2) {
   const MoeSizes z = check_experts(x, w1, std::nullopt, w2, std::nullopt, gates);
   const long C = w1.size(1), H = w1.size(2), Co = w2.size(2);
   check_bf16(dy, x, "dy");
   TORCH_CHECK(dy.dim() == 2 && dy.size(0) == z.n && dy.size(1) == Co, "experts_bwd: dy must be [n, co]");
-  TORCH_CHECK(saved.size() == 5, "experts_bwd: the forward's plan, xp, pre, act and yp expected");
+  TORCH_CHECK(saved.size() == 2, "experts_bwd: the forward's plan and rows expected");
   const auto wt = dw1.scalar_type();
   TORCH_CHECK(wt == at::kFloat || wt == at::kBFloat16, "experts_bwd: fp32 or bf16 weight gradients");
   const auto check_grad = [&](const at::Tensor& t, at::IntArrayRef sizes, const char* what) {
@@ -1200,64 +1469,69 @@ std::vector<at::Tensor> experts_bwd(at::Tensor dy, at::Tensor x, at::Tensor w1, 
                     t.is_contiguous() && (reinterpret_cast<uintptr_t>(t.data_ptr()) & 15) == 0,
                 "experts_bwd: ", what, " must be a contiguous, 16-byte aligned ", wt, " tensor of its weight's shape");
   };
+  const bool has1 = db1 && db1->defined(), has2 = db2 && db2->defined();
   check_grad(dw1, w1.sizes(), "dw1");
   check_grad(dw2, w2.sizes(), "dw2");
-  if (db1 && db1->defined()) check_grad(*db1, {z.E, H}, "db1");
-  if (db2 && db2->defined()) check_grad(*db2, {z.E, Co}, "db2");
+  if (has1) check_grad(*db1, {z.E, H}, "db1");
+  if (has2) check_grad(*db2, {z.E, Co}, "db2");
   c10::cuda::CUDAGuard guard(x.device());
   bind_device_context(x.get_device());
   cudaStream_t st = at::cuda::getCurrentCUDAStream();
   auto dx = at::empty({z.n, C}, x.options());
-  auto dgates = at::zeros_like(gates);
+  auto dgates = at::empty_like(gates);
   if (z.n == 0) {
     dw1.zero_();
     dw2.zero_();
-    if (db1 && db1->defined()) db1->zero_();
-    if (db2 && db2->defined()) db2->zero_();
+    if (has1) db1->zero_();
+    if (has2) db2->zero_();
     return {dx, dgates};
   }
-  const at::Tensor &plan = saved[0], &xp = saved[1], &pre = saved[2], &act = saved[3], &yp = saved[4];
-  TORCH_CHECK(plan.scalar_type() == at::kInt && plan.numel() == plan_ints(z.P, z.E) && xp.size(0) == z.R &&
-                  xp.size(1) == C && pre.size(0) == z.R && pre.size(1) == H && act.sizes() == pre.sizes() &&
-                  yp.size(0) == z.R && yp.size(1) == Co,
+  const at::Tensor &plan = saved[0], &rows = saved[1];
+  TORCH_CHECK(plan.scalar_type() == at::kInt && plan.numel() == plan_ints(z.P, z.E) &&
+                  rows.scalar_type() == at::kBFloat16 && rows.numel() == saved_numel(z, C, H, Co),
               "experts_bwd: saved tensors of another forward");
   const MoePlan pl = plan_views(plan.data_ptr<int>(), z.P, z.E);
-  const bool gf = gates.scalar_type() == at::kFloat;
-  auto u = at::empty({z.R, Co}, x.options());
-  const bool has1 = db1 && db1->defined(), has2 = db2 && db2->defined();
-  at::Tensor s1, s2;  // column sums of blocks of rows
-  if (has1) s1 = at::empty({z.R / 32, H}, x.options().dtype(at::kFloat));
-  if (has2) s2 = at::empty({z.R / kRowPad, Co}, x.options().dtype(at::kFloat));
-  float* p1 = has1 ? s1.data_ptr<float>() : nullptr;
-  float* p2 = has2 ? s2.data_ptr<float>() : nullptr;
-  const int gr = (int)std::min<long>(z.R / kRowPad, 148L * 4);
-  if (gf)
-    moe_grad_rows_kernel<float><<<gr, 256, 0, st>>>(bptr(dy), bptr(yp), gates.data_ptr<float>(), bptr_mut(u),
-                                                   dgates.data_ptr<float>(), p2, pl, (int)z.E, (int)Co, (int)z.k);
-  else
-    moe_grad_rows_kernel<bf16><<<gr, 256, 0, st>>>(bptr(dy), bptr(yp), bptr(gates), bptr_mut(u), bptr_mut(dgates), p2,
-                                                  pl, (int)z.E, (int)Co, (int)z.k);
+  const MoeSaved v = saved_views(rows, z, C, H);
+  // scratch: u (later dx's rows) and dpre, and the column sums of blocks of rows
+  const long urows = z.R * std::max(C, Co), sums = has1 ? z.R / 32 * H : 0, sums2 = has2 ? z.R / kRowPad * Co : 0;
+  auto scratch = at::empty({urows + z.R * H + 2 * (sums + sums2)}, x.options());
+  bf16* u = bptr_mut(scratch);
+  bf16* dpre = u + urows;
+  bf16* dxp = u;
+  float* p1 = has1 ? reinterpret_cast<float*>(dpre + z.R * H) : nullptr;
+  float* p2 = has2 ? reinterpret_cast<float*>(dpre + z.R * H) + sums : nullptr;
+  const bf16* yp = v.yp;
+  const int gr = (int)std::min<long>(z.R / kRowPad, 1L << 16);
+  const int Q = (int)std::min<long>(4, (Co + 255) / 256);
+#define DTB_GRAD_ROWS(G, g, dg)                                                                                       \
+  if (Q == 1) moe_grad_rows_kernel<G, 1><<<gr, 256, 0, st>>>(bptr(dy), yp, g, u, dg, p2, pl, (int)z.E, (int)Co, (int)z.k, z.P); \
+  else if (Q == 2) moe_grad_rows_kernel<G, 2><<<gr, 256, 0, st>>>(bptr(dy), yp, g, u, dg, p2, pl, (int)z.E, (int)Co, (int)z.k, z.P); \
+  else if (Q == 3) moe_grad_rows_kernel<G, 3><<<gr, 256, 0, st>>>(bptr(dy), yp, g, u, dg, p2, pl, (int)z.E, (int)Co, (int)z.k, z.P); \
+  else moe_grad_rows_kernel<G, 4><<<gr, 256, 0, st>>>(bptr(dy), yp, g, u, dg, p2, pl, (int)z.E, (int)Co, (int)z.k, z.P);
+  if (gates.scalar_type() == at::kFloat) {
+    DTB_GRAD_ROWS(float, gates.data_ptr<float>(), dgates.data_ptr<float>())
+  } else {
+    DTB_GRAD_ROWS(bf16, bptr(gates), bptr_mut(dgates))
+  }
+#undef DTB_GRAD_ROWS
   count_launch();
-  const auto join = [&](const float* part, const at::Tensor& out, long N, int rows) {
-    const dim3 grid((unsigned)((N + 63) / 64), (unsigned)z.E);
-    if (wt == at::kFloat) moe_join_sums_kernel<float><<<grid, 256, 0, st>>>(part, out.data_ptr<float>(), pl, (int)N, rows);
-    else moe_join_sums_kernel<bf16><<<grid, 256, 0, st>>>(part, bptr_mut(out), pl, (int)N, rows);
+  moe_rows_gemm(MOE_DX, u, bptr(w2), dpre, (int)H, (int)Co, MOE_DGELU, nullptr, v.pre, p1, pl, z, st);
+  moe_weight_gemm(v.act, u, dw2, (int)H, (int)Co, pl, z, st);
+  moe_rows_gemm(MOE_DX, dpre, bptr(w1), dxp, (int)C, (int)H, MOE_PLAIN, nullptr, nullptr, nullptr, pl, z, st);
+  moe_weight_gemm(v.xp, dpre, dw1, (int)C, (int)H, pl, z, st);
+  if (has1 || has2) {
+    const auto join = [&](auto* o1, auto* o2) {
+      using O = std::remove_pointer_t<decltype(o1)>;
+      JoinArgs<O> a{p1, o1, (int)H, 32}, b{p2, o2, (int)Co, kRowPad};
+      const long widest = std::max(has1 ? H : 0, has2 ? Co : 0);
+      const dim3 grid((unsigned)((widest + 63) / 64), (unsigned)z.E, has1 && has2 ? 2 : 1);
+      moe_join_sums_kernel<O><<<grid, 256, 0, st>>>(has1 ? a : b, b, pl);
+    };
+    if (wt == at::kFloat) join(has1 ? db1->data_ptr<float>() : nullptr, has2 ? db2->data_ptr<float>() : nullptr);
+    else join(has1 ? bptr_mut(*db1) : nullptr, has2 ? bptr_mut(*db2) : nullptr);
     count_launch();
-  };
-  auto dpre = at::empty({z.R, H}, x.options());
-  moe_rows_gemm(MOE_DX, bptr(u), bptr(w2), bptr_mut(dpre), (int)H, (int)Co, MOE_DGELU, nullptr, bptr_mut(pre), p1, pl,
-                z, st);
-  moe_weight_gemm(bptr(act), bptr(u), dw2, (int)H, (int)Co, pl, z, st);
-  if (has2) join(p2, *db2, Co, kRowPad);
-  auto dxp = at::empty({z.R, C}, x.options());
-  moe_rows_gemm(MOE_DX, bptr(dpre), bptr(w1), bptr_mut(dxp), (int)C, (int)H, MOE_PLAIN, nullptr, nullptr, nullptr, pl,
-                z, st);
-  moe_weight_gemm(bptr(xp), bptr(dpre), dw1, (int)C, (int)H, pl, z, st);
-  if (has1) join(p1, *db1, H, 32);
-  moe_combine_kernel<float><<<warp_grid(z.n), 256, 0, st>>>(bptr(dxp), nullptr, bptr_mut(dx), pl, (int)z.n, (int)C,
-                                                           (int)z.k);
-  count_launch();
-  C10_CUDA_KERNEL_LAUNCH_CHECK();
+  }
+  moe_combine<float>(dxp, nullptr, dx, C, pl, z, st);
   return {dx, dgates};
 }
 

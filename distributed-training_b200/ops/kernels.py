@@ -156,7 +156,7 @@ def experts(x, w1, b1, w2, b2, idx, gates) -> torch.Tensor:
 
 def experts_fwd(x, w1, b1, w2, b2, idx, gates, save: bool = False):
     """The experts' products (``functional.expert_mlp``) on bf16 rows ``x`` [n, c].
-    Returns [y], or with ``save`` [y, plan, xp, pre, act, yp]: what ``experts_bwd`` reads."""
+    Returns [y], or with ``save`` [y, plan, rows]: what ``experts_bwd`` reads."""
     return lib().experts_fwd(x, w1, b1, w2, b2, idx, gates, save)
 
 
