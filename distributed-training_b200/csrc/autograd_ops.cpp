@@ -93,13 +93,45 @@ struct ExpertsFn : public torch::autograd::Function<ExpertsFn> {
   }
 };
 
-torch::Tensor experts_autograd(torch::Tensor x, torch::Tensor w1, c10::optional<torch::Tensor> b1, torch::Tensor w2,
-                               c10::optional<torch::Tensor> b2, torch::Tensor idx, torch::Tensor gates) {
-  const auto wants = [](const c10::optional<torch::Tensor>& t) { return t && t->defined() && t->requires_grad(); };
+// expert_mlp on inputs of any leading shape and layout; nothing where the kernels do not take them (other
+// types or devices, widths that are not multiples of 8).
+c10::optional<torch::Tensor> experts_autograd(torch::Tensor x, torch::Tensor w1, c10::optional<torch::Tensor> b1,
+                                              torch::Tensor w2, c10::optional<torch::Tensor> b2, torch::Tensor idx,
+                                              torch::Tensor gates) {
+  TORCH_CHECK_VALUE(x.dim() >= 1 && w1.dim() == 3 && w2.dim() == 3 && w1.size(1) == x.size(-1) &&
+                        w2.size(0) == w1.size(0) && w2.size(1) == w1.size(2),
+                    "expert_mlp: x ", x.sizes(), ", w1 ", w1.sizes(), " and w2 ", w2.sizes(), " do not fit");
+  TORCH_CHECK_VALUE(idx.dim() == x.dim() && idx.sizes() == gates.sizes() &&
+                        idx.sizes().slice(0, idx.dim() - 1) == x.sizes().slice(0, x.dim() - 1),
+                    "expert_mlp: idx ", idx.sizes(), " and gates ", gates.sizes(), " must be x's rows by slots");
+  const auto it = idx.scalar_type(), gt = gates.scalar_type();
+  TORCH_CHECK_VALUE(it == at::kInt || it == at::kLong, "expert_mlp: idx must be int32 or int64, got ", it);
+  const auto there = [](const c10::optional<torch::Tensor>& t) { return t && t->defined(); };
+  const auto fast = [](const torch::Tensor& t) { return t.is_cuda() && t.scalar_type() == at::kBFloat16; };
+  const int64_t c = x.size(-1), k = idx.size(-1);
+  if (!fast(x) || !fast(w1) || !fast(w2) || (there(b1) && !fast(*b1)) || (there(b2) && !fast(*b2)) ||
+      !gates.is_cuda() || (gt != at::kFloat && gt != at::kBFloat16) || c % 8 || w1.size(2) % 8 || w2.size(2) % 8 ||
+      w1.size(0) > 512 || k > 32)
+    return c10::nullopt;
+  const bool two = x.dim() == 2;
+  auto shape = x.sizes().vec();
+  shape.back() = w2.size(2);
+  const auto flat = [two](const torch::Tensor& t, int64_t n) { return (two ? t : t.reshape({-1, n})).contiguous(); };
+  x = flat(x, c);
+  idx = flat(idx, k);
+  gates = flat(gates, k);
+  w1 = w1.contiguous();
+  w2 = w2.contiguous();
+  if (there(b1)) b1 = b1->contiguous();
+  if (there(b2)) b2 = b2->contiguous();
+  const auto wants = [&](const c10::optional<torch::Tensor>& t) { return there(t) && t->requires_grad(); };
+  torch::Tensor y;
   if (!torch::GradMode::is_enabled() || !(x.requires_grad() || w1.requires_grad() || w2.requires_grad() ||
                                           gates.requires_grad() || wants(b1) || wants(b2)))
-    return experts_fwd(x, w1, b1, w2, b2, idx, gates, false)[0];
-  return ExpertsFn::apply(x, w1, b1, w2, b2, idx, gates);
+    y = experts_fwd(x, w1, b1, w2, b2, idx, gates, false)[0];
+  else
+    y = ExpertsFn::apply(x, w1, b1, w2, b2, idx, gates);
+  return two ? y : y.view(shape);
 }
 
 }  // namespace dtb

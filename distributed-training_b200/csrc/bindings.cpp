@@ -63,8 +63,9 @@ std::vector<torch::Tensor> experts_bwd(torch::Tensor dy, torch::Tensor x, torch:
 std::vector<torch::Tensor> route_autograd(torch::Tensor logits, int64_t k, bool softmax,
                                           c10::optional<torch::Tensor> bias, int64_t groups, int64_t keep, int64_t top,
                                           bool renorm, double scale);
-torch::Tensor experts_autograd(torch::Tensor x, torch::Tensor w1, c10::optional<torch::Tensor> b1, torch::Tensor w2,
-                               c10::optional<torch::Tensor> b2, torch::Tensor idx, torch::Tensor gates);
+c10::optional<torch::Tensor> experts_autograd(torch::Tensor x, torch::Tensor w1, c10::optional<torch::Tensor> b1,
+                                              torch::Tensor w2, c10::optional<torch::Tensor> b2, torch::Tensor idx,
+                                              torch::Tensor gates);
 // clip.cu
 torch::Tensor clip_grads(std::vector<c10::optional<torch::Tensor>> in,
                          c10::optional<std::vector<c10::optional<torch::Tensor>>> out, double max_norm, bool scale);

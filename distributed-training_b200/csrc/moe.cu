@@ -29,6 +29,13 @@
 
 namespace dtb {
 
+// Programmatic dependent launch: a kernel that is launched this way may start while the one before it runs.
+// pdl_wait returns once that one is complete and its writes are visible; pdl_launch lets the next one start.
+// Kernels here call pdl_launch after pdl_wait, so what a kernel's own predecessor waited for is complete too.
+__device__ __forceinline__ void pdl_wait() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
+__device__ __forceinline__ void pdl_launch() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
+__device__ __forceinline__ void prefetch_l2(const void* p) { asm volatile("prefetch.global.L2 [%0];" ::"l"(p)); }
+
 constexpr int kMoeMaxExperts = 512;
 constexpr int kMoeMaxK = 32;
 constexpr int kRowPad = 64;
@@ -37,7 +44,8 @@ constexpr int kRowPad = 64;
 struct MoePlan {
   int4* tile;   // row tiles of 128 in expert order: {expert, first row, end of the expert's rows, 0}
   int4* tile2;  // the same of 256 rows
-  int* ntile;   // [2] their numbers, padded to 4
+  int4* tile3;  // and of 64, with the end of the expert's rows that are not padding; their number is off[E] / 64
+  int* ntile;   // [2] the numbers of the first two, padded to 4
   int* off;    // [E + 1] first row of each expert, a multiple of 64
   int* count;  // [E] rows of each expert, without the padding
   int* inv;    // [P] row of a slot, -1: none
@@ -52,13 +60,14 @@ constexpr int kPlanThreads = 256;
 constexpr int kPlanChunk = 2048;  // slots a block sorts: 8 warps x 256
 static long plan_blocks(long P) { return std::max<long>(1, (P + kPlanChunk - 1) / kPlanChunk); }
 static long plan_ints(long P, long E) {
-  return 8 * moe_max_tiles(P, E) + 4 + (E + 1) + E + P + moe_max_rows(P, E) + plan_blocks(P) * E;
+  return 8 * moe_max_tiles(P, E) + moe_max_rows(P, E) / kRowPad * 4 + 4 + (E + 1) + E + P + moe_max_rows(P, E) + plan_blocks(P) * E;
 }
 static MoePlan plan_views(int* p, long P, long E) {
   MoePlan v;
   v.tile = reinterpret_cast<int4*>(p);
   v.tile2 = v.tile + moe_max_tiles(P, E);
-  v.ntile = p + 8 * moe_max_tiles(P, E);
+  v.tile3 = v.tile2 + moe_max_tiles(P, E);
+  v.ntile = reinterpret_cast<int*>(v.tile3 + moe_max_rows(P, E) / kRowPad);
   v.off = v.ntile + 4;
   v.count = v.off + E + 1;
   v.inv = v.count + E;
@@ -116,6 +125,7 @@ __device__ __forceinline__ int plan_expert(const MoePlan& pl, int e, int E, int 
     if (e == 0) pl.off[0] = 0;
     for (int t = 0; t < t1; ++t) pl.tile[n1 - t1 + t] = make_int4(e, start + t * kBM, end, 0);
     for (int t = 0; t < t2; ++t) pl.tile2[n2 - t2 + t] = make_int4(e, start + t * 2 * kBM, end, 0);
+    for (int r = start; r < end; r += kRowPad) pl.tile3[r / kRowPad] = make_int4(e, r, start + total, 0);
     if (e == E - 1) {
       pl.ntile[0] = n1;
       pl.ntile[1] = n2;
@@ -169,6 +179,7 @@ constexpr int kPlanSmall = 4096;
 template <typename I>
 __global__ void __launch_bounds__(kMoeMaxExperts) moe_plan_kernel(const I* __restrict__ idx, int P, int E, MoePlan pl) {
   extern __shared__ int s_w[];  // [16][E]
+  pdl_launch();
   constexpr int W = kMoeMaxExperts / 32;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int per = ((P + W - 1) / W + 31) / 32 * 32;
@@ -246,6 +257,8 @@ __device__ __forceinline__ void store_gate(bf16* g, long i, float v) { g[i] = f2
 // One warp per row; padding rows become zeros.
 __global__ void __launch_bounds__(256)
     moe_gather_kernel(const bf16* __restrict__ x, bf16* __restrict__ xp, MoePlan pl, int E, int C, int k) {
+  pdl_wait();
+  pdl_launch();
   const int lane = threadIdx.x & 31;
   const int rows = pl.off[E];
   for (int r = (blockIdx.x * blockDim.x + threadIdx.x) >> 5; r < rows; r += (gridDim.x * blockDim.x) >> 5) {
@@ -437,10 +450,6 @@ __global__ void __launch_bounds__(256) moe_join_sums_kernel(JoinArgs<O> first, J
 constexpr int kFewCluster = 8;
 constexpr int kFewThreads = 256;
 
-__device__ __forceinline__ void pdl_wait() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
-__device__ __forceinline__ void pdl_launch() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
-__device__ __forceinline__ void prefetch_l2(const void* p) { asm volatile("prefetch.global.L2 [%0];" ::"l"(p)); }
-
 // acc (8 columns a thread) summed over the CTA's 256 / L row lanes: s_out[0 .. 8 L), valid after the
 // __syncthreads that the caller does.
 template <int L>
@@ -630,6 +639,52 @@ __device__ __forceinline__ MoeUnit moe_unit(const MoeGemmArgs& a, int u, int mt,
   return q;
 }
 
+// Two fp32 operations an instruction: the epilogues with an activation are bound by instruction issue (one
+// 32x32 chunk of dpre took 1,100 instructions a warp with scalar ones).
+__device__ __forceinline__ uint64_t f2(float a, float b) {
+  uint64_t r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
+  return r;
+}
+__device__ __forceinline__ void f2_get(uint64_t v, float& a, float& b) {
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(v));
+}
+__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
+  uint64_t r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+  return r;
+}
+__device__ __forceinline__ uint64_t mul2(uint64_t a, uint64_t b) {
+  uint64_t r;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+__device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
+  uint64_t r;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+__device__ __forceinline__ uint64_t f2s(float a) { return f2(a, a); }
+constexpr float kGeluC = 0.7978845608028654f;       // sqrt(2 / pi)
+constexpr float kGeluC3 = kGeluC * 0.044715f;
+// t = tanh(c x + c3 x^3), two at a time; x2 = x^2
+__device__ __forceinline__ uint64_t gelu_tanh2(uint64_t x, uint64_t x2) {
+  float a, b;
+  f2_get(mul2(x, fma2(x2, f2s(kGeluC3), f2s(kGeluC))), a, b);
+  return f2(tanh_fast(a), tanh_fast(b));
+}
+__device__ __forceinline__ uint64_t gelu2(uint64_t x) {  // x / 2 (1 + t)
+  const uint64_t h = mul2(x, f2s(0.5f));
+  return fma2(h, gelu_tanh2(x, mul2(x, x)), h);
+}
+__device__ __forceinline__ uint64_t gelu_slope2(uint64_t x) {  // (1 + t) / 2 + x / 2 (1 - t^2) (c + 3 c3 x^2)
+  const uint64_t x2 = mul2(x, x);
+  const uint64_t t = gelu_tanh2(x, x2);
+  const uint64_t r = mul2(x, fma2(x2, f2s(1.5f * kGeluC3), f2s(0.5f * kGeluC)));
+  const uint64_t w = fma2(mul2(t, f2s(-1.f)), t, f2s(1.f));
+  return fma2(r, w, fma2(t, f2s(0.5f), f2s(0.5f)));
+}
+
 // Unpack this lane's 64-byte row of a slab to fp32.
 __device__ __forceinline__ void slab_get_bf16(const uint8_t* slab, int lane, float* v) {
   const uint4* src = reinterpret_cast<const uint4*>(slab + lane * 64);
@@ -649,12 +704,12 @@ __device__ __forceinline__ void moe_epi_chunk(const MoeGemmArgs& a, const CUtens
         float b[32];
         load_row32(a.bias + (long)e * a.N, col, a.N, b);
 #pragma unroll
-        for (int j = 0; j < 32; ++j) v[j] += b[j];
+        for (int j = 0; j < 32; j += 2) f2_get(add2(f2(v[j], v[j + 1]), f2(b[j], b[j + 1])), v[j], v[j + 1]);
       }
       if (a.epi == MOE_GELU) {
         if (a.save_aux) slab_put_bf16(slab + 2048, lane, v);
 #pragma unroll
-        for (int j = 0; j < 32; ++j) v[j] = gelu_fast(v[j]);
+        for (int j = 0; j < 32; j += 2) f2_get(gelu2(f2(v[j], v[j + 1])), v[j], v[j + 1]);
       }
       slab_put_bf16(slab, lane, v);
       break;
@@ -664,7 +719,8 @@ __device__ __forceinline__ void moe_epi_chunk(const MoeGemmArgs& a, const CUtens
       if (staged) slab_get_bf16(staged, lane, h);
       else load_row32(a.aux_in + (long)(row0 + lane) * a.N, col, a.N, h);
 #pragma unroll
-      for (int j = 0; j < 32; ++j) v[j] *= gelu_grad_fast(h[j]);
+      for (int j = 0; j < 32; j += 2)
+        f2_get(mul2(f2(v[j], v[j + 1]), gelu_slope2(f2(h[j], h[j + 1]))), v[j], v[j + 1]);
       slab_put_bf16(slab, lane, v);
       break;
     }
@@ -678,14 +734,15 @@ __device__ __forceinline__ void moe_epi_chunk(const MoeGemmArgs& a, const CUtens
   if (a.epi == MOE_DGELU && a.sums != nullptr) {
     // lane: two columns of every other row, from the slab (as rounded); the two row halves meet in lanes 0-15
     const int cp = lane & 15, h = lane >> 4;
-    float s0 = 0.f, s1 = 0.f;
+    uint64_t acc = 0;
 #pragma unroll
     for (int i = 0; i < 16; ++i) {
       const int r = 2 * i + h;
       const uint32_t w = *reinterpret_cast<const uint32_t*>(slab + r * 64 + slab_unit_bf16(r, cp >> 2) * 16 + (cp & 3) * 4);
-      s0 += __uint_as_float(w << 16);
-      s1 += __uint_as_float(w & 0xffff0000u);
+      acc = add2(acc, f2(__uint_as_float(w << 16), __uint_as_float(w & 0xffff0000u)));
     }
+    float s0, s1;
+    f2_get(acc, s0, s1);
     s0 += __shfl_xor_sync(0xffffffffu, s0, 16);
     s1 += __shfl_xor_sync(0xffffffffu, s1, 16);
     if (h == 0 && col + 2 * cp < a.N)
@@ -1117,6 +1174,168 @@ __global__ void __maxnreg__(DTB_CORESIDENT_MAXNREG)
   }
 }
 
+// -------------------------------------------------------------------------
+// Forward products for few rows an expert (generation with a batch): 64-row tiles with the
+// operands swapped, out^T = W_e^T . rows^T.  The weights' 128 columns are the M side of the
+// tile (MN-major), up to 64 rows the N side, so a k-block is 16 KB of weights and 8 KB of
+// rows instead of 32 KB and 16 KB for rows that are mostly padding; two CTAs an SM keep
+// 192 KB in flight.  A CTA makes one tile over one part of K: the first product all of it,
+// with the activation; the second leaves fp32 parts that moe_thin_combine joins.  Bound by
+// the weights' way from DRAM.  48 tokens x 2 of 8 experts, 1024 x 4096: 11 + 10 us a product
+// (67 MB each), where the 128-row tiles took 25 + 25.
+struct MoeThinCfg {
+  static constexpr int A_BYTES = 128 * kBK * 2;
+  static constexpr int B_BYTES = kRowPad * kBK * 2;
+  static constexpr int STAGE_BYTES = A_BYTES + B_BYTES;
+  static constexpr int STAGES = 4;
+  static constexpr int SMEM_BYTES = STAGES * STAGE_BYTES + 1024 /*align*/ + 128 /*barriers*/;
+  static constexpr int THREADS = 192;
+};
+struct MoeThinArgs {
+  const int4* tile;
+  const int* off;
+  int E, N, K, splits;
+  const bf16* bias;  // act: [E, N] or null
+  bf16* act;         // [R, N] = gelu(acc + bias), or
+  float* part;       // [splits, R, N] = acc
+  long R;
+};
+
+__global__ void __launch_bounds__(MoeThinCfg::THREADS)
+    moe_thin_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_constant__ CUtensorMap tmX, MoeThinArgs a) {
+  using Cfg = MoeThinCfg;
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  uint64_t* full_bar = reinterpret_cast<uint64_t*>(smem + Cfg::STAGES * Cfg::STAGE_BYTES);
+  uint64_t* empty_bar = full_bar + Cfg::STAGES;
+  uint64_t* done_bar = empty_bar + Cfg::STAGES;
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(done_bar + 1);
+  volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < Cfg::STAGES; ++s) {
+      mbar_init(&full_bar[s], 1);
+      mbar_init(&empty_bar[s], 1);
+    }
+    mbar_init(done_bar, 1);
+    *abort_flag = 0;
+    fence_barrier_init();
+    tma_prefetch_desc(&tmW);
+    tma_prefetch_desc(&tmX);
+  }
+  if (warp == 1) tmem_alloc(tmem_slot, kRowPad);
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = *tmem_slot;
+  pdl_wait();
+  pdl_launch();
+
+  const int nt = (a.N + 127) / 128;
+  const int per = nt * a.splits;
+  const int ti = blockIdx.x / per, ni = blockIdx.x % per / a.splits, sp = blockIdx.x % a.splits;
+  const bool there = ti < __ldcg(a.off + a.E) / kRowPad;
+  if (there) {
+    const int4 t = __ldcg(a.tile + ti);
+    const int n0 = ni * 128;
+    const int kbs = (a.K + kBK - 1) / kBK;
+    const int kb0 = (int)((long)kbs * sp / a.splits), kb1 = (int)((long)kbs * (sp + 1) / a.splits);
+    if (warp == 0) {
+      if (lane == 0) {
+        int stage = 0;
+        uint32_t phase = 0;
+        for (int kb = kb0; kb < kb1; ++kb) {
+          if (!mbar_wait(&empty_bar[stage], phase ^ 1, abort_flag)) break;
+          uint8_t* sA = smem + stage * Cfg::STAGE_BYTES;
+          mbar_arrive_expect_tx(&full_bar[stage], Cfg::STAGE_BYTES);
+          tma_load_3d(&tmW, sA, &full_bar[stage], n0, kb * kBK, t.x);
+          tma_load_3d(&tmW, sA + 8192, &full_bar[stage], n0 + 64, kb * kBK, t.x);
+          tma_load_2d(&tmX, sA + Cfg::A_BYTES, &full_bar[stage], kb * kBK, t.y);
+          if (++stage == Cfg::STAGES) { stage = 0; phase ^= 1; }
+        }
+      }
+    } else if (warp == 1) {
+      if (lane == 0) {
+        constexpr uint32_t idesc = make_idesc_bf16(128, kRowPad, true, false);
+        int stage = 0;
+        uint32_t phase = 0;
+        bool ok = true;
+        for (int kb = kb0; kb < kb1; ++kb) {
+          if (!mbar_wait(&full_bar[stage], phase, abort_flag)) { ok = false; break; }
+          tc_fence_after();
+          const uint32_t aBase = smem_u32(smem + stage * Cfg::STAGE_BYTES);
+          const uint32_t bBase = aBase + Cfg::A_BYTES;
+#pragma unroll
+          for (int kk = 0; kk < kBK / 16; ++kk)
+            tc_mma_f16(tmem, make_sw128_desc(aBase + kk * 2048, 8192, 1024), make_sw128_desc(bBase + kk * 32, 16, 1024),
+                       idesc, (kb > kb0 || kk > 0) ? 1u : 0u);
+          tc_commit(&empty_bar[stage]);
+          if (++stage == Cfg::STAGES) { stage = 0; phase ^= 1; }
+        }
+        if (ok) tc_commit(done_bar);
+      }
+    } else {
+      // lane = a column of the output, TMEM column = a row
+      const int col = n0 + (warp & 3) * 32 + lane;
+      const int rows = min(kRowPad, t.z - t.y);
+      if (mbar_wait(done_bar, 0, abort_flag)) {
+        tc_fence_after();
+        const float b = a.bias && col < a.N ? bf2f(a.bias[(long)t.x * a.N + col]) : 0.f;
+#pragma unroll 1
+        for (int h = 0; h < kRowPad; h += 32) {
+          if (h >= rows) break;
+          float v[32];
+          tmem_ld32(tmem + ((uint32_t)((warp & 3) * 32) << 16) + h, v);
+          if (col < a.N) {
+#pragma unroll
+            for (int j = 0; j < 32; ++j) {
+              if (h + j >= rows) break;
+              if (a.act) a.act[(long)(t.y + h + j) * a.N + col] = f2bf(gelu_fast(v[j] + b));
+              else a.part[((long)sp * a.R + t.y + h + j) * a.N + col] = v[j];
+            }
+          }
+        }
+      }
+    }
+  }
+  tc_fence_before();
+  __syncthreads();
+  if (warp == 1) {
+    tc_fence_after();
+    tmem_dealloc(tmem, kRowPad);
+  }
+}
+
+// y[n] = sum_j gate_j (sum of the row's parts + b2_e): a thread per four columns.
+template <typename I, typename G>
+__global__ void __launch_bounds__(128)
+    moe_thin_combine_kernel(const float* __restrict__ part, const bf16* __restrict__ b2, const I* __restrict__ idx,
+                            const G* __restrict__ gates, bf16* __restrict__ y, MoePlan pl, int E, int Co, int k,
+                            int splits, long R) {
+  pdl_wait();
+  const long n = blockIdx.x;
+  const int c = (blockIdx.y * 128 + threadIdx.x) * 4;
+  if (c >= Co) return;
+  float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+  for (int j = 0; j < k; ++j) {
+    const int r = __ldcg(pl.inv + n * k + j);
+    if (r < 0) continue;
+    const float g = load_gate(gates, n * k + j);
+    float4 s = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 4
+    for (int p = 0; p < splits; ++p) {
+      const float4 v = __ldcg(reinterpret_cast<const float4*>(part + ((long)p * R + r) * Co + c));
+      s.x += v.x; s.y += v.y; s.z += v.z; s.w += v.w;
+    }
+    if (b2) {
+      const bf16* b = b2 + (long)slot_expert(idx, n * k + j, E) * Co + c;
+      s.x += bf2f(b[0]); s.y += bf2f(b[1]); s.z += bf2f(b[2]); s.w += bf2f(b[3]);
+    }
+    acc.x = fmaf(g, s.x, acc.x); acc.y = fmaf(g, s.y, acc.y); acc.z = fmaf(g, s.z, acc.z); acc.w = fmaf(g, s.w, acc.w);
+  }
+  *reinterpret_cast<uint2*>(y + n * Co + c) = make_uint2(pack_bf16x2(acc.x, acc.y), pack_bf16x2(acc.z, acc.w));
+}
+
 // ------------------------------------------------------------------ host
 // 3-D bf16 operand map over [depth, rows, cols], 128B swizzle: a box never leaves its expert's matrix
 // (rows and columns past its end read as zeros).
@@ -1334,6 +1553,8 @@ static MoeSizes check_experts(const at::Tensor& x, const at::Tensor& w1, const s
 // Up to this many slots go the streaming way: each slot reads its expert's weights, so it loses once many
 // slots share experts.
 constexpr long kFewSlots = 16;
+// Up to this many rows an expert on average, the 64-row tiles.
+constexpr long kThinRows = 48;
 
 template <typename I, typename G>
 static void moe_few_launch(const bf16* x, const bf16* w1, const bf16* b1, const bf16* w2, const bf16* b2, const I* idx,
@@ -1389,6 +1610,62 @@ static void moe_few(const at::Tensor& x, const at::Tensor& w1, const bf16* b1, c
   else go(pl, bptr(gates));
 }
 
+// Programmatic dependent launch of `kern` on `st` (common shape of the launches below).
+template <typename... Args, typename... Given>
+static void launch_pdl(void (*kern)(Args...), dim3 grid, int threads, int smem, cudaStream_t st, Given&&... given) {
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = grid;
+  cfg.blockDim = dim3(threads, 1, 1);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = st;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  C10_CUDA_CHECK(cudaLaunchKernelEx(&cfg, kern, Args(given)...));
+  count_launch();
+}
+
+// Few rows an expert, without a gradient: the plan is built, `rows` holds xp [R, C] and act [R, H].
+static void moe_thin(const at::Tensor& x, const at::Tensor& w1, const bf16* b1, const at::Tensor& w2, const bf16* b2,
+                     const at::Tensor& idx, const at::Tensor& gates, const at::Tensor& y, const MoePlan& pl,
+                     const MoeSizes& z, cudaStream_t st) {
+  static bool attr_set = false;
+  if (!attr_set) {
+    cudaFuncSetAttribute(moe_thin_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, MoeThinCfg::SMEM_BYTES);
+    attr_set = true;
+  }
+  const int C = (int)w1.size(1), H = (int)w1.size(2), Co = (int)w2.size(2), E = (int)z.E;
+  // K is split until there are two CTAs an SM (as many tiles as experts that can have a row), 256 of K a part at least
+  const long busy = std::min(z.P, z.E) * ((Co + 127) / 128);
+  const int splits = (int)std::max<long>(1, std::min<long>({296 / busy, (H + 255) / 256, 16}));
+  const long tiles = z.R / kRowPad;
+  auto rows = at::empty({z.R * (C + H)}, x.options());
+  auto part = at::empty({splits * z.R * Co}, x.options().dtype(at::kFloat));
+  bf16 *xp = bptr_mut(rows), *act = xp + z.R * C;
+  launch_pdl(moe_gather_kernel, dim3(warp_grid(z.R)), 256, 0, st, bptr(x), xp, pl, E, C, (int)z.k);
+  MoeThinArgs a{pl.tile3, pl.off, E, H, C, 1, b1, act, nullptr, z.R};
+  launch_pdl(moe_thin_kernel, dim3((unsigned)(tiles * ((H + 127) / 128))), MoeThinCfg::THREADS, MoeThinCfg::SMEM_BYTES, st,
+             make_map3(bptr(w1), z.E, C, H, 64, 64), make_map(xp, z.R, C, C, 64, kRowPad), a);
+  a = MoeThinArgs{pl.tile3, pl.off, E, Co, H, splits, nullptr, nullptr, part.data_ptr<float>(), z.R};
+  launch_pdl(moe_thin_kernel, dim3((unsigned)(tiles * ((Co + 127) / 128) * splits)), MoeThinCfg::THREADS,
+             MoeThinCfg::SMEM_BYTES, st, make_map3(bptr(w2), z.E, H, Co, 64, 64), make_map(act, z.R, H, H, 64, kRowPad), a);
+  const auto go = [&](auto* i, auto* g) {
+    using I = std::remove_const_t<std::remove_pointer_t<decltype(i)>>;
+    using G = std::remove_const_t<std::remove_pointer_t<decltype(g)>>;
+    launch_pdl(moe_thin_combine_kernel<I, G>, dim3((unsigned)z.n, (unsigned)((Co + 511) / 512)), 128, 0, st,
+               part.data_ptr<float>(), b2, i, g, bptr_mut(y), pl, E, Co, (int)z.k, splits, z.R);
+  };
+  const bool i32 = idx.scalar_type() == at::kInt, f32 = gates.scalar_type() == at::kFloat;
+  const int* pi = i32 ? idx.const_data_ptr<int>() : nullptr;
+  const long* pj = i32 ? nullptr : reinterpret_cast<const long*>(idx.const_data_ptr<int64_t>());
+  if (i32 && f32) go(pi, gates.const_data_ptr<float>());
+  else if (i32) go(pi, bptr(gates));
+  else if (f32) go(pj, gates.const_data_ptr<float>());
+  else go(pj, bptr(gates));
+}
+
 // What the backward reads of the forward, in one bf16 buffer.
 struct MoeSaved {
   bf16 *xp, *pre, *act, *yp;
@@ -1435,6 +1712,10 @@ std::vector<at::Tensor> experts_fwd(at::Tensor x, at::Tensor w1, std::optional<a
   auto plan = at::empty({plan_ints(z.P, z.E)}, x.options().dtype(at::kInt));
   const MoePlan pl = plan_views(plan.data_ptr<int>(), z.P, z.E);
   moe_build_plan(idx, pl, z, st);
+  if (!save && z.P <= kThinRows * z.E) {
+    moe_thin(x, w1, bptr_opt(b1), w2, bptr_opt(b2), idx, gates, y, pl, z, st);
+    return {y};
+  }
   auto rows = at::empty({saved_numel(z, C, H, Co) - (save ? 0 : z.R * H)}, x.options());
   MoeSaved v = saved_views(rows, z, C, H);
   if (!save) {  // no pre-activations

@@ -253,6 +253,10 @@ def expert_mlp(x, w1, b1, w2, b2, idx, gates):
     x, the weights, the biases and the gates, each in its own type.  An expert that no
     slot names gets a gradient of zeros.
     """
+    if x.is_cuda:
+        y = K.experts(x, w1, b1, w2, b2, idx, gates)
+        if y is not None:
+            return y
     c = x.shape[-1]
     if w1.dim() != 3 or w2.dim() != 3 or w1.shape[1] != c or w2.shape[:2] != (w1.shape[0], w1.shape[2]):
         raise ValueError(f"expert_mlp: x {tuple(x.shape)}, w1 {tuple(w1.shape)} and w2 {tuple(w2.shape)} do not fit")
@@ -260,16 +264,9 @@ def expert_mlp(x, w1, b1, w2, b2, idx, gates):
         raise ValueError(f"expert_mlp: idx {tuple(idx.shape)} and gates {tuple(gates.shape)} must be x's rows by slots")
     if idx.dtype not in (torch.int32, torch.int64):
         raise ValueError(f"expert_mlp: idx must be int32 or int64, got {idx.dtype}")
-    co = w2.shape[2]
-    x2, idx2, gates2 = x.reshape(-1, c), idx.reshape(-1, idx.shape[-1]), gates.reshape(-1, idx.shape[-1])
-    ok = _fast(x, w1, w2) and (b1 is None or _fast(b1)) and (b2 is None or _fast(b2)) and gates.is_cuda
-    if ok and c % 8 == 0 and w1.shape[2] % 8 == 0 and co % 8 == 0 and w1.shape[0] <= 512 and idx.shape[-1] <= 32 \
-            and gates.dtype in (torch.float32, torch.bfloat16):
-        y = K.experts(x2.contiguous(), w1.contiguous(), None if b1 is None else b1.contiguous(), w2.contiguous(),
-                      None if b2 is None else b2.contiguous(), idx2.contiguous(), gates2.contiguous())
-    else:
-        y = _experts_math(x2, w1, b1, w2, b2, idx2, gates2)
-    return y if x.dim() == 2 else y.view(*x.shape[:-1], co)
+    k = idx.shape[-1]
+    y = _experts_math(x.reshape(-1, c), w1, b1, w2, b2, idx.reshape(-1, k), gates.reshape(-1, k))
+    return y.view(*x.shape[:-1], w2.shape[2])
 
 
 # ---------------------------------------------------------------- others

@@ -149,8 +149,9 @@ def route(logits, k, softmax, bias, groups, keep, top, renorm, scale):
     return lib().route(logits, k, softmax, bias, groups, keep, top, renorm, scale)
 
 
-def experts(x, w1, b1, w2, b2, idx, gates) -> torch.Tensor:
-    """The experts' products with autograd (csrc/autograd_ops.cpp); gradients in the tensors' own types."""
+def experts(x, w1, b1, w2, b2, idx, gates) -> torch.Tensor | None:
+    """The experts' products with autograd (csrc/autograd_ops.cpp), any leading shape and layout; gradients in
+    the tensors' own types.  None where the kernels do not take the inputs."""
     return lib().experts(x, w1, b1, w2, b2, idx, gates)
 
 
