@@ -50,14 +50,14 @@ struct MoePlan {
   int* count;  // [E] rows of each expert, without the padding
   int* inv;    // [P] row of a slot, -1: none
   int* src;    // [R] slot of a row, -1: padding
-  int* hist;   // [blocks, E] scratch
+  int* hist;   // [E, blocks] scratch: rows of each expert in a block of slots, then its first row there
 };
 static long moe_max_rows(long P, long E) {
   return (P + (kRowPad - 1) * std::min(P, E) + kRowPad - 1) / kRowPad * kRowPad;
 }
 static long moe_max_tiles(long P, long E) { return P / kBM + std::min(P, E); }
 constexpr int kPlanThreads = 256;
-constexpr int kPlanChunk = 2048;  // slots a block sorts: 8 warps x 256
+constexpr int kPlanChunk = 1024;  // slots a block sorts: 8 warps x 128
 static long plan_blocks(long P) { return std::max<long>(1, (P + kPlanChunk - 1) / kPlanChunk); }
 static long plan_ints(long P, long E) {
   return 8 * moe_max_tiles(P, E) + moe_max_rows(P, E) / kRowPad * 4 + 4 + (E + 1) + E + P + moe_max_rows(P, E) + plan_blocks(P) * E;
@@ -85,6 +85,7 @@ __device__ __forceinline__ int slot_expert(const I* idx, long s, int E) {
 template <typename I>
 __global__ void __launch_bounds__(kPlanThreads) moe_hist_kernel(const I* __restrict__ idx, long P, int E, MoePlan pl) {
   extern __shared__ int s_h[];
+  pdl_launch();
   for (int i = threadIdx.x; i < E; i += blockDim.x) s_h[i] = 0;
   __syncthreads();
   const long lo = (long)blockIdx.x * kPlanChunk, hi = min(P, lo + kPlanChunk);
@@ -94,7 +95,7 @@ __global__ void __launch_bounds__(kPlanThreads) moe_hist_kernel(const I* __restr
     else if (idx[s] >= (I)E) set_status(kStatusBadArgument);
   }
   __syncthreads();
-  for (int i = threadIdx.x; i < E; i += blockDim.x) pl.hist[(long)blockIdx.x * E + i] = s_h[i];
+  for (int i = threadIdx.x; i < E; i += blockDim.x) pl.hist[(long)i * gridDim.x + blockIdx.x] = s_h[i];
 }
 
 // Inclusive sums over the block's 512 threads of (a, b, c); every thread calls it.
@@ -135,20 +136,39 @@ __device__ __forceinline__ int plan_expert(const MoePlan& pl, int e, int E, int 
   return start;
 }
 
-// One block of 512 threads (one per expert): totals, offsets, and each block's start in its experts' rows.
+// One block of 512 threads: totals (a warp per expert over the blocks' counts), offsets (a thread per expert), and
+// each block's first row of its experts (a warp per expert again).
 __global__ void __launch_bounds__(kMoeMaxExperts) moe_offsets_kernel(int nb, int E, MoePlan pl) {
-  const int e = threadIdx.x;
-  int total = 0;
-  if (e < E)
-    for (int b = 0; b < nb; ++b) total += pl.hist[(long)b * E + e];
-  int at = plan_expert(pl, e, E, total);
-  if (e < E)
-    for (int b = 0; b < nb; ++b) {
-      const long h = (long)b * E + e;
-      const int c = pl.hist[h];
-      pl.hist[h] = at;
-      at += c;
+  __shared__ int s_e[kMoeMaxExperts];
+  pdl_wait();
+  pdl_launch();
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  for (int e = warp; e < E; e += kMoeMaxExperts / 32) {
+    int t = 0;
+    for (int b = lane; b < nb; b += 32) t += __ldcg(pl.hist + (long)e * nb + b);
+    t = __reduce_add_sync(0xffffffffu, t);
+    if (lane == 0) s_e[e] = t;
+  }
+  __syncthreads();
+  const int mine = threadIdx.x < E ? s_e[threadIdx.x] : 0;
+  const int start = plan_expert(pl, threadIdx.x, E, mine);
+  s_e[threadIdx.x] = start;
+  __syncthreads();
+  for (int e = warp; e < E; e += kMoeMaxExperts / 32) {
+    int at = s_e[e];
+    for (int b0 = 0; b0 < nb; b0 += 32) {
+      const long i = (long)e * nb + b0 + lane;
+      const int c = b0 + lane < nb ? __ldcg(pl.hist + i) : 0;
+      int sum = c;
+#pragma unroll
+      for (int o = 1; o < 32; o <<= 1) {
+        const int x = __shfl_up_sync(0xffffffffu, sum, o);
+        if (lane >= o) sum += x;
+      }
+      if (b0 + lane < nb) pl.hist[i] = at + sum - c;
+      at += __shfl_sync(0xffffffffu, sum, 31);
     }
+  }
 }
 
 // A warp gives the slots [base, base + count) their rows, in order; `next` holds its experts' next rows.
@@ -209,7 +229,7 @@ __global__ void __launch_bounds__(kMoeMaxExperts) moe_plan_kernel(const I* __res
   place_slots(idx, (long)warp * per, per, P, E, s_w + warp * E, pl);
 }
 
-// Each warp places 256 slots in a row: first it counts its experts, then (after the
+// Each warp places 128 slots in a row: first it counts its experts, then (after the
 // warps before it are known) it gives the slots their rows in order.
 template <typename I>
 __global__ void __launch_bounds__(kPlanThreads) moe_place_kernel(const I* __restrict__ idx, long P, int E, MoePlan pl) {
@@ -225,8 +245,10 @@ __global__ void __launch_bounds__(kPlanThreads) moe_place_kernel(const I* __rest
     if (e >= 0) atomicAdd(&mine[e], 1);
   }
   __syncthreads();
+  pdl_wait();
+  pdl_launch();
   for (int e = threadIdx.x; e < E; e += blockDim.x) {
-    int at = pl.hist[(long)blockIdx.x * E + e];
+    int at = __ldcg(pl.hist + (long)e * gridDim.x + blockIdx.x);
     for (int w = 0; w < W; ++w) {
       const int c = s_w[w * E + e];
       s_w[w * E + e] = at;
@@ -279,6 +301,7 @@ template <typename G>
 __global__ void __launch_bounds__(256)
     moe_combine_kernel(const bf16* __restrict__ yp, const G* __restrict__ gates, bf16* __restrict__ y, MoePlan pl,
                        int n, int C, int k) {
+  pdl_wait();
   const int lane = threadIdx.x & 31;
   for (int t = (blockIdx.x * blockDim.x + threadIdx.x) >> 5; t < n; t += (gridDim.x * blockDim.x) >> 5) {
     int row = -1;
@@ -317,7 +340,8 @@ __global__ void __launch_bounds__(256)
 // A block of 64 rows (one expert's) per CTA, 8 rows a warp: u = gate * dy[token],
 // d(gate) = dy[token] . yp[row], and the block's column sums of u (as rounded), from one
 // pass over the rows.  u is rounded to bf16: it is the tensor cores' operand in two products.
-// Q x 16 bytes a lane at a time, 256 Q columns.
+// Q x 16 bytes a lane at a time, 256 Q columns: whole rows up to 1024 columns.  (Two at a time for every width,
+// with twice the warps an SM, took 79 us where this takes 53, over 65536 rows of 768 columns.)
 template <typename G, int Q>
 __global__ void __launch_bounds__(256)
     moe_grad_rows_kernel(const bf16* __restrict__ dy, const bf16* __restrict__ yp, const G* __restrict__ gates,
@@ -325,6 +349,7 @@ __global__ void __launch_bounds__(256)
                          int C, int k, long P) {
   constexpr int kGradCols = 256 * Q;
   __shared__ float s_sum[8][kGradCols];
+  pdl_launch();
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int blocks = pl.off[E] / kRowPad;
   for (long s = (long)blockIdx.x * blockDim.x + threadIdx.x; s < P; s += (long)gridDim.x * blockDim.x)
@@ -410,6 +435,8 @@ struct JoinArgs {
 template <typename O>
 __global__ void __launch_bounds__(256) moe_join_sums_kernel(JoinArgs<O> first, JoinArgs<O> second, MoePlan pl) {
   __shared__ float s_sum[16][68];
+  pdl_wait();
+  pdl_launch();
   const JoinArgs<O> a = blockIdx.z == 0 ? first : second;
   const float* __restrict__ part = a.part;
   O* __restrict__ out = a.out;
@@ -809,6 +836,8 @@ __global__ void __maxnreg__(DTB_CORESIDENT_MAXNREG)
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem_base = *tmem_slot;
+  pdl_wait();
+  pdl_launch();
 
   const int nt = (args.N + BN - 1) / BN;
   const int mt = MODE == MOE_DW ? (args.M + kBM - 1) / kBM : __ldg(args.ntile);
@@ -1011,6 +1040,8 @@ __global__ void __maxnreg__(DTB_CORESIDENT_MAXNREG)
   cluster_sync_all();  // both CTAs' barriers initialised and TMEM allocated
   tc_fence_after();
   const uint32_t tmem_base = *tmem_slot;
+  pdl_wait();
+  pdl_launch();
 
   const int nt = (args.N + 255) / 256;
   const int mt = MODE == MOE_DW ? (args.M + 255) / 256 : __ldg(args.ntile);
@@ -1352,6 +1383,23 @@ static CUtensorMap make_map3(const void* base, long depth, long rows, long cols,
   return m;
 }
 
+// Programmatic dependent launch of `kern` on `st` (common shape of the launches below).
+template <typename... Args, typename... Given>
+static void launch_pdl(void (*kern)(Args...), dim3 grid, int threads, int smem, cudaStream_t st, Given&&... given) {
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = grid;
+  cfg.blockDim = dim3(threads, 1, 1);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = st;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  C10_CUDA_CHECK(cudaLaunchKernelEx(&cfg, kern, Args(given)...));
+  count_launch();
+}
+
 template <int BN, int MODE>
 static void launch_moe(const CUtensorMap& ta, const CUtensorMap& tb, const CUtensorMap& to, const CUtensorMap& tx,
                        const MoeGemmArgs& a, long units, cudaStream_t st) {
@@ -1362,9 +1410,7 @@ static void launch_moe(const CUtensorMap& ta, const CUtensorMap& tb, const CUten
     attr_set = true;
   }
   const int grid = (int)std::min<long>(units, num_sms());
-  kern<<<grid, kThreads, MoeCfg<BN>::SMEM_BYTES, st>>>(ta, tb, to, tx, a);
-  count_launch();
-  C10_CUDA_KERNEL_LAUNCH_CHECK();
+  launch_pdl(kern, dim3(grid), kThreads, MoeCfg<BN>::SMEM_BYTES, st, ta, tb, to, tx, a);
 }
 
 // Pairs that can be resident at once.
@@ -1406,12 +1452,14 @@ static void launch_moe2(const CUtensorMap& ta, const CUtensorMap& tb, const CUte
   cfg.blockDim = dim3(kThreads, 1, 1);
   cfg.dynamicSmemBytes = MoePairCfg::SMEM_BYTES;
   cfg.stream = st;
-  cudaLaunchAttribute attr[1];
+  cudaLaunchAttribute attr[2];
   attr[0].id = cudaLaunchAttributeClusterDimension;
   attr[0].val.clusterDim.x = 2;
   attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+  attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[1].val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = attr;
-  cfg.numAttrs = 1;
+  cfg.numAttrs = 2;
   C10_CUDA_CHECK(cudaLaunchKernelEx(&cfg, kern, ta, tb, to, tx, a));
   count_launch();
 }
@@ -1491,9 +1539,9 @@ static void moe_build_plan_of(const I* idx, const MoePlan& pl, const MoeSizes& z
     count_launch();
   } else {
     moe_hist_kernel<I><<<nb, kPlanThreads, E * 4, st>>>(idx, z.P, E, pl);
-    moe_offsets_kernel<<<1, kMoeMaxExperts, 0, st>>>(nb, E, pl);
-    moe_place_kernel<I><<<nb, kPlanThreads, 8 * E * 4, st>>>(idx, z.P, E, pl);
-    count_launch(3);
+    count_launch();
+    launch_pdl(moe_offsets_kernel, dim3(1), kMoeMaxExperts, 0, st, nb, E, pl);
+    launch_pdl(moe_place_kernel<I>, dim3(nb), kPlanThreads, 8 * E * 4, st, idx, z.P, E, pl);
   }
   C10_CUDA_KERNEL_LAUNCH_CHECK();
 }
@@ -1610,23 +1658,6 @@ static void moe_few(const at::Tensor& x, const at::Tensor& w1, const bf16* b1, c
   else go(pl, bptr(gates));
 }
 
-// Programmatic dependent launch of `kern` on `st` (common shape of the launches below).
-template <typename... Args, typename... Given>
-static void launch_pdl(void (*kern)(Args...), dim3 grid, int threads, int smem, cudaStream_t st, Given&&... given) {
-  cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = grid;
-  cfg.blockDim = dim3(threads, 1, 1);
-  cfg.dynamicSmemBytes = smem;
-  cfg.stream = st;
-  cudaLaunchAttribute attr[1];
-  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  attr[0].val.programmaticStreamSerializationAllowed = 1;
-  cfg.attrs = attr;
-  cfg.numAttrs = 1;
-  C10_CUDA_CHECK(cudaLaunchKernelEx(&cfg, kern, Args(given)...));
-  count_launch();
-}
-
 // Few rows an expert, without a gradient: the plan is built, `rows` holds xp [R, C] and act [R, H].
 static void moe_thin(const at::Tensor& x, const at::Tensor& w1, const bf16* b1, const at::Tensor& w2, const bf16* b2,
                      const at::Tensor& idx, const at::Tensor& gates, const at::Tensor& y, const MoePlan& pl,
@@ -1683,9 +1714,8 @@ static MoeSaved saved_views(const at::Tensor& t, const MoeSizes& z, long C, long
 template <typename G>
 static void moe_combine(const bf16* rows, const G* gates, const at::Tensor& y, long C, const MoePlan& pl,
                         const MoeSizes& z, cudaStream_t st) {
-  moe_combine_kernel<G><<<warp_grid(z.n), 256, 0, st>>>(rows, gates, bptr_mut(y), pl, (int)z.n, (int)C, (int)z.k);
-  count_launch();
-  C10_CUDA_KERNEL_LAUNCH_CHECK();
+  launch_pdl(moe_combine_kernel<G>, dim3(warp_grid(z.n)), 256, 0, st, rows, gates, bptr_mut(y), pl, (int)z.n, (int)C,
+             (int)z.k);
 }
 
 // Forward.  Returns [y] or, with `save`, [y, plan, rows] for experts_bwd.
@@ -1723,8 +1753,7 @@ std::vector<at::Tensor> experts_fwd(at::Tensor x, at::Tensor w1, std::optional<a
     v.pre = nullptr;
     v.yp = v.act + z.R * H;
   }
-  moe_gather_kernel<<<warp_grid(z.R), 256, 0, st>>>(bptr(x), v.xp, pl, (int)z.E, (int)C, (int)z.k);
-  count_launch();
+  launch_pdl(moe_gather_kernel, dim3(warp_grid(z.R)), 256, 0, st, bptr(x), v.xp, pl, (int)z.E, (int)C, (int)z.k);
   moe_rows_gemm(MOE_FWD, v.xp, bptr(w1), v.act, (int)H, (int)C, MOE_GELU, bptr_opt(b1), v.pre, nullptr, pl, z, st);
   moe_rows_gemm(MOE_FWD, v.act, bptr(w2), v.yp, (int)Co, (int)H, MOE_PLAIN, bptr_opt(b2), nullptr, nullptr, pl, z, st);
   if (gates.scalar_type() == at::kFloat) moe_combine(v.yp, gates.data_ptr<float>(), y, Co, pl, z, st);
@@ -1806,11 +1835,10 @@ std::vector<at::Tensor> experts_bwd(at::Tensor dy, at::Tensor x, at::Tensor w1, 
       JoinArgs<O> a{p1, o1, (int)H, 32}, b{p2, o2, (int)Co, kRowPad};
       const long widest = std::max(has1 ? H : 0, has2 ? Co : 0);
       const dim3 grid((unsigned)((widest + 63) / 64), (unsigned)z.E, has1 && has2 ? 2 : 1);
-      moe_join_sums_kernel<O><<<grid, 256, 0, st>>>(has1 ? a : b, b, pl);
+      launch_pdl(moe_join_sums_kernel<O>, grid, 256, 0, st, has1 ? a : b, b, pl);
     };
     if (wt == at::kFloat) join(has1 ? db1->data_ptr<float>() : nullptr, has2 ? db2->data_ptr<float>() : nullptr);
     else join(has1 ? bptr_mut(*db1) : nullptr, has2 ? bptr_mut(*db2) : nullptr);
-    count_launch();
   }
   moe_combine<float>(dxp, nullptr, dx, C, pl, z, st);
   return {dx, dgates};

@@ -396,19 +396,26 @@ __global__ void __launch_bounds__(256) route_bwd_kernel(RouteBwdArgs a) {
   const int base = lane * V;
   const int valid = max(0, min(V, a.e - base));
   const bool vec = a.vec && valid == V;
-  for (int t = (blockIdx.x * blockDim.x + threadIdx.x) >> 5; t < a.n; t += warps) {
+  int t = (blockIdx.x * blockDim.x + threadIdx.x) >> 5;
+  // the next token's choices are loaded while this one is worked on
+  int next_at = -1;
+  float next_G = 0.f;
+  const auto fetch = [&](int n) {
+    next_at = -1;
+    if (n < a.n && lane < a.k) {
+      next_at = a.idx[(long)n * a.k + lane];
+      next_G = a.dgates[(long)n * a.k + lane];
+    }
+  };
+  fetch(t);
+  for (; t < a.n; t += warps) {
     const T* row = reinterpret_cast<const T*>(a.logits) + (long)t * a.e;
     T* out = reinterpret_cast<T*>(a.dlogits) + (long)t * a.e;
-    int at = -1;
-    float G = 0.f, zj = 0.f;
-    if (lane < a.k) {
-      at = a.idx[(long)t * a.k + lane];
-      if (at >= a.e) at = -1;
-      if (at >= 0) {
-        G = a.dgates[(long)t * a.k + lane];
-        zj = load_logit(row + at);
-      }
-    }
+    int at = next_at < a.e ? next_at : -1;
+    if (at < 0) at = -1;
+    const float G = at >= 0 ? next_G : 0.f;
+    const float zj = at >= 0 ? load_logit(row + at) : 0.f;
+    fetch(t + warps);
     float w[V];
 #pragma unroll
     for (int v = 0; v < V; ++v) w[v] = 0.f;
