@@ -121,3 +121,34 @@ def test_clip_refusals():
     with pytest.raises(TypeError, match="floating"):
         clip_grads([torch.zeros(3, dtype=torch.int64)], 1.0)
     assert float(global_norm([])) == 0.0 and float(clip_grads([None], 1.0)) == 0.0
+
+
+def _example():
+    import importlib.util
+    import os
+    path = os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), "examples", "train_moe.py")
+    spec = importlib.util.spec_from_file_location("train_moe", path)
+    mod = importlib.util.module_from_spec(spec)
+    spec.loader.exec_module(mod)
+    return mod
+
+
+@pytest.mark.parametrize("score", ["softmax", "sigmoid"])
+def test_example_learns_cpu(score):
+    losses = _example().main(["--device", "cpu", "--steps", "12", "--batch", "4", "--ctx", "32", "--vocab", "32", "--dim",
+                              "32", "--experts", "4", "--layers", "1", "--lr", "5e-3", "--score", score])
+    assert losses[0] == pytest.approx(math.log(32), abs=0.2) and losses[-1] < losses[0] - 0.3
+
+
+def test_balance_moves_the_bias_against_the_load():
+    import numpy as np
+    from dtrain_b200.models.moe import MoE
+    m = MoE(8, 16, 4, 1, np.random.default_rng(0))
+    with torch.no_grad():
+        m.gate.zero_()
+    m(torch.randn(12, 8))                                 # equal scores: every token goes to expert 0
+    assert m.load.tolist() == [12, 0, 0, 0]
+    m.balance(0.1)
+    torch.testing.assert_close(m.bias, torch.tensor([-0.1, 0.1, 0.1, 0.1]))
+    m(torch.randn(12, 8))
+    assert m.load.tolist() == [0, 12, 0, 0]

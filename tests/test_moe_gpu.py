@@ -429,3 +429,31 @@ def test_clip_refusals_gpu():
     with pytest.raises(RuntimeError, match="device"):
         clip_grads([a, torch.zeros(3)], 1.0)
     assert float(global_norm([None, torch.full((4,), 2.0, device="cuda"), None])) == 4.0
+
+
+# ----------------------------------------------------------------------- together
+def test_example_learns_and_layer_matches_fp32():
+    import numpy as np
+
+    from dtrain_b200.models.moe import MoE
+    from test_moe import _example
+    losses = _example().main(["--device", "cuda", "--steps", "30", "--batch", "8", "--ctx", "64", "--vocab", "64",
+                              "--layers", "1"])
+    assert losses[0] == pytest.approx(math.log(64), abs=0.2) and losses[-1] < losses[0] - 0.5
+    # the layer's output and gradients against its fp64 math at the same choices
+    m = MoE(64, 128, 8, 2, np.random.default_rng(1), torch.bfloat16).cuda()
+    with torch.no_grad():
+        m.gate.mul_(20.0)
+    x = torch.randn(40, 64, device="cuda").bfloat16()
+    y = m(x)
+    gates, idx, _ = F.route(F.linear(x, m.gate), 2, bias=m.bias, score="sigmoid")
+    d = [t.detach().double() for t in (x, m.w1, m.b1, m.w2, m.b2)]
+    ref = experts64(*d, idx, gates.detach().to(torch.bfloat16).double())
+    assert _rel(y, ref) <= 2 * U
+    y.sum().backward()
+    assert all(p.grad is not None and torch.isfinite(p.grad).all() for p in m.parameters())
+    # generation's form: one token at a time gives what the batch gives, to the rounding of both
+    with torch.no_grad():
+        one = torch.cat([F.expert_mlp(x[i:i + 1], m.w1, m.b1, m.w2, m.b2, idx[i:i + 1], gates[i:i + 1].to(x.dtype))
+                         for i in range(8)])
+    assert _rel(one, ref[:8]) <= 2 * U
