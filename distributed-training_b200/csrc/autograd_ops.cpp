@@ -17,7 +17,8 @@ std::vector<torch::Tensor> experts_fwd(torch::Tensor x, torch::Tensor w1, c10::o
                                        torch::Tensor w2, c10::optional<torch::Tensor> b2, torch::Tensor idx,
                                        torch::Tensor gates, bool save);
 std::vector<torch::Tensor> experts_bwd(torch::Tensor dy, torch::Tensor x, torch::Tensor w1, torch::Tensor w2,
-                                       torch::Tensor gates, std::vector<torch::Tensor> saved, torch::Tensor dw1,
+                                       c10::optional<torch::Tensor> b2, torch::Tensor gates,
+                                       std::vector<torch::Tensor> saved, torch::Tensor dw1,
                                        c10::optional<torch::Tensor> db1, torch::Tensor dw2,
                                        c10::optional<torch::Tensor> db2);
 
@@ -63,11 +64,10 @@ struct ExpertsFn : public torch::autograd::Function<ExpertsFn> {
                           c10::optional<Variable> b2, Variable idx, Variable gates) {
     at::AutoDispatchBelowADInplaceOrView guard;
     auto out = experts_fwd(x, w1, b1, w2, b2, idx, gates, true);
-    variable_list keep{x, w1, w2, gates};
+    variable_list keep{x, w1, w2, gates, b2.has_value() ? *b2 : torch::Tensor()};
     keep.insert(keep.end(), out.begin() + 1, out.end());
     ctx->save_for_backward(keep);
     ctx->saved_data["b1"] = b1.has_value() && b1->defined();
-    ctx->saved_data["b2"] = b2.has_value() && b2->defined();
     ctx->set_materialize_grads(false);
     return out[0];
   }
@@ -80,9 +80,13 @@ struct ExpertsFn : public torch::autograd::Function<ExpertsFn> {
     auto dw1 = torch::empty_like(w1), dw2 = torch::empty_like(w2);
     c10::optional<torch::Tensor> db1, db2;
     if (ctx->saved_data["b1"].toBool()) db1 = torch::empty({w1.size(0), w1.size(2)}, w1.options());
-    if (ctx->saved_data["b2"].toBool()) db2 = torch::empty({w2.size(0), w2.size(2)}, w2.options());
-    auto d = experts_bwd(grads[0].contiguous(), x, w1, w2, gates,
-                         std::vector<torch::Tensor>(saved.begin() + 4, saved.end()), dw1, db1, dw2, db2);
+    c10::optional<torch::Tensor> b2;
+    if (saved[4].defined()) {
+      b2 = saved[4];
+      db2 = torch::empty_like(*b2);
+    }
+    auto d = experts_bwd(grads[0].contiguous(), x, w1, w2, b2, gates,
+                         std::vector<torch::Tensor>(saved.begin() + 5, saved.end()), dw1, db1, dw2, db2);
     out[0] = d[0];
     out[1] = dw1;
     if (db1) out[2] = *db1;

@@ -56,7 +56,8 @@ std::vector<torch::Tensor> experts_fwd(torch::Tensor x, torch::Tensor w1, c10::o
                                        torch::Tensor w2, c10::optional<torch::Tensor> b2, torch::Tensor idx,
                                        torch::Tensor gates, bool save);
 std::vector<torch::Tensor> experts_bwd(torch::Tensor dy, torch::Tensor x, torch::Tensor w1, torch::Tensor w2,
-                                       torch::Tensor gates, std::vector<torch::Tensor> saved, torch::Tensor dw1,
+                                       c10::optional<torch::Tensor> b2, torch::Tensor gates,
+                                       std::vector<torch::Tensor> saved, torch::Tensor dw1,
                                        c10::optional<torch::Tensor> db1, torch::Tensor dw2,
                                        c10::optional<torch::Tensor> db2);
 // autograd_ops.cpp
@@ -180,7 +181,7 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("route_bwd", &route_bwd);
   m.def("experts_fwd", &experts_fwd, py::arg("x"), py::arg("w1"), py::arg("b1"), py::arg("w2"), py::arg("b2"),
         py::arg("idx"), py::arg("gates"), py::arg("save"));
-  m.def("experts_bwd", &experts_bwd, py::arg("dy"), py::arg("x"), py::arg("w1"), py::arg("w2"), py::arg("gates"),
+  m.def("experts_bwd", &experts_bwd, py::arg("dy"), py::arg("x"), py::arg("w1"), py::arg("w2"), py::arg("b2"), py::arg("gates"),
         py::arg("saved"), py::arg("dw1"), py::arg("db1"), py::arg("dw2"), py::arg("db2"));
   m.def("route", &route_autograd);
   m.def("experts", &experts_autograd);

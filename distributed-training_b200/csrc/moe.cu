@@ -6,14 +6,17 @@
 // rows start at a multiple of 64 and are padded with zero rows to the next one, so that
 // a k-block of 64 rows never mixes two experts' rows in the weight gradients.
 //
-//   moe_hist / moe_offsets / moe_place   the plan: a stable counting sort of the slots
+//   moe_plan          a stable counting sort of the slots by expert (three kernels for many slots)
 //   moe_gather        xp[r] = x[token of r]
-//   grouped GEMMs     pre = xp W1 + b1, act = gelu(pre) ; yp = act W2 + b2
-//   moe_combine       y[n] = sum_j gate_nj yp[row of (n, j)]
-//   moe_grad_rows     u[r] = gate dy[token of r],  dgate = dy . yp[r]
-//   grouped GEMMs     dpre = (u W2^T) gelu'(pre) ; dxp = dpre W1^T
-//   grouped GEMMs     dW2_e = act_e^T u_e ; dW1_e = xp_e^T dpre_e   (over the expert's rows)
-//   moe_join_sums     db2_e, db1_e from sums over blocks of rows that moe_grad_rows and the dpre GEMM leave
+//   grouped GEMMs     pre = xp W1 + b1, act = gate gelu(pre) ; yp = act W2 + gate b2
+//   moe_combine       y[n] = sum_j yp[row of (n, j)]
+//   moe_dy_rows       dyp[r] = dy[token of r], sums of gate dyp for db2, dyp . b2
+//   grouped GEMMs     t = dyp W2^T: dpre = gate t gelu'(pre), and t . gelu(pre) (d(gate), with dyp . b2) ; dxp = dpre W1^T
+//   grouped GEMMs     dW2_e = act_e^T dyp_e ; dW1_e = xp_e^T dpre_e   (over the expert's rows)
+//   moe_join_sums     db2_e, db1_e from sums over blocks of rows
+//   moe_combine       dx[n] = sum_j dxp[row of (n, j)], d(gate)
+//
+// The gates are applied in the epilogues, so the backward reads neither the rows' outputs nor a scaled copy of dy.
 //
 // The number of rows of each expert stays on the device: grids are sized by the most
 // tiles that the slots can fill, and the kernels read the real counts from the plan.
@@ -68,11 +71,11 @@ static MoePlan plan_views(int* p, long P, long E) {
   v.tile2 = v.tile + moe_max_tiles(P, E);
   v.tile3 = v.tile2 + moe_max_tiles(P, E);
   v.ntile = reinterpret_cast<int*>(v.tile3 + moe_max_rows(P, E) / kRowPad);
-  v.off = v.ntile + 4;
+  v.src = v.ntile + 4;
+  v.off = v.src + moe_max_rows(P, E);
   v.count = v.off + E + 1;
   v.inv = v.count + E;
-  v.src = v.inv + P;
-  v.hist = v.src + moe_max_rows(P, E);
+  v.hist = v.inv + P;
   return v;
 }
 
@@ -295,131 +298,129 @@ __global__ void __launch_bounds__(256)
   }
 }
 
-// One warp per token: y = sum over its slots of gate * yp[row] (gates null: of yp[row]).
-// The rows are read once, four slots' loads in flight a lane; bound by memory.
+// One warp per token: y = sum over its slots of rows[row].  The rows are read once, four slots' loads in
+// flight a lane; bound by memory.  In the backward also the token's d(gate): the parts of its row's
+// product that the dpre GEMM left, in order, and its product with the bias.
+struct GateParts {
+  const float* part;  // [parts, R], or null
+  const float* bias;  // [bias_parts, R], or null
+  int parts, bias_parts;
+  long R;
+};
 template <typename G>
 __global__ void __launch_bounds__(256)
-    moe_combine_kernel(const bf16* __restrict__ yp, const G* __restrict__ gates, bf16* __restrict__ y, MoePlan pl,
-                       int n, int C, int k) {
+    moe_combine_kernel(const bf16* __restrict__ rows, bf16* __restrict__ y, G* __restrict__ dgates, GateParts gp,
+                       MoePlan pl, int n, int C, int k) {
   pdl_wait();
   const int lane = threadIdx.x & 31;
   for (int t = (blockIdx.x * blockDim.x + threadIdx.x) >> 5; t < n; t += (gridDim.x * blockDim.x) >> 5) {
     int row = -1;
-    float gate = 1.f;
-    if (lane < k) {
-      row = pl.inv[(long)t * k + lane];
-      if (gates) gate = load_gate(gates, (long)t * k + lane);
-    }
+    if (lane < k) row = pl.inv[(long)t * k + lane];
     for (int c0 = 0; c0 < C / 8; c0 += 32) {
       const int c = c0 + lane;
       float acc[8] = {};
       for (int j = 0; j < k; j += 4) {
         uint4 u[4];
-        float g[4];
 #pragma unroll
         for (int q = 0; q < 4; ++q) {
           const int r = __shfl_sync(0xffffffffu, row, (j + q) & 31);
-          g[q] = __shfl_sync(0xffffffffu, gate, (j + q) & 31);
           const bool there = j + q < k && r >= 0 && c < C / 8;
-          if (!there) g[q] = 0.f;
-          u[q] = there ? __ldcs(reinterpret_cast<const uint4*>(yp + (long)r * C) + c) : make_uint4(0, 0, 0, 0);
+          u[q] = there ? __ldcs(reinterpret_cast<const uint4*>(rows + (long)r * C) + c) : make_uint4(0, 0, 0, 0);
         }
 #pragma unroll
         for (int q = 0; q < 4; ++q) {
           float v[8];
           unpack8(u[q], v);
 #pragma unroll
-          for (int i = 0; i < 8; ++i) acc[i] = fmaf(g[q], v[i], acc[i]);
+          for (int i = 0; i < 8; ++i) acc[i] += v[i];
         }
       }
       if (c < C / 8) *(reinterpret_cast<uint4*>(y + (long)t * C) + c) = pack8(acc);
     }
+    if (gp.part != nullptr && lane < k) {
+      float d = 0.f;
+      if (row >= 0) {
+#pragma unroll 8
+        for (int p = 0; p < gp.parts; ++p) d += gp.part[(long)p * gp.R + row];
+        if (gp.bias != nullptr)
+          for (int p = 0; p < gp.bias_parts; ++p) d += gp.bias[(long)p * gp.R + row];
+      }
+      store_gate(dgates, (long)t * k + lane, d);
+    }
   }
 }
 
-// A block of 64 rows (one expert's) per CTA, 8 rows a warp: u = gate * dy[token],
-// d(gate) = dy[token] . yp[row], and the block's column sums of u (as rounded), from one
-// pass over the rows.  u is rounded to bf16: it is the tensor cores' operand in two products.
-// Q x 16 bytes a lane at a time, 256 Q columns: whole rows up to 1024 columns.  (Two at a time for every width,
-// with twice the warps an SM, took 79 us where this takes 53, over 65536 rows of 768 columns.)
-template <typename G, int Q>
-__global__ void __launch_bounds__(256)
-    moe_grad_rows_kernel(const bf16* __restrict__ dy, const bf16* __restrict__ yp, const G* __restrict__ gates,
-                         bf16* __restrict__ u, G* __restrict__ dgates, float* __restrict__ sums, MoePlan pl, int E,
-                         int C, int k, long P) {
-  constexpr int kGradCols = 256 * Q;
-  __shared__ float s_sum[8][kGradCols];
+// A block of 64 rows (one expert's) and 256 columns per CTA, 8 rows a warp, 16 bytes a lane: dyp[r] = dy[token of r]
+// (zeros: padding) and, where the layer has b2, the column sums of gate * dyp (db2's parts) and the columns' part of
+// dyp . b2_e (for d(gate)).  Bound by the rows' way to DRAM; dy itself stays in L2.  Warps hide the loads' latency:
+// whole rows of 768 (2048) columns a CTA, with 128 (166) registers a thread, took 61 (162) us for 65536 (32768) rows.
+// (The grouped GEMMs could fetch the tokens' rows themselves, four a TMA gather, and no copy would be made.  The gather
+// moves a row of 128 bytes in 24 cycles an SM: the first product of 65536 rows x 1536, K 768, took 418 us that way and
+// takes 153 from a copy that costs 25.)
+template <typename G>
+__global__ void __launch_bounds__(256, 5)
+    moe_dy_rows_kernel(const bf16* __restrict__ dy, const bf16* __restrict__ b2, const G* __restrict__ gates,
+                       bf16* __restrict__ dyp, float* __restrict__ sums, float* __restrict__ dots, MoePlan pl, int E,
+                       int C, int k, long R) {
+  __shared__ float s_sum[8][256];
   pdl_launch();
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int blocks = pl.off[E] / kRowPad;
-  for (long s = (long)blockIdx.x * blockDim.x + threadIdx.x; s < P; s += (long)gridDim.x * blockDim.x)
-    if (pl.inv[s] < 0) store_gate(dgates, s, 0.f);
+  const int c0 = blockIdx.y * 256, c = c0 + lane * 8;
+  const bool in = c < C;
   for (int b = blockIdx.x; b < blocks; b += gridDim.x) {
     const int r0 = b * kRowPad + warp * 8;
     const int slot = lane < 8 ? pl.src[r0 + lane] : -1;
-    const float gate = slot >= 0 ? load_gate(gates, slot) : 0.f;
+    const float gate = b2 && slot >= 0 ? load_gate(gates, slot) : 0.f;
+    uint4 bv = make_uint4(0, 0, 0, 0);
+    if (b2 && in) bv = *reinterpret_cast<const uint4*>(b2 + (long)pl.tile3[b].x * C + c);
     float dot = 0.f;  // lane i: row i's
-    for (int c0 = 0; c0 < C; c0 += kGradCols) {
-      float acc[Q][8] = {};
-#pragma unroll 2
-      for (int i = 0; i < 8; ++i) {
-        const int s = __shfl_sync(0xffffffffu, slot, i);
-        const float g = __shfl_sync(0xffffffffu, gate, i);
-        const uint4* d = reinterpret_cast<const uint4*>(dy + (long)(max(s, 0) / k) * C + c0);
-        const uint4* o = reinterpret_cast<const uint4*>(yp + (long)(r0 + i) * C + c0);
-        uint4* dst = reinterpret_cast<uint4*>(u + (long)(r0 + i) * C + c0);
-        uint4 dv[Q], ov[Q];
+    float acc[8] = {};
 #pragma unroll
-        for (int q = 0; q < Q; ++q) {
-          const int c = lane + 32 * q;
-          const bool there = s >= 0 && c0 + c * 8 < C;
-          dv[q] = there ? d[c] : make_uint4(0, 0, 0, 0);
-          ov[q] = there ? __ldcs(o + c) : make_uint4(0, 0, 0, 0);
-        }
-        float p = 0.f;
+    for (int i0 = 0; i0 < 8; i0 += 4) {
+      uint4 u[4];
 #pragma unroll
-        for (int q = 0; q < Q; ++q) {
-          const int c = lane + 32 * q;
-          float a[8], w[8];
-          unpack8(dv[q], a);
-          unpack8(ov[q], w);
-#pragma unroll
-          for (int x = 0; x < 8; ++x) {
-            p = fmaf(a[x], w[x], p);
-            a[x] *= g;
-          }
-          if (s < 0) {
-#pragma unroll
-            for (int x = 0; x < 8; ++x) a[x] = 0.f;
-          }
-          const uint4 packed = pack8(a);
-          if (c0 + c * 8 < C) dst[c] = packed;
-          unpack8(packed, a);
-#pragma unroll
-          for (int x = 0; x < 8; ++x) acc[q][x] += a[x];
-        }
-#pragma unroll
-        for (int o2 = 16; o2; o2 >>= 1) p += __shfl_xor_sync(0xffffffffu, p, o2);
-        if (lane == i) dot += p;
+      for (int i = 0; i < 4; ++i) {
+        const int s = __shfl_sync(0xffffffffu, slot, i0 + i);
+        u[i] = s >= 0 && in ? __ldg(reinterpret_cast<const uint4*>(dy + (long)(s / k) * C + c)) : make_uint4(0, 0, 0, 0);
       }
-      if (sums != nullptr) {
 #pragma unroll
-        for (int q = 0; q < Q; ++q)
+      for (int i = 0; i < 4; ++i) {
+        if (in) *reinterpret_cast<uint4*>(dyp + (long)(r0 + i0 + i) * C + c) = u[i];
+        if (b2) {
+          const int s = __shfl_sync(0xffffffffu, slot, i0 + i);
+          const float g = __shfl_sync(0xffffffffu, gate, i0 + i);
+          float p = 0.f;
+          if (s >= 0) {  // a padding row takes part in no sum (the bias need not be finite)
+            float a[8], w[8];
+            unpack8(u[i], a);
+            unpack8(bv, w);
 #pragma unroll
-          for (int x = 0; x < 8; x += 4)
-            *reinterpret_cast<float4*>(&s_sum[warp][(lane + 32 * q) * 8 + x]) =
-                make_float4(acc[q][x], acc[q][x + 1], acc[q][x + 2], acc[q][x + 3]);
-        __syncthreads();
-        for (int c = threadIdx.x; c < kGradCols && c0 + c < C; c += 256) {
-          float t = 0.f;
+            for (int x = 0; x < 8; ++x) {
+              p = fmaf(a[x], w[x], p);
+              acc[x] = fmaf(g, a[x], acc[x]);
+            }
+          }
 #pragma unroll
-          for (int w = 0; w < 8; ++w) t += s_sum[w][c];
-          sums[(long)b * C + c0 + c] = t;
+          for (int o2 = 16; o2; o2 >>= 1) p += __shfl_xor_sync(0xffffffffu, p, o2);
+          if (lane == i0 + i) dot = p;
         }
-        __syncthreads();
       }
     }
-    if (lane < 8 && slot >= 0) store_gate(dgates, slot, dot);
+    if (b2) {
+#pragma unroll
+      for (int x = 0; x < 8; x += 4)
+        *reinterpret_cast<float4*>(&s_sum[warp][lane * 8 + x]) = make_float4(acc[x], acc[x + 1], acc[x + 2], acc[x + 3]);
+      __syncthreads();
+      if (c0 + (int)threadIdx.x < C) {
+        float t = 0.f;
+#pragma unroll
+        for (int w = 0; w < 8; ++w) t += s_sum[w][threadIdx.x];
+        sums[(long)b * C + c0 + threadIdx.x] = t;
+      }
+      __syncthreads();
+      if (lane < 8) dots[(long)blockIdx.y * R + r0 + lane] = dot;
+    }
   }
 }
 
@@ -620,9 +621,9 @@ enum MoeMode : int {
   MOE_DW = 2,   // out_e = A_e^T . B_e over the expert's rows
 };
 enum MoeEpi : int {
-  MOE_PLAIN = 0,  // out = acc [+ bias_e], bf16
-  MOE_GELU = 1,   // out = gelu(acc [+ bias_e]); aux = acc [+ bias_e] where asked for
-  MOE_DGELU = 2,  // out = acc * gelu'(aux)
+  MOE_PLAIN = 0,  // out = acc [+ gate * bias_e], bf16
+  MOE_GELU = 1,   // out = gate * gelu(acc [+ bias_e]); aux = acc [+ bias_e] where asked for
+  MOE_DGELU = 2,  // out = gate * acc * gelu'(aux), and the rows' products of acc with gelu(aux)
   MOE_F32 = 3,    // out = acc, fp32
 };
 struct MoeGemmArgs {
@@ -635,6 +636,11 @@ struct MoeGemmArgs {
   const bf16* aux_in;  // [R, N]
   int save_aux;
   float* sums;         // MOE_DGELU: [R / 32, N] column sums of each 32 rows of the output, or null
+  float* dots;         // MOE_DGELU: [2 x tiles of N, R] each row's product of acc and gelu(aux), a half tile a part
+  long R;
+  const int* src;      // slot of a row, and the gates by slot (their type): the rows' gates, or null
+  const void* gates;
+  int gates_f32;
 };
 
 // Where unit u of the grid lies: expert, first row and column of the tile, end of its rows, first row
@@ -651,11 +657,11 @@ __device__ __forceinline__ MoeUnit moe_unit(const MoeGemmArgs& a, int u, int mt,
     tile_coords(u - q.e * mt * nt, mt, nt, mi, ni);
     q.m0 = mi * BM;
     q.row_end = a.M;
-    q.r0 = __ldg(a.off + q.e);
-    q.kb = (__ldg(a.off + q.e + 1) - q.r0) / kBK;
+    q.r0 = __ldcg(a.off + q.e);
+    q.kb = (__ldcg(a.off + q.e + 1) - q.r0) / kBK;
   } else {
     tile_coords(u, mt, nt, mi, ni);
-    const int4 t = __ldg(a.tile + mi);
+    const int4 t = __ldcg(a.tile + mi);
     q.e = t.x;
     q.m0 = t.y;
     q.row_end = t.z;
@@ -704,12 +710,22 @@ __device__ __forceinline__ uint64_t gelu2(uint64_t x) {  // x / 2 (1 + t)
   const uint64_t h = mul2(x, f2s(0.5f));
   return fma2(h, gelu_tanh2(x, mul2(x, x)), h);
 }
-__device__ __forceinline__ uint64_t gelu_slope2(uint64_t x) {  // (1 + t) / 2 + x / 2 (1 - t^2) (c + 3 c3 x^2)
+// act = x / 2 (1 + t), slope = (1 + t) / 2 + x / 2 (1 - t^2) (c + 3 c3 x^2)
+__device__ __forceinline__ void gelu_both2(uint64_t x, uint64_t& act, uint64_t& slope) {
   const uint64_t x2 = mul2(x, x);
   const uint64_t t = gelu_tanh2(x, x2);
-  const uint64_t r = mul2(x, fma2(x2, f2s(1.5f * kGeluC3), f2s(0.5f * kGeluC)));
+  const uint64_t hx = mul2(x, f2s(0.5f));
+  act = fma2(hx, t, hx);
+  const uint64_t r = mul2(hx, fma2(x2, f2s(3.f * kGeluC3), f2s(kGeluC)));
   const uint64_t w = fma2(mul2(t, f2s(-1.f)), t, f2s(1.f));
-  return fma2(r, w, fma2(t, f2s(0.5f), f2s(0.5f)));
+  slope = fma2(r, w, fma2(t, f2s(0.5f), f2s(0.5f)));
+}
+
+__device__ __forceinline__ float row_gate(const MoeGemmArgs& a, int row) {
+  if (a.gates == nullptr) return 1.f;
+  const int s = __ldcg(a.src + row);
+  if (s < 0) return 0.f;
+  return a.gates_f32 ? reinterpret_cast<const float*>(a.gates)[s] : bf2f(reinterpret_cast<const bf16*>(a.gates)[s]);
 }
 
 // Unpack this lane's 64-byte row of a slab to fp32.
@@ -723,7 +739,7 @@ __device__ __forceinline__ void slab_get_bf16(const uint8_t* slab, int lane, flo
 // pre-activations, already in shared memory; null: read from global memory.
 __device__ __forceinline__ void moe_epi_chunk(const MoeGemmArgs& a, const CUtensorMap* tmOut, const CUtensorMap* tmAux,
                                               uint8_t* slab, int lane, int row0, int col, int e, bool dw, float* v,
-                                              const uint8_t* staged = nullptr) {
+                                              float gate, float& dot, const uint8_t* staged) {
   switch (a.epi) {
     case MOE_PLAIN:
     case MOE_GELU: {
@@ -731,12 +747,13 @@ __device__ __forceinline__ void moe_epi_chunk(const MoeGemmArgs& a, const CUtens
         float b[32];
         load_row32(a.bias + (long)e * a.N, col, a.N, b);
 #pragma unroll
-        for (int j = 0; j < 32; j += 2) f2_get(add2(f2(v[j], v[j + 1]), f2(b[j], b[j + 1])), v[j], v[j + 1]);
+        for (int j = 0; j < 32; j += 2)
+          f2_get(fma2(f2s(a.epi == MOE_PLAIN ? gate : 1.f), f2(b[j], b[j + 1]), f2(v[j], v[j + 1])), v[j], v[j + 1]);
       }
       if (a.epi == MOE_GELU) {
         if (a.save_aux) slab_put_bf16(slab + 2048, lane, v);
 #pragma unroll
-        for (int j = 0; j < 32; j += 2) f2_get(gelu2(f2(v[j], v[j + 1])), v[j], v[j + 1]);
+        for (int j = 0; j < 32; j += 2) f2_get(mul2(f2s(gate), gelu2(f2(v[j], v[j + 1]))), v[j], v[j + 1]);
       }
       slab_put_bf16(slab, lane, v);
       break;
@@ -745,9 +762,18 @@ __device__ __forceinline__ void moe_epi_chunk(const MoeGemmArgs& a, const CUtens
       float h[32];
       if (staged) slab_get_bf16(staged, lane, h);
       else load_row32(a.aux_in + (long)(row0 + lane) * a.N, col, a.N, h);
+      uint64_t d2 = 0;
 #pragma unroll
-      for (int j = 0; j < 32; j += 2)
-        f2_get(mul2(f2(v[j], v[j + 1]), gelu_slope2(f2(h[j], h[j + 1]))), v[j], v[j + 1]);
+      for (int j = 0; j < 32; j += 2) {
+        uint64_t act, slope;
+        const uint64_t acc = f2(v[j], v[j + 1]);
+        gelu_both2(f2(h[j], h[j + 1]), act, slope);
+        d2 = fma2(acc, act, d2);
+        f2_get(mul2(mul2(f2s(gate), acc), slope), v[j], v[j + 1]);
+      }
+      float da, db;
+      f2_get(d2, da, db);
+      dot += da + db;
       slab_put_bf16(slab, lane, v);
       break;
     }
@@ -840,7 +866,7 @@ __global__ void __maxnreg__(DTB_CORESIDENT_MAXNREG)
   pdl_launch();
 
   const int nt = (args.N + BN - 1) / BN;
-  const int mt = MODE == MOE_DW ? (args.M + kBM - 1) / kBM : __ldg(args.ntile);
+  const int mt = MODE == MOE_DW ? (args.M + kBM - 1) / kBM : __ldcg(args.ntile);
   const int units = MODE == MOE_DW ? args.E * mt * nt : mt * nt;
 
   if (warp == 0) {
@@ -934,6 +960,8 @@ __global__ void __maxnreg__(DTB_CORESIDENT_MAXNREG)
       const uint32_t tbase = tmem_base + ((uint32_t)(q4 * 32) << 16) + (uint32_t)(ab * BN);
       const int c_begin = half * (BN / 2), c_end = c_begin + BN / 2;
       if (row0 < q.row_end) {  // rows of the next expert (or past the matrix) are not this tile's
+        const float gate = MODE == MOE_DW ? 1.f : row_gate(args, row0 + lane);
+        float dot = 0.f;
 #pragma unroll 1
         for (int c = c_begin; c < c_end; c += 32) {
           if (q.n0 + c >= args.N) break;
@@ -946,9 +974,11 @@ __global__ void __maxnreg__(DTB_CORESIDENT_MAXNREG)
           }
           epi_slab_acquire(lane, dbl);
           moe_epi_chunk(args, &tmOut, &tmAux, slab + (dbl ? (ck & 1) * 2048 : 0), lane, row0, q.n0 + c, q.e,
-                        MODE == MOE_DW, v);
+                        MODE == MOE_DW, v, gate, dot, nullptr);
           ++ck;
         }
+        if (MODE == MOE_DX && args.dots != nullptr)
+          args.dots[(long)(q.n0 / (BN / 2) + half) * args.R + row0 + lane] = dot;
       }
       if (q.kb > 0) {
         tc_fence_before();
@@ -1044,7 +1074,7 @@ __global__ void __maxnreg__(DTB_CORESIDENT_MAXNREG)
   pdl_launch();
 
   const int nt = (args.N + 255) / 256;
-  const int mt = MODE == MOE_DW ? (args.M + 255) / 256 : __ldg(args.ntile);
+  const int mt = MODE == MOE_DW ? (args.M + 255) / 256 : __ldcg(args.ntile);
   const int units = MODE == MOE_DW ? args.E * mt * nt : mt * nt;
   const int pair = blockIdx.x >> 1, npairs = gridDim.x >> 1;
 
@@ -1160,6 +1190,8 @@ __global__ void __maxnreg__(DTB_CORESIDENT_MAXNREG)
         tc_fence_after();
       }
       const uint32_t tbase = tmem_base + ((uint32_t)(q4 * 32) << 16) + (uint32_t)(ab * 256 + half * 128);
+      const float gate = MODE == MOE_DW || row0 >= q.row_end ? 1.f : row_gate(args, row0 + lane);
+      float dot = 0.f;
 #pragma unroll 1
       for (int i = 0; i < chunks; ++i) {
         uint8_t* sl = slab + (ck & 1) * kEpiSlab;
@@ -1172,14 +1204,16 @@ __global__ void __maxnreg__(DTB_CORESIDENT_MAXNREG)
         }
         epi_slab_acquire(lane, true);
         if (stage_aux) mbar_wait(&abar[ck & 1], (ck >> 1) & 1, abort_flag);
-        moe_epi_chunk(args, &tmOut, &tmAux, sl, lane, row0, c0 + 32 * i, q.e, MODE == MOE_DW, v,
-                      stage_aux ? sl + 2048 : nullptr);
+        moe_epi_chunk(args, &tmOut, &tmAux, sl, lane, row0, c0 + 32 * i, q.e, MODE == MOE_DW, v, gate,
+                      dot, stage_aux ? sl + 2048 : nullptr);
         if (stage_aux && i + 2 < chunks && lane == 0) {  // every lane has read the buffer (moe_epi_chunk synchronises)
           mbar_arrive_expect_tx(&abar[ck & 1], 2048);
           tma_load_2d(&tmAux, sl + 2048, &abar[ck & 1], c0 + 32 * (i + 2), row0);
         }
         ++ck;
       }
+      if (MODE == MOE_DX && args.dots != nullptr && row0 < q.row_end)
+        args.dots[(long)(q.n0 / 128 + half) * args.R + row0 + lane] = dot;
       if (q.kb > 0) {
         tc_fence_before();
         __syncwarp();
@@ -1468,36 +1502,58 @@ struct MoeSizes {
   long n, k, P, E, R;  // tokens, slots a token, slots, experts, most padded rows
 };
 
-// rows [R, N] = rows [R, K] . W_e (MOE_FWD, w [E, K, N]) or . W_e^T (MOE_DX, w [E, N, K])
-static void moe_rows_gemm(int mode, const bf16* a, const bf16* w, bf16* out, int N, int K, int epi, const bf16* bias,
-                          bf16* aux, float* sums, const MoePlan& pl, const MoeSizes& z, cudaStream_t st) {
-  // 256-row pair tiles once the experts have 256 rows on average (below, half of a tile is padding)
-  const bool pair = N > 128 && z.P >= 256 * z.E;
+// What a grouped GEMM has beside its operands.
+struct MoeExtra {
+  int epi = MOE_PLAIN;
+  const bf16* bias = nullptr;
+  bf16* aux = nullptr;     // MOE_GELU: written, MOE_DGELU: read
+  float* sums = nullptr;
+  float* dots = nullptr;
+  const at::Tensor* gates = nullptr;
+};
+static MoeGemmArgs moe_args(const MoeExtra& x, const MoePlan& pl, const MoeSizes& z) {
   MoeGemmArgs g{};
   g.off = pl.off;
+  g.E = (int)z.E;
+  g.epi = x.epi;
+  g.bias = x.bias;
+  g.aux_in = x.aux;
+  g.save_aux = x.epi == MOE_GELU && x.aux != nullptr;
+  g.sums = x.sums;
+  g.dots = x.dots;
+  g.R = z.R;
+  g.src = pl.src;
+  if (x.gates) {
+    g.gates = x.gates->const_data_ptr();
+    g.gates_f32 = x.gates->scalar_type() == at::kFloat;
+  }
+  return g;
+}
+
+// Columns of an output tile: 128 where there are no more, else 256.
+static int moe_tile_n(int N) { return N <= 128 ? 128 : 256; }
+
+// rows [R, N] = rows [R, K] . W_e (MOE_FWD, w [E, K, N]) or . W_e^T (MOE_DX, w [E, N, K])
+static void moe_rows_gemm(int mode, const bf16* a, const bf16* w, bf16* out, int N, int K, const MoeExtra& x,
+                          const MoePlan& pl, const MoeSizes& z, cudaStream_t st) {
+  // 256-row pair tiles once the experts have 256 rows on average (below, half of a tile is padding)
+  const bool pair = N > 128 && z.P >= 256 * z.E;
+  MoeGemmArgs g = moe_args(x, pl, z);
   g.tile = pair ? pl.tile2 : pl.tile;
   g.ntile = pl.ntile + (pair ? 1 : 0);
-  g.sums = sums;
-  g.E = (int)z.E;
   g.N = N;
   g.K = K;
   g.M = 1;
-  g.epi = epi;
-  g.bias = bias;
-  g.aux_in = aux;
-  g.save_aux = epi == MOE_GELU && aux != nullptr;
-  const int bn = N <= 128 ? 128 : 256;
+  const int bn = moe_tile_n(N);
   const CUtensorMap ta = make_map(a, z.R, K, K, 64, kBM);
   const CUtensorMap tb = mode == MOE_FWD ? make_map3(w, z.E, K, N, 64, 64) : make_map3(w, z.E, N, K, 64, pair ? 128 : bn);
   const CUtensorMap to = make_store_map(out, false, z.R, N, N);
-  const CUtensorMap tx = aux ? make_store_map(aux, false, z.R, N, N) : to;
+  const CUtensorMap tx = x.aux ? make_store_map(x.aux, false, z.R, N, N) : to;
   const long units = moe_max_tiles(z.P, z.E) * ((N + bn - 1) / bn);
   if (pair) {
     if (mode == MOE_FWD) launch_moe2<MOE_FWD>(ta, tb, to, tx, g, units, st);
     else launch_moe2<MOE_DX>(ta, tb, to, tx, g, units, st);
-    return;
-  }
-  if (mode == MOE_FWD) {
+  } else if (mode == MOE_FWD) {
     if (bn == 256) launch_moe<256, MOE_FWD>(ta, tb, to, tx, g, units, st);
     else launch_moe<128, MOE_FWD>(ta, tb, to, tx, g, units, st);
   } else {
@@ -1507,16 +1563,15 @@ static void moe_rows_gemm(int mode, const bf16* a, const bf16* w, bf16* out, int
 }
 
 // out_e [M, N] (fp32 or bf16) = a_e^T . b_e over the expert's rows
-static void moe_weight_gemm(const bf16* a, const bf16* b, at::Tensor& out, int M, int N, const MoePlan& pl,
+static void moe_weight_gemm(const bf16* a, const bf16* b, const at::Tensor& out, int M, int N, const MoePlan& pl,
                             const MoeSizes& z, cudaStream_t st) {
-  MoeGemmArgs g{};
-  g.off = pl.off;
-  g.E = (int)z.E;
+  const bool f32 = out.scalar_type() == at::kFloat;
+  MoeExtra x;
+  x.epi = f32 ? MOE_F32 : MOE_PLAIN;
+  MoeGemmArgs g = moe_args(x, pl, z);
   g.M = M;
   g.N = N;
-  const bool f32 = out.scalar_type() == at::kFloat;
-  g.epi = f32 ? MOE_F32 : MOE_PLAIN;
-  const int bn = N <= 128 ? 128 : 256;
+  const int bn = moe_tile_n(N);
   const CUtensorMap ta = make_map(a, z.R, M, M, 64, 64);
   const CUtensorMap tb = make_map(b, z.R, N, N, 64, 64);
   const CUtensorMap to = make_store_map(out.data_ptr(), f32, M, N, N, z.E);
@@ -1697,27 +1752,6 @@ static void moe_thin(const at::Tensor& x, const at::Tensor& w1, const bf16* b1, 
   else go(pj, bptr(gates));
 }
 
-// What the backward reads of the forward, in one bf16 buffer.
-struct MoeSaved {
-  bf16 *xp, *pre, *act, *yp;
-};
-static long saved_numel(const MoeSizes& z, long C, long H, long Co) { return z.R * (C + 2 * H + Co); }
-static MoeSaved saved_views(const at::Tensor& t, const MoeSizes& z, long C, long H) {
-  MoeSaved v;
-  v.xp = bptr_mut(t);
-  v.pre = v.xp + z.R * C;
-  v.act = v.pre + z.R * H;
-  v.yp = v.act + z.R * H;
-  return v;
-}
-
-template <typename G>
-static void moe_combine(const bf16* rows, const G* gates, const at::Tensor& y, long C, const MoePlan& pl,
-                        const MoeSizes& z, cudaStream_t st) {
-  launch_pdl(moe_combine_kernel<G>, dim3(warp_grid(z.n)), 256, 0, st, rows, gates, bptr_mut(y), pl, (int)z.n, (int)C,
-             (int)z.k);
-}
-
 // Forward.  Returns [y] or, with `save`, [y, plan, rows] for experts_bwd.
 std::vector<at::Tensor> experts_fwd(at::Tensor x, at::Tensor w1, std::optional<at::Tensor> b1, at::Tensor w2,
                                     std::optional<at::Tensor> b2, at::Tensor idx, at::Tensor gates, bool save) {
@@ -1746,28 +1780,32 @@ std::vector<at::Tensor> experts_fwd(at::Tensor x, at::Tensor w1, std::optional<a
     moe_thin(x, w1, bptr_opt(b1), w2, bptr_opt(b2), idx, gates, y, pl, z, st);
     return {y};
   }
-  auto rows = at::empty({saved_numel(z, C, H, Co) - (save ? 0 : z.R * H)}, x.options());
-  MoeSaved v = saved_views(rows, z, C, H);
-  if (!save) {  // no pre-activations
-    v.act = v.pre;
-    v.pre = nullptr;
-    v.yp = v.act + z.R * H;
-  }
-  launch_pdl(moe_gather_kernel, dim3(warp_grid(z.R)), 256, 0, st, bptr(x), v.xp, pl, (int)z.E, (int)C, (int)z.k);
-  moe_rows_gemm(MOE_FWD, v.xp, bptr(w1), v.act, (int)H, (int)C, MOE_GELU, bptr_opt(b1), v.pre, nullptr, pl, z, st);
-  moe_rows_gemm(MOE_FWD, v.act, bptr(w2), v.yp, (int)Co, (int)H, MOE_PLAIN, bptr_opt(b2), nullptr, nullptr, pl, z, st);
-  if (gates.scalar_type() == at::kFloat) moe_combine(v.yp, gates.data_ptr<float>(), y, Co, pl, z, st);
-  else moe_combine(v.yp, bptr(gates), y, Co, pl, z, st);
+  // what the backward reads: the tokens' rows, the activations times their rows' gates, and the pre-activations
+  auto rows = at::empty({z.R * (C + H * (save ? 2 : 1))}, x.options());
+  auto yp = at::empty({z.R * Co}, x.options());
+  bf16 *xp = bptr_mut(rows), *act = xp + z.R * C;
+  launch_pdl(moe_gather_kernel, dim3(warp_grid(z.R)), 256, 0, st, bptr(x), xp, pl, (int)z.E, (int)C, (int)z.k);
+  MoeExtra up, down;
+  up.epi = MOE_GELU;
+  up.bias = bptr_opt(b1);
+  up.aux = save ? act + z.R * H : nullptr;
+  up.gates = &gates;
+  down.bias = bptr_opt(b2);
+  down.gates = down.bias ? &gates : nullptr;
+  moe_rows_gemm(MOE_FWD, xp, bptr(w1), act, (int)H, (int)C, up, pl, z, st);
+  moe_rows_gemm(MOE_FWD, act, bptr(w2), bptr_mut(yp), (int)Co, (int)H, down, pl, z, st);
+  launch_pdl(moe_combine_kernel<float>, dim3(warp_grid(z.n)), 256, 0, st, bptr(yp), bptr_mut(y), nullptr, GateParts{}, pl,
+             (int)z.n, (int)Co, (int)z.k);
   if (!save) return {y};
   return {y, plan, rows};
 }
 
 // Backward: returns [dx, dgates]; the weights' and biases' gradients are written to dw1, db1, dw2, db2
 // (all bf16 or all fp32; db1 / db2 only where the layer has the bias).
-std::vector<at::Tensor> experts_bwd(at::Tensor dy, at::Tensor x, at::Tensor w1, at::Tensor w2, at::Tensor gates,
-                                    std::vector<at::Tensor> saved, at::Tensor dw1, std::optional<at::Tensor> db1,
-                                    at::Tensor dw2, std::optional<at::Tensor> db2) {
-  const MoeSizes z = check_experts(x, w1, std::nullopt, w2, std::nullopt, gates);
+std::vector<at::Tensor> experts_bwd(at::Tensor dy, at::Tensor x, at::Tensor w1, at::Tensor w2, std::optional<at::Tensor> b2,
+                                    at::Tensor gates, std::vector<at::Tensor> saved, at::Tensor dw1,
+                                    std::optional<at::Tensor> db1, at::Tensor dw2, std::optional<at::Tensor> db2) {
+  const MoeSizes z = check_experts(x, w1, std::nullopt, w2, b2, gates);
   const long C = w1.size(1), H = w1.size(2), Co = w2.size(2);
   check_bf16(dy, x, "dy");
   TORCH_CHECK(dy.dim() == 2 && dy.size(0) == z.n && dy.size(1) == Co, "experts_bwd: dy must be [n, co]");
@@ -1780,6 +1818,7 @@ std::vector<at::Tensor> experts_bwd(at::Tensor dy, at::Tensor x, at::Tensor w1, 
                 "experts_bwd: ", what, " must be a contiguous, 16-byte aligned ", wt, " tensor of its weight's shape");
   };
   const bool has1 = db1 && db1->defined(), has2 = db2 && db2->defined();
+  TORCH_CHECK(has2 == (bptr_opt(b2) != nullptr), "experts_bwd: b2 and db2 go together");
   check_grad(dw1, w1.sizes(), "dw1");
   check_grad(dw2, w2.sizes(), "dw2");
   if (has1) check_grad(*db1, {z.E, H}, "db1");
@@ -1798,37 +1837,44 @@ std::vector<at::Tensor> experts_bwd(at::Tensor dy, at::Tensor x, at::Tensor w1, 
   }
   const at::Tensor &plan = saved[0], &rows = saved[1];
   TORCH_CHECK(plan.scalar_type() == at::kInt && plan.numel() == plan_ints(z.P, z.E) &&
-                  rows.scalar_type() == at::kBFloat16 && rows.numel() == saved_numel(z, C, H, Co),
+                  rows.scalar_type() == at::kBFloat16 && rows.numel() == z.R * (C + 2 * H),
               "experts_bwd: saved tensors of another forward");
   const MoePlan pl = plan_views(plan.data_ptr<int>(), z.P, z.E);
-  const MoeSaved v = saved_views(rows, z, C, H);
-  // scratch: u (later dx's rows) and dpre, and the column sums of blocks of rows
-  const long urows = z.R * std::max(C, Co), sums = has1 ? z.R / 32 * H : 0, sums2 = has2 ? z.R / kRowPad * Co : 0;
-  auto scratch = at::empty({urows + z.R * H + 2 * (sums + sums2)}, x.options());
-  bf16* u = bptr_mut(scratch);
-  bf16* dpre = u + urows;
-  bf16* dxp = u;
-  float* p1 = has1 ? reinterpret_cast<float*>(dpre + z.R * H) : nullptr;
-  float* p2 = has2 ? reinterpret_cast<float*>(dpre + z.R * H) + sums : nullptr;
-  const bf16* yp = v.yp;
-  const int gr = (int)std::min<long>(z.R / kRowPad, 1L << 16);
-  const int Q = (int)std::min<long>(4, (Co + 255) / 256);
-#define DTB_GRAD_ROWS(G, g, dg)                                                                                       \
-  if (Q == 1) moe_grad_rows_kernel<G, 1><<<gr, 256, 0, st>>>(bptr(dy), yp, g, u, dg, p2, pl, (int)z.E, (int)Co, (int)z.k, z.P); \
-  else if (Q == 2) moe_grad_rows_kernel<G, 2><<<gr, 256, 0, st>>>(bptr(dy), yp, g, u, dg, p2, pl, (int)z.E, (int)Co, (int)z.k, z.P); \
-  else if (Q == 3) moe_grad_rows_kernel<G, 3><<<gr, 256, 0, st>>>(bptr(dy), yp, g, u, dg, p2, pl, (int)z.E, (int)Co, (int)z.k, z.P); \
-  else moe_grad_rows_kernel<G, 4><<<gr, 256, 0, st>>>(bptr(dy), yp, g, u, dg, p2, pl, (int)z.E, (int)Co, (int)z.k, z.P);
-  if (gates.scalar_type() == at::kFloat) {
-    DTB_GRAD_ROWS(float, gates.data_ptr<float>(), dgates.data_ptr<float>())
-  } else {
-    DTB_GRAD_ROWS(bf16, bptr(gates), bptr_mut(dgates))
-  }
-#undef DTB_GRAD_ROWS
+  const bf16 *xp = bptr(rows), *act = xp + z.R * C;
+  bf16* pre = bptr_mut(rows) + z.R * (C + H);
+  // scratch: dpre, dy's rows (later dx's); fp32: the rows' products, the column sums of blocks of rows
+  const int parts = 2 * (int)((H + moe_tile_n((int)H) - 1) / moe_tile_n((int)H));
+  const int bparts = has2 ? (int)((Co + 255) / 256) : 0;
+  const long sums = has1 ? z.R / 32 * H : 0, sums2 = has2 ? z.R / kRowPad * Co : 0;
+  const long wide = std::max(C, Co);
+  auto scratch = at::empty({z.R * (H + wide) + 2 * (z.R * (parts + bparts) + sums + sums2)}, x.options());
+  bf16* dpre = bptr_mut(scratch);
+  bf16* dyp = dpre + z.R * H;
+  bf16* dxp = dyp;
+  float* dots = reinterpret_cast<float*>(dyp + z.R * wide);
+  float* bias_dots = has2 ? dots + z.R * parts : nullptr;
+  float* p1 = has1 ? dots + z.R * (parts + bparts) : nullptr;
+  float* p2 = has2 ? dots + z.R * (parts + bparts) + sums : nullptr;
+  const auto dy_rows = [&](auto* g) {
+    using G = std::remove_const_t<std::remove_pointer_t<decltype(g)>>;
+    const dim3 grid((unsigned)std::min<long>(z.R / kRowPad, 1L << 16), (unsigned)((Co + 255) / 256));
+    moe_dy_rows_kernel<G><<<grid, 256, 0, st>>>(bptr(dy), bptr_opt(b2), g, dyp, p2, bias_dots, pl, (int)z.E, (int)Co,
+                                                (int)z.k, z.R);
+  };
+  if (gates.scalar_type() == at::kFloat) dy_rows(gates.const_data_ptr<float>());
+  else dy_rows(bptr(gates));
   count_launch();
-  moe_rows_gemm(MOE_DX, u, bptr(w2), dpre, (int)H, (int)Co, MOE_DGELU, nullptr, v.pre, p1, pl, z, st);
-  moe_weight_gemm(v.act, u, dw2, (int)H, (int)Co, pl, z, st);
-  moe_rows_gemm(MOE_DX, dpre, bptr(w1), dxp, (int)C, (int)H, MOE_PLAIN, nullptr, nullptr, nullptr, pl, z, st);
-  moe_weight_gemm(v.xp, dpre, dw1, (int)C, (int)H, pl, z, st);
+  C10_CUDA_KERNEL_LAUNCH_CHECK();
+  MoeExtra back;
+  back.epi = MOE_DGELU;
+  back.aux = pre;
+  back.sums = p1;
+  back.dots = dots;
+  back.gates = &gates;
+  moe_rows_gemm(MOE_DX, dyp, bptr(w2), dpre, (int)H, (int)Co, back, pl, z, st);
+  moe_weight_gemm(act, dyp, dw2, (int)H, (int)Co, pl, z, st);
+  moe_rows_gemm(MOE_DX, dpre, bptr(w1), dxp, (int)C, (int)H, MoeExtra{}, pl, z, st);
+  moe_weight_gemm(xp, dpre, dw1, (int)C, (int)H, pl, z, st);
   if (has1 || has2) {
     const auto join = [&](auto* o1, auto* o2) {
       using O = std::remove_pointer_t<decltype(o1)>;
@@ -1840,7 +1886,14 @@ std::vector<at::Tensor> experts_bwd(at::Tensor dy, at::Tensor x, at::Tensor w1, 
     if (wt == at::kFloat) join(has1 ? db1->data_ptr<float>() : nullptr, has2 ? db2->data_ptr<float>() : nullptr);
     else join(has1 ? bptr_mut(*db1) : nullptr, has2 ? bptr_mut(*db2) : nullptr);
   }
-  moe_combine<float>(dxp, nullptr, dx, C, pl, z, st);
+  const GateParts gp{dots, bias_dots, parts, bparts, z.R};
+  const auto last = [&](auto* dg) {
+    using G = std::remove_pointer_t<decltype(dg)>;
+    launch_pdl(moe_combine_kernel<G>, dim3(warp_grid(z.n)), 256, 0, st, (const bf16*)dxp, bptr_mut(dx), dg, gp, pl, (int)z.n,
+               (int)C, (int)z.k);
+  };
+  if (gates.scalar_type() == at::kFloat) last(dgates.data_ptr<float>());
+  else last(bptr_mut(dgates));
   return {dx, dgates};
 }
 

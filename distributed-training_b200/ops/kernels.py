@@ -161,10 +161,10 @@ def experts_fwd(x, w1, b1, w2, b2, idx, gates, save: bool = False):
     return lib().experts_fwd(x, w1, b1, w2, b2, idx, gates, save)
 
 
-def experts_bwd(dy, x, w1, w2, gates, saved, dw1, db1, dw2, db2):
+def experts_bwd(dy, x, w1, w2, b2, gates, saved, dw1, db1, dw2, db2):
     """Returns (dx, dgates); writes the parameters' gradients into ``dw1`` .. ``db2``
     (all fp32 or all bf16; None for a bias that the layer has not)."""
-    return lib().experts_bwd(dy, x, w1, w2, gates, list(saved), dw1, db1, dw2, db2)
+    return lib().experts_bwd(dy, x, w1, w2, b2, gates, list(saved), dw1, db1, dw2, db2)
 
 
 def clip_grads(grads, out, max_norm: float, scale: bool = True) -> torch.Tensor:

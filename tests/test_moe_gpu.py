@@ -295,11 +295,11 @@ def test_experts_kernel_refusals():
     y, *saved = K.experts_fwd(*ok, save=True)
     g = [torch.empty_like(t[m]) for m in ("w1", "b1", "w2", "b2")]
     with pytest.raises(RuntimeError, match="experts_bwd"):
-        K.experts_bwd(dy[:, :32].contiguous(), t["x"], t["w1"], t["w2"], t["gates"], saved, *g)
+        K.experts_bwd(dy[:, :32].contiguous(), t["x"], t["w1"], t["w2"], t["b2"], t["gates"], saved, *g)
     with pytest.raises(RuntimeError, match="experts_bwd"):
-        K.experts_bwd(dy, t["x"], t["w1"], t["w2"], t["gates"], saved, g[0].float(), *g[1:])
+        K.experts_bwd(dy, t["x"], t["w1"], t["w2"], t["b2"], t["gates"], saved, g[0].float(), *g[1:])
     with pytest.raises(RuntimeError, match="experts_bwd"):
-        K.experts_bwd(dy, t["x"], t["w1"], t["w2"], t["gates"], saved[:1], *g)
+        K.experts_bwd(dy, t["x"], t["w1"], t["w2"], t["b2"], t["gates"], saved[:1], *g)
 
 
 def test_experts_bwd_fp32_weight_gradients():
@@ -307,8 +307,8 @@ def test_experts_bwd_fp32_weight_gradients():
     y, *saved = K.experts_fwd(**t, save=True)
     b = [torch.empty_like(t[m]) for m in ("w1", "b1", "w2", "b2")]
     f = [torch.empty_like(v, dtype=torch.float32) for v in b]
-    a = K.experts_bwd(dy, t["x"], t["w1"], t["w2"], t["gates"], saved, *b)
-    c = K.experts_bwd(dy, t["x"], t["w1"], t["w2"], t["gates"], saved, *f)
+    a = K.experts_bwd(dy, t["x"], t["w1"], t["w2"], t["b2"], t["gates"], saved, *b)
+    c = K.experts_bwd(dy, t["x"], t["w1"], t["w2"], t["b2"], t["gates"], saved, *f)
     assert all(torch.equal(p, q) for p, q in zip(a, c))
     assert all(torch.equal(p, q.to(torch.bfloat16)) for p, q in zip(b, f))
 
