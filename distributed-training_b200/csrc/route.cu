@@ -36,7 +36,7 @@ struct RouteArgs {
   int n, e, k;
   int groups, keep, top;
   int softmax, renorm;
-  int lanes;     // route_fwd_kernel: lanes of a group
+  int log_lanes; // route_fwd_kernel: log2 of a group's lanes
   int vec;       // its lanes' values start at 16-byte boundaries
   int need_sum;  // the softmax's sum takes part: not when the gates are renormalised over the row's largest
   float scale;
@@ -46,8 +46,8 @@ struct RouteArgs {
 // "taken or absent" (the key of -inf is above it).
 __device__ __forceinline__ unsigned order_key(float x) {
   if (x != x) return 0xffffffffu;
-  const unsigned b = __float_as_uint(x + 0.f);
-  return (b & 0x80000000u) ? ~b : (b | 0x80000000u);
+  const int b = __float_as_int(x + 0.f);
+  return (unsigned)(b ^ ((b >> 31) | (int)0x80000000));
 }
 constexpr unsigned kKeyNegInf = 0x007fffffu;
 __device__ __forceinline__ float key_value(unsigned k) {
@@ -157,8 +157,8 @@ __device__ __forceinline__ void store_logits(T* p, int valid, bool vec, const fl
 // heads of its lanes' lists by xor-shuffles, all groups at once, and each of the k rounds
 // takes the largest head of the warp (redux) and pops it.
 //
-// Bound by instruction issue: per token about 25 V for the scores, 5 V (V - 1) / 2 for the
-// sort and 18 a round.  The form that keeps the values unsorted and rescans V values a
+// Bound by instruction issue: per token about 28 V for scores and keys, 5 V (V - 1) / 2 for the
+// sort, 5 a group and 25 a round.  The form that keeps the values unsorted and rescans V values a
 // round (route_fwd_wide_kernel) costs 7 V a round and 10 V a group: it serves V > 8, where
 // the sort would cost more.
 template <typename T, int V>
@@ -169,7 +169,8 @@ __global__ void __launch_bounds__(256) route_fwd_kernel(RouteArgs a) {
   const int lane = threadIdx.x & 31;
   const int warps = (gridDim.x * blockDim.x) >> 5;
   const int per = a.e / a.groups;
-  const int group = lane / a.lanes, part = lane % a.lanes;  // lanes: of a group, a power of two
+  const int lanes = 1 << a.log_lanes;  // of a group
+  const int group = lane >> a.log_lanes, part = lane & (lanes - 1);
   const int base = group * per + part * V;
   const int valid = group < a.groups ? max(0, min(V, per - part * V)) : 0;
   const bool by_score = a.bias != nullptr || a.top == 2;
@@ -205,7 +206,7 @@ __global__ void __launch_bounds__(256) route_fwd_kernel(RouteArgs a) {
         if (a.bias != nullptr) c = __fadd_rn(c, bias[v]);
         if (z[v] == -INFINITY) c = -INFINITY;
       }
-      key[v] = v < valid ? order_key(c) : 0u;
+      key[v] = order_key(c);  // absent experts: -inf, as masked ones
       at[v] = v;
     }
 #pragma unroll
@@ -226,7 +227,7 @@ __global__ void __launch_bounds__(256) route_fwd_kernel(RouteArgs a) {
     if (a.groups > 1) {
       unsigned k1 = key[0], k2 = 0u;
       if constexpr (V > 1) k2 = key[1];
-      for (int o = 1; o < a.lanes; o <<= 1) {
+      for (int o = 1; o < lanes; o <<= 1) {
         const unsigned b1 = __shfl_xor_sync(kAll, k1, o), b2 = __shfl_xor_sync(kAll, k2, o);
         k2 = max(min(k1, b1), max(k2, b2));
         k1 = max(k1, b1);
@@ -234,16 +235,13 @@ __global__ void __launch_bounds__(256) route_fwd_kernel(RouteArgs a) {
       unsigned score = k1;
       if (a.top == 2 && k1 > kKeyNegInf && k2 > kKeyNegInf)
         score = order_key(__fadd_rn(key_value(k1), key_value(k2)));
-      if (part != 0 || group >= a.groups) score = 0u;  // one lane a group
-      unsigned kept = 0u;
-      for (int r = 0; r < a.keep; ++r) {
-        const unsigned best = __reduce_max_sync(kAll, score);
-        const int l = __ffs(__ballot_sync(kAll, score == best && part == 0 && group < a.groups &&
-                                                    !((kept >> group) & 1u))) - 1;
-        kept |= 1u << (l / a.lanes);
-        if (lane == l) score = 0u;
+      // the group's place among the groups: those with a larger score, or an equal one and a lower number
+      int place = 0;
+      for (int g = 0; g < a.groups; ++g) {
+        const unsigned other = __shfl_sync(kAll, score, g << a.log_lanes);
+        place += other > score || (other == score && g < group);
       }
-      if (!((kept >> group) & 1u)) {
+      if (place >= a.keep) {
 #pragma unroll
         for (int v = 0; v < V; ++v) key[v] = 0u;
       }
@@ -255,12 +253,11 @@ __global__ void __launch_bounds__(256) route_fwd_kernel(RouteArgs a) {
       const int l = __ffs(__ballot_sync(kAll, key[0] == best)) - 1;
       const int i = __shfl_sync(kAll, base + (int)(where & 15u), l);
       if (lane == j) mine = i;
-      if (lane == l) {
+      const bool pop = lane == l;
 #pragma unroll
-        for (int v = 0; v < V - 1; ++v) key[v] = key[v + 1];
-        key[V - 1] = 0u;
-        where >>= 4;
-      }
+      for (int v = 0; v < V - 1; ++v) key[v] = pop ? key[v + 1] : key[v];
+      key[V - 1] = pop ? 0u : key[V - 1];
+      where = pop ? where >> 4 : where;
     }
     route_finish(a, row, t, lane, mine, mx, sum, s_load);
   }
@@ -507,10 +504,9 @@ std::vector<at::Tensor> route_fwd(at::Tensor logits, int64_t k, bool softmax, st
   a.renorm = renorm;
   a.scale = (float)scale;
   a.need_sum = !(renorm && !a.bias && groups == 1 && top == 1);
-  int pow2 = 1;
-  while (pow2 < groups) pow2 *= 2;
-  a.lanes = 32 / pow2;
-  const long per = e / groups, v = (per + a.lanes - 1) / a.lanes;
+  a.log_lanes = 5;
+  while ((32 >> a.log_lanes) < groups) --a.log_lanes;
+  const long per = e / groups, lanes = 1 << a.log_lanes, v = (per + lanes - 1) / lanes;
   const int V = v <= 1 ? 1 : v <= 2 ? 2 : v <= 4 ? 4 : 8;
   const int es = f32 ? 4 : 2;
   a.vec = per % V == 0 && (V * es) % 16 == 0 && (e * es) % 16 == 0 &&
