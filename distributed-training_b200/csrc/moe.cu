@@ -474,9 +474,13 @@ __global__ void __launch_bounds__(256) moe_join_sums_kernel(JoinArgs<O> first, J
 //         up in order through distributed shared memory
 // `down` is launched while `up` runs (programmatic dependent launch) and asks for its weights
 // in L2 before it waits for h, so both matrices stream at once.  L is 4, 8 or 16 by
-// how many CTAs that makes.
+// how many CTAs that makes.  The loads' latency is hidden by warps (512 threads, 64 registers;
+// 256 threads took 26 us where this takes 19, 4 tokens of 16 experts 768 x 2048), and the last
+// batch of a thread's loads is issued at once like the others.  One token there takes 9.6 us
+// on the GPU for 12.6 MB (1.9 us at the copy rate): two launches, and in each the chain
+// expert, weights, sum.
 constexpr int kFewCluster = 8;
-constexpr int kFewThreads = 256;
+constexpr int kFewThreads = 512;
 
 // acc (8 columns a thread) summed over the CTA's 256 / L row lanes: s_out[0 .. 8 L), valid after the
 // __syncthreads that the caller does.
@@ -530,16 +534,15 @@ __global__ void __launch_bounds__(kFewThreads)
   if (col < H) {
     const uint4* w = reinterpret_cast<const uint4*>(w1 + (long)e * C * H + col);
     const long step = H / 8;
-    constexpr int U = 8;
-    int c = r;
-    for (; c + (U - 1) * R < C; c += U * R) {
+    constexpr int U = 6;  // loads in flight, the last batch's too
+    for (int c = r; c < C; c += U * R) {
       uint4 u[U];
 #pragma unroll
-      for (int j = 0; j < U; ++j) u[j] = __ldg(w + (c + j * R) * step);
+      for (int j = 0; j < U; ++j) u[j] = c + j * R < C ? __ldg(w + (c + j * R) * step) : make_uint4(0, 0, 0, 0);
 #pragma unroll
-      for (int j = 0; j < U; ++j) few_fma(acc, u[j], s_x[c + j * R]);
+      for (int j = 0; j < U; ++j)
+        if (c + j * R < C) few_fma(acc, u[j], s_x[c + j * R]);
     }
-    for (; c < C; c += R) few_fma(acc, __ldg(w + c * step), s_x[c]);
   }
   few_reduce<L>(acc, s_part, s_out);
   const int oc = blockIdx.x * 8 * L + threadIdx.x;
@@ -578,20 +581,20 @@ __global__ void __cluster_dims__(kFewCluster, 1, 1) __launch_bounds__(kFewThread
     const float g = load_gate(gates, n * k + j);
     const uint4* w = reinterpret_cast<const uint4*>(w2 + (long)e * H * Co + col);
     const float* hr = h + (n * k + j) * H;
-    constexpr int U = 8;
-    int c = lo + r;
-    for (; c + (U - 1) * R < hi; c += U * R) {
+    constexpr int U = 4;
+    for (int c = lo + r; c < hi; c += U * R) {
       uint4 u[U];
       float a[U];
 #pragma unroll
       for (int q = 0; q < U; ++q) {
-        u[q] = __ldg(w + (c + q * R) * step);
-        a[q] = __ldcg(hr + c + q * R);
+        const bool there = c + q * R < hi;
+        u[q] = there ? __ldg(w + (c + q * R) * step) : make_uint4(0, 0, 0, 0);
+        a[q] = there ? __ldcg(hr + c + q * R) : 0.f;
       }
 #pragma unroll
-      for (int q = 0; q < U; ++q) few_fma(acc, u[q], g * a[q]);
+      for (int q = 0; q < U; ++q)
+        if (c + q * R < hi) few_fma(acc, u[q], g * a[q]);
     }
-    for (; c < hi; c += R) few_fma(acc, __ldg(w + c * step), g * __ldcg(hr + c));
   }
   few_reduce<L>(acc, s_part, s_out);
   cluster_sync_all();
@@ -1653,9 +1656,12 @@ static MoeSizes check_experts(const at::Tensor& x, const at::Tensor& w1, const s
   return z;
 }
 
-// Up to this many slots go the streaming way: each slot reads its expert's weights, so it loses once many
-// slots share experts.
-constexpr long kFewSlots = 16;
+// Up to this many slots go the streaming way: each slot reads its expert's weights, so it loses once many slots share
+// experts.  Streaming against the 64-row tiles, in a CUDA graph with cold weights, two slots a token:
+//   1 token  of 16 experts 768 x 2048: 10.3 / 20.6 us,  of 8 experts 1024 x 4096: 15.7 / 27.0 us
+//   4 tokens                           19.0 / 27.7                                30.4 / 32.3
+//   8 tokens                           28.7 / 30.0                                49.6 / 36.3
+constexpr long kFewSlots = 8;
 // Up to this many rows an expert on average, the 64-row tiles.
 constexpr long kThinRows = 48;
 

@@ -158,6 +158,22 @@ def _inputs(n, c, h, co, e, k, bias=True, skew=0.0, gate=torch.bfloat16, idx_typ
     return t, r(n, co).to(bf)
 
 
+@pytest.mark.parametrize("n,c,h,co,e,k,bias", [(1, 768, 200, 136, 5, 2, True), (4, 72, 1032, 264, 6, 2, False),
+                                               (8, 200, 136, 72, 3, 1, True), (30, 264, 520, 200, 40, 3, True),
+                                               (100, 136, 1544, 72, 4, 2, False), (300, 72, 136, 200, 64, 8, True)])
+@pytest.mark.parametrize("gate,idx_type", [(torch.bfloat16, torch.int64), (torch.float32, torch.int32)])
+def test_expert_mlp_without_gradient(n, c, h, co, e, k, bias, gate, idx_type):
+    # the forms for a few slots and for few rows an expert
+    t, _ = _inputs(n, c, h, co, e, k, bias, 0.0, gate, idx_type)
+    if n > 1:
+        t["idx"][n - 1] = -1
+    y = F.expert_mlp(**t)
+    ref = experts64(**{m: v.double() if v is not None and v.is_floating_point() else v for m, v in t.items()})
+    assert _rel(y, ref) <= 2 * U
+    assert n == 1 or torch.all(y[n - 1] == 0)
+    assert torch.equal(y, F.expert_mlp(**t)), "fixed orders of summation"
+
+
 EXPERTS = [  # n, c, h, co, e, k, bias, skew
     (1, 64, 128, 64, 4, 2, True, 0.0),
     (1, 8, 8, 8, 1, 1, False, 0.0),
@@ -272,6 +288,16 @@ def test_expert_mlp_inf_and_nan_stay_in_their_rows():
     assert torch.isnan(y[7]).all() and not torch.isfinite(y[9]).all()
     rest = [i for i in range(40) if i not in (7, 9)]
     assert torch.isfinite(y[rest]).all()
+    # in the gradients they reach their own experts' weights only
+    t, dy = _inputs(300, 64, 64, 64, 4, 1)
+    t["x"][7] = math.nan
+    e = int(t["idx"][7, 0])
+    for m in ("x", "w1", "w2", "gates"):
+        t[m].requires_grad_()
+    F.expert_mlp(**t).backward(dy)
+    for q in range(4):
+        assert torch.isfinite(t["w1"].grad[q]).all() == (q != e) and torch.isfinite(t["w2"].grad[q]).all() == (q != e)
+    assert torch.isfinite(t["x"].grad[[i for i in range(300) if i != 7]]).all()
     # an expert that no token names may hold anything
     t, dy = _inputs(40, 64, 64, 64, 4, 1)
     t["idx"].clamp_(max=2)
