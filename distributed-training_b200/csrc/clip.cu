@@ -13,6 +13,11 @@
 // graph.  Each CTA of the first kernel sums its chunks in a fixed order into one fp64
 // partial; each CTA of the second adds the partials up in the same order, so every CTA
 // gets the same factor, and the result does not depend on scheduling.
+//
+// Bound by memory: the gradients are read twice (the norm has to be known before the first of
+// them is scaled) and written once.  406M fp32 gradients: norm 250 us (6.5 TB/s), scaling
+// 530 us (6.1 TB/s; it starts with the chunks that the norm left in L2); 266M bf16 ones into
+// fp32: 113 and 261 us.  A few small tensors: two launches, 7.5 us on the GPU.
 #include <ATen/core/Tensor.h>
 #include <ATen/ops/empty.h>
 #include <ATen/MemoryOverlap.h>

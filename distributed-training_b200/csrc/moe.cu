@@ -1009,6 +1009,11 @@ __global__ void __maxnreg__(DTB_CORESIDENT_MAXNREG)
 // Barriers as in the dense pair GEMM (gemm.cu): full (leader; both CTAs' bytes), empty and
 // tile-full (both, by the leader's commit), tile-empty (leader; both epilogues), done.
 // No load is multicast.
+//
+// Bound: at K 2048 by the tensor cores at the power limit (32768 rows x 2048 x 2048: 218 us a
+// product, 1.26 PFLOP/s, with an eighth of the tiles' rows padding; the dense pair GEMM of the
+// same size 190); at K 768 with an activation by the epilogue's issue slots and its two tensors
+// of rows x 1536 in DRAM (153 us forward, 179 backward; 112 us without them).
 __device__ __forceinline__ void tma_load_3d_pair(const CUtensorMap* map, void* dst, uint32_t leader_bar, int x, int y,
                                                  int z) {
   asm volatile(
@@ -1162,8 +1167,8 @@ __global__ void __maxnreg__(DTB_CORESIDENT_MAXNREG)
     uint64_t* abar = aux_bar + ew * 2;
     const uint32_t lead_tempty0 = mapa_shared(&tempty_bar[0], 0);
     // MOE_DGELU: a chunk's pre-activations come by TMA into the second half of its slab, two chunks ahead and
-    // the tile's first two before its products are done.  (Read by the lanes themselves, a row each, they cost
-    // the dpre GEMM of 65536 rows x 1536 columns, K 768, 224 us.)
+    // the tile's first two before its products are done.  (The dpre GEMM of 65536 rows x 1536, K 768, took 224 us
+    // with the lanes reading a row each and scalar arithmetic, 198 with TMA, 179 with two operations an instruction.)
     const bool stage_aux = MODE == MOE_DX && args.epi == MOE_DGELU;
     uint32_t ck = 0;
     int ab = 0;
@@ -1249,8 +1254,8 @@ __global__ void __maxnreg__(DTB_CORESIDENT_MAXNREG)
 // rows instead of 32 KB and 16 KB for rows that are mostly padding; two CTAs an SM keep
 // 192 KB in flight.  A CTA makes one tile over one part of K: the first product all of it,
 // with the activation; the second leaves fp32 parts that moe_thin_combine joins.  Bound by
-// the weights' way from DRAM.  48 tokens x 2 of 8 experts, 1024 x 4096: 11 + 10 us a product
-// (67 MB each), where the 128-row tiles took 25 + 25.
+// the weights' way from DRAM and five launches in a row: 48 tokens x 2 of 8 experts, 1024 x 4096
+// (134 MB of weights, 20.4 us at the copy rate), take 41 us in all, with the 128-row tiles 69.
 struct MoeThinCfg {
   static constexpr int A_BYTES = 128 * kBK * 2;
   static constexpr int B_BYTES = kRowPad * kBK * 2;
@@ -1539,7 +1544,9 @@ static int moe_tile_n(int N) { return N <= 128 ? 128 : 256; }
 // rows [R, N] = rows [R, K] . W_e (MOE_FWD, w [E, K, N]) or . W_e^T (MOE_DX, w [E, N, K])
 static void moe_rows_gemm(int mode, const bf16* a, const bf16* w, bf16* out, int N, int K, const MoeExtra& x,
                           const MoePlan& pl, const MoeSizes& z, cudaStream_t st) {
-  // 256-row pair tiles once the experts have 256 rows on average (below, half of a tile is padding)
+  // 256-row pair tiles once the experts have 256 rows on average (below, half of a tile is padding).  Pairs against
+  // 1-SM tiles, 16 experts 2048 x 2048, forward, 256 / 512 / 1024 / 2048 rows each: 118 / 178 / 289 / 533 us
+  // (129 / 174 / 302 / 562)
   const bool pair = N > 128 && z.P >= 256 * z.E;
   MoeGemmArgs g = moe_args(x, pl, z);
   g.tile = pair ? pl.tile2 : pl.tile;
@@ -1662,8 +1669,10 @@ static MoeSizes check_experts(const at::Tensor& x, const at::Tensor& w1, const s
 //   4 tokens                           19.0 / 27.7                                30.4 / 32.3
 //   8 tokens                           28.7 / 30.0                                49.6 / 36.3
 constexpr long kFewSlots = 8;
-// Up to this many rows an expert on average, the 64-row tiles.
-constexpr long kThinRows = 48;
+// Up to this many rows an expert on average, the 64-row tiles; past it experts need a second one.  Against the
+// 128-row tiles, in a CUDA graph with cold weights: 8 experts 1024 x 4096, 32 / 64 / 128 rows each on average,
+// 43 / 56 / 73 us (61 / 62 / 68); 32 experts 768 x 1536, 64 / 96 rows, 59 / 76 us (61 / 61).
+constexpr long kThinRows = 64;
 
 template <typename I, typename G>
 static void moe_few_launch(const bf16* x, const bf16* w1, const bf16* b1, const bf16* w2, const bf16* b2, const I* idx,

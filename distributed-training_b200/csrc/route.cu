@@ -157,10 +157,11 @@ __device__ __forceinline__ void store_logits(T* p, int valid, bool vec, const fl
 // heads of its lanes' lists by xor-shuffles, all groups at once, and each of the k rounds
 // takes the largest head of the warp (redux) and pops it.
 //
-// Bound by instruction issue: per token about 28 V for scores and keys, 5 V (V - 1) / 2 for the
-// sort, 5 a group and 25 a round.  The form that keeps the values unsorted and rescans V values a
-// round (route_fwd_wide_kernel) costs 7 V a round and 10 V a group: it serves V > 8, where
-// the sort would cost more.
+// Bound by the integer pipe (half rate: selects, compares, minima): per token about 28 V for
+// scores and keys, 5 V (V - 1) / 2 for the sort, 5 a group and 25 a round, 1050 instructions at
+// V = 8.  65536 tokens x 256 fp32 logits in 8 groups, 8 a token: 82 us (71 MB, 11 us at the copy
+// rate); unsorted values rescanned each round (route_fwd_wide_kernel, 7 V a round and 10 V a
+// group) took 194 us there.  That form serves V > 8, where the sort would cost more.
 template <typename T, int V>
 __global__ void __launch_bounds__(256) route_fwd_kernel(RouteArgs a) {
   extern __shared__ int s_load[];
@@ -382,8 +383,9 @@ struct RouteBwdArgs {
 //   ds_j = scale / D (G_j - [renorm, S > tiny] sum_i G_i s_i / D)
 //   sigmoid: dz_j = ds_j s_j (1 - s_j);  softmax: dz_i = s_i (ds_i - sum_j ds_j s_j)
 // The row is put together in shared memory (each lane owns V experts in a row) and
-// written with 16-byte stores.  Bound by memory: the sigmoid reads the chosen logits
-// only, the softmax the row; both write the row.
+// written with 16-byte stores.  The sigmoid reads the chosen logits only, the softmax the
+// row; both write the row.  Bound by the latency of the chain choice, logit, row: 65536 x 256
+// fp32, 8 a token, sigmoid, takes 23 us (71 MB, 3.1 TB/s).
 template <typename T, int V>
 __global__ void __launch_bounds__(256) route_bwd_kernel(RouteBwdArgs a) {
   extern __shared__ __align__(16) float s_row[];
