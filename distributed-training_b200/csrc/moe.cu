@@ -1274,6 +1274,7 @@ struct MoeThinArgs {
   long R;
 };
 
+// The plan is complete before this kernel can start (its predecessor has waited for it), so only the rows are waited for.
 __global__ void __launch_bounds__(MoeThinCfg::THREADS)
     moe_thin_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_constant__ CUtensorMap tmX, MoeThinArgs a) {
   using Cfg = MoeThinCfg;
@@ -1301,8 +1302,6 @@ __global__ void __launch_bounds__(MoeThinCfg::THREADS)
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem = *tmem_slot;
-  pdl_wait();
-  pdl_launch();
 
   const int nt = (a.N + 127) / 128;
   const int per = nt * a.splits;
@@ -1315,15 +1314,25 @@ __global__ void __launch_bounds__(MoeThinCfg::THREADS)
     const int kb0 = (int)((long)kbs * sp / a.splits), kb1 = (int)((long)kbs * (sp + 1) / a.splits);
     if (warp == 0) {
       if (lane == 0) {
-        int stage = 0;
-        uint32_t phase = 0;
-        for (int kb = kb0; kb < kb1; ++kb) {
-          if (!mbar_wait(&empty_bar[stage], phase ^ 1, abort_flag)) break;
+        const auto weights = [&](int stage, int kb) {
           uint8_t* sA = smem + stage * Cfg::STAGE_BYTES;
           mbar_arrive_expect_tx(&full_bar[stage], Cfg::STAGE_BYTES);
           tma_load_3d(&tmW, sA, &full_bar[stage], n0, kb * kBK, t.x);
           tma_load_3d(&tmW, sA + 8192, &full_bar[stage], n0 + 64, kb * kBK, t.x);
-          tma_load_2d(&tmX, sA + Cfg::A_BYTES, &full_bar[stage], kb * kBK, t.y);
+        };
+        // the first weights come while the rows are still being made
+        const int first = min(kb1 - kb0, Cfg::STAGES);
+        for (int i = 0; i < first; ++i) weights(i, kb0 + i);
+        pdl_wait();
+        pdl_launch();
+        int stage = 0;
+        uint32_t phase = 0;
+        for (int kb = kb0; kb < kb1; ++kb) {
+          if (kb - kb0 >= Cfg::STAGES) {
+            if (!mbar_wait(&empty_bar[stage], phase ^ 1, abort_flag)) break;
+            weights(stage, kb);
+          }
+          tma_load_2d(&tmX, smem + stage * Cfg::STAGE_BYTES + Cfg::A_BYTES, &full_bar[stage], kb * kBK, t.y);
           if (++stage == Cfg::STAGES) { stage = 0; phase ^= 1; }
         }
       }
