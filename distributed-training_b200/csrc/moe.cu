@@ -1251,19 +1251,21 @@ __global__ void __maxnreg__(DTB_CORESIDENT_MAXNREG)
 // Forward products for few rows an expert (generation with a batch): 64-row tiles with the
 // operands swapped, out^T = W_e^T . rows^T.  The weights' 128 columns are the M side of the
 // tile (MN-major), up to 64 rows the N side, so a k-block is 16 KB of weights and 8 KB of
-// rows instead of 32 KB and 16 KB for rows that are mostly padding; two CTAs an SM keep
-// 192 KB in flight.  A CTA makes one tile over one part of K: the first product all of it,
+// rows instead of 32 KB and 16 KB for rows that are mostly padding; two or three CTAs an SM
+// keep about 200 KB in flight.  A CTA makes one tile over one part of K: the first product all of it,
 // with the activation; the second leaves fp32 parts that moe_thin_combine joins.  Bound by
 // the weights' way from DRAM and five launches in a row: 48 tokens x 2 of 8 experts, 1024 x 4096
-// (134 MB of weights, 20.4 us at the copy rate), take 41 us in all, with the 128-row tiles 69.
+// (134 MB of weights, 20.4 us at the copy rate), take 39 us in all, with the 128-row tiles 69.
+// (Asking for all of a CTA's weights in L2 at its start made that 42.)
+template <int S>
 struct MoeThinCfg {
   static constexpr int A_BYTES = 128 * kBK * 2;
   static constexpr int B_BYTES = kRowPad * kBK * 2;
   static constexpr int STAGE_BYTES = A_BYTES + B_BYTES;
-  static constexpr int STAGES = 4;
+  static constexpr int STAGES = S;
   static constexpr int SMEM_BYTES = STAGES * STAGE_BYTES + 1024 /*align*/ + 128 /*barriers*/;
-  static constexpr int THREADS = 192;
 };
+constexpr int kThinThreads = 192;
 struct MoeThinArgs {
   const int4* tile;
   const int* off;
@@ -1275,9 +1277,10 @@ struct MoeThinArgs {
 };
 
 // The plan is complete before this kernel can start (its predecessor has waited for it), so only the rows are waited for.
-__global__ void __launch_bounds__(MoeThinCfg::THREADS)
+template <int S>
+__global__ void __launch_bounds__(kThinThreads)
     moe_thin_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_constant__ CUtensorMap tmX, MoeThinArgs a) {
-  using Cfg = MoeThinCfg;
+  using Cfg = MoeThinCfg<S>;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   uint64_t* full_bar = reinterpret_cast<uint64_t*>(smem + Cfg::STAGES * Cfg::STAGE_BYTES);
@@ -1737,30 +1740,41 @@ static void moe_few(const at::Tensor& x, const at::Tensor& w1, const bf16* b1, c
   else go(pl, bptr(gates));
 }
 
+template <int S>
+static void launch_thin_of(const CUtensorMap& tw, const CUtensorMap& tx, const MoeThinArgs& a, long grid, cudaStream_t st) {
+  static bool attr_set = false;
+  if (!attr_set) {
+    cudaFuncSetAttribute(moe_thin_kernel<S>, cudaFuncAttributeMaxDynamicSharedMemorySize, MoeThinCfg<S>::SMEM_BYTES);
+    attr_set = true;
+  }
+  launch_pdl(moe_thin_kernel<S>, dim3((unsigned)grid), kThinThreads, MoeThinCfg<S>::SMEM_BYTES, st, tw, tx, a);
+}
+// Four stages (two CTAs an SM), or three (three CTAs) where there are more CTAs than those hold.  In a CUDA graph with
+// cold weights, two a token of 8 experts 1024 x 4096, 48 / 128 / 256 tokens: 38.8 / 39.7 / 54.3 us with four,
+// 39.4 / 41.9 / 43.9 with three; four a token of 64 experts 768 x 1536, 64 tokens: 72.5 and 64.9.
+static void launch_thin(const CUtensorMap& tw, const CUtensorMap& tx, const MoeThinArgs& a, const MoeSizes& z, cudaStream_t st) {
+  const long each = (long)((a.N + 127) / 128) * a.splits, grid = z.R / kRowPad * each;
+  const long likely = (std::min(z.P, z.E) + z.P / kRowPad) * each;  // tiles: one an expert, and the rows past them
+  if (likely > 3L * num_sms()) launch_thin_of<3>(tw, tx, a, grid, st);
+  else launch_thin_of<4>(tw, tx, a, grid, st);
+}
+
 // Few rows an expert, without a gradient: the plan is built, `rows` holds xp [R, C] and act [R, H].
 static void moe_thin(const at::Tensor& x, const at::Tensor& w1, const bf16* b1, const at::Tensor& w2, const bf16* b2,
                      const at::Tensor& idx, const at::Tensor& gates, const at::Tensor& y, const MoePlan& pl,
                      const MoeSizes& z, cudaStream_t st) {
-  static bool attr_set = false;
-  if (!attr_set) {
-    cudaFuncSetAttribute(moe_thin_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, MoeThinCfg::SMEM_BYTES);
-    attr_set = true;
-  }
   const int C = (int)w1.size(1), H = (int)w1.size(2), Co = (int)w2.size(2), E = (int)z.E;
   // K is split until there are two CTAs an SM (as many tiles as experts that can have a row), 256 of K a part at least
   const long busy = std::min(z.P, z.E) * ((Co + 127) / 128);
   const int splits = (int)std::max<long>(1, std::min<long>({296 / busy, (H + 255) / 256, 16}));
-  const long tiles = z.R / kRowPad;
   auto rows = at::empty({z.R * (C + H)}, x.options());
   auto part = at::empty({splits * z.R * Co}, x.options().dtype(at::kFloat));
   bf16 *xp = bptr_mut(rows), *act = xp + z.R * C;
   launch_pdl(moe_gather_kernel, dim3(warp_grid(z.R)), 256, 0, st, bptr(x), xp, pl, E, C, (int)z.k);
   MoeThinArgs a{pl.tile3, pl.off, E, H, C, 1, b1, act, nullptr, z.R};
-  launch_pdl(moe_thin_kernel, dim3((unsigned)(tiles * ((H + 127) / 128))), MoeThinCfg::THREADS, MoeThinCfg::SMEM_BYTES, st,
-             make_map3(bptr(w1), z.E, C, H, 64, 64), make_map(xp, z.R, C, C, 64, kRowPad), a);
+  launch_thin(make_map3(bptr(w1), z.E, C, H, 64, 64), make_map(xp, z.R, C, C, 64, kRowPad), a, z, st);
   a = MoeThinArgs{pl.tile3, pl.off, E, Co, H, splits, nullptr, nullptr, part.data_ptr<float>(), z.R};
-  launch_pdl(moe_thin_kernel, dim3((unsigned)(tiles * ((Co + 127) / 128) * splits)), MoeThinCfg::THREADS,
-             MoeThinCfg::SMEM_BYTES, st, make_map3(bptr(w2), z.E, H, Co, 64, 64), make_map(act, z.R, H, H, 64, kRowPad), a);
+  launch_thin(make_map3(bptr(w2), z.E, H, Co, 64, 64), make_map(act, z.R, H, H, 64, kRowPad), a, z, st);
   const auto go = [&](auto* i, auto* g) {
     using I = std::remove_const_t<std::remove_pointer_t<decltype(i)>>;
     using G = std::remove_const_t<std::remove_pointer_t<decltype(g)>>;
