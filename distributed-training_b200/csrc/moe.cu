@@ -1677,13 +1677,13 @@ static MoeSizes check_experts(const at::Tensor& x, const at::Tensor& w1, const s
 
 // Up to this many slots go the streaming way: each slot reads its expert's weights, so it loses once many slots share
 // experts.  Streaming against the 64-row tiles, in a CUDA graph with cold weights, two slots a token:
-//   1 token  of 16 experts 768 x 2048: 10.3 / 20.6 us,  of 8 experts 1024 x 4096: 15.7 / 27.0 us
-//   4 tokens                           19.0 / 27.7                                30.4 / 32.3
-//   8 tokens                           28.7 / 30.0                                49.6 / 36.3
+//   1 token  of 16 experts 768 x 2048: 10.3 / 19.3 us,  of 8 experts 1024 x 4096: 15.5 / 26.7 us
+//   4 tokens                           18.7 / 26.0                                28.0 / 31.3
+//   8 tokens                           28.6 / 29.3                                49.4 / 34.8
 constexpr long kFewSlots = 8;
-// Up to this many rows an expert on average, the 64-row tiles; past it experts need a second one.  Against the
-// 128-row tiles, in a CUDA graph with cold weights: 8 experts 1024 x 4096, 32 / 64 / 128 rows each on average,
-// 43 / 56 / 73 us (61 / 62 / 68); 32 experts 768 x 1536, 64 / 96 rows, 59 / 76 us (61 / 61).
+// Up to this many rows an expert on average, the 64-row tiles; past it most experts need a second one.  Against the
+// 128-row tiles, in a CUDA graph with cold weights: 8 experts 1024 x 4096, 32 / 64 / 96 / 128 rows each on average,
+// 40 / 43 / 60 / 64 us (61 / 62 / 67 / 68); 32 experts 768 x 1536, 64 / 96 / 128 rows, 57 / 64 / 83 us (60 / 61 / 64).
 constexpr long kThinRows = 64;
 
 template <typename I, typename G>
