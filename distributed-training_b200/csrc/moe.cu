@@ -1383,6 +1383,7 @@ __global__ void __launch_bounds__(kThinThreads)
       }
     }
   }
+  if (threadIdx.x == 0) pdl_wait();  // CTAs without a tile too: none is done before the rows are
   tc_fence_before();
   __syncthreads();
   if (warp == 1) {

@@ -280,6 +280,19 @@ def test_expert_mlp_shapes_and_streams():
     assert _rel(F.expert_mlp(**q), experts64(**{m: v.double() if v.is_floating_point() else v for m, v in q.items()})) < 2 * U
 
 
+def test_expert_mlp_all_slots_empty():
+    for n in (2, 20, 600):
+        t, dy = _inputs(n, 64, 136, 72, 4, 2)
+        t["idx"].fill_(-1)
+        with torch.no_grad():
+            assert torch.all(F.expert_mlp(**t) == 0)
+        for m in ("x", "w1", "b1", "w2", "b2", "gates"):
+            t[m].requires_grad_()
+        y = F.expert_mlp(**t)
+        y.backward(dy)
+        assert torch.all(y == 0) and all(torch.all(t[m].grad == 0) for m in ("x", "w1", "b1", "w2", "b2", "gates"))
+
+
 def test_expert_mlp_inf_and_nan_stay_in_their_rows():
     t, _ = _inputs(40, 64, 64, 64, 4, 1)
     t["x"][7] = math.nan
