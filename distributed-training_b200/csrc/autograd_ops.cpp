@@ -51,12 +51,35 @@ struct RouteFn : public torch::autograd::Function<RouteFn> {
   }
 };
 
-std::vector<torch::Tensor> route_autograd(torch::Tensor logits, int64_t k, bool softmax,
-                                          c10::optional<torch::Tensor> bias, int64_t groups, int64_t keep, int64_t top,
-                                          bool renorm, double scale) {
-  if (!torch::GradMode::is_enabled() || !logits.requires_grad())
-    return route_fwd(logits, k, softmax, bias, groups, keep, top, renorm, scale);
-  return RouteFn::apply(logits, k, softmax, bias, groups, keep, top, renorm, scale);
+// route on logits of any leading shape and layout; nothing where the kernels do not take them (other types or
+// devices, more than 512 experts, 32 slots or 32 groups).
+c10::optional<std::tuple<torch::Tensor, torch::Tensor, torch::Tensor>> route_autograd(
+    torch::Tensor logits, int64_t k, const std::string& score, c10::optional<torch::Tensor> bias, int64_t groups,
+    int64_t keep, int64_t top, bool renorm, double scale) {
+  TORCH_CHECK_VALUE(score == "softmax" || score == "sigmoid", "route: score must be 'softmax' or 'sigmoid', got '", score,
+                    "'");
+  TORCH_CHECK_VALUE(logits.dim() >= 1, "route: logits (..., experts) expected");
+  const int64_t e = logits.size(-1);
+  TORCH_CHECK_VALUE(k >= 1 && k <= e, "route: k must be in [1, ", e, "], got ", k);
+  TORCH_CHECK_VALUE(groups >= 1 && e % groups == 0 && keep >= 1 && keep <= groups && keep * (e / groups) >= k, "route: ", e,
+                    " experts in ", groups, " groups, ", keep, " kept, do not give ", k, " experts a token");
+  TORCH_CHECK_VALUE(top == 1 || (top == 2 && e / groups >= 2), "route: group_top must be 1, or 2 with groups of at least 2, got ",
+                    top);
+  const bool biased = bias && bias->defined();
+  TORCH_CHECK_VALUE(!biased || (bias->dim() == 1 && bias->size(0) == e && bias->device() == logits.device()),
+                    "route: bias must be [", e, "] on the logits' device");
+  const auto t = logits.scalar_type();
+  if (!logits.is_cuda() || (t != at::kFloat && t != at::kBFloat16) || e > 512 || k > 32 || groups > 32) return c10::nullopt;
+  if (biased) bias = bias->detach().to(at::kFloat).contiguous();
+  const bool two = logits.dim() == 2;
+  auto shape = logits.sizes().vec();
+  shape.back() = k;
+  const auto z = (two ? logits : logits.reshape({-1, e})).contiguous();
+  const auto out = torch::GradMode::is_enabled() && z.requires_grad()
+                       ? RouteFn::apply(z, k, score == "softmax", bias, groups, keep, top, renorm, scale)
+                       : route_fwd(z, k, score == "softmax", bias, groups, keep, top, renorm, scale);
+  if (two) return std::make_tuple(out[0], out[1], out[2]);
+  return std::make_tuple(out[0].view(shape), out[1].view(shape), out[2]);
 }
 
 struct ExpertsFn : public torch::autograd::Function<ExpertsFn> {

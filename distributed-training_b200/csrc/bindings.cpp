@@ -61,9 +61,9 @@ std::vector<torch::Tensor> experts_bwd(torch::Tensor dy, torch::Tensor x, torch:
                                        c10::optional<torch::Tensor> db1, torch::Tensor dw2,
                                        c10::optional<torch::Tensor> db2);
 // autograd_ops.cpp
-std::vector<torch::Tensor> route_autograd(torch::Tensor logits, int64_t k, bool softmax,
-                                          c10::optional<torch::Tensor> bias, int64_t groups, int64_t keep, int64_t top,
-                                          bool renorm, double scale);
+c10::optional<std::tuple<torch::Tensor, torch::Tensor, torch::Tensor>> route_autograd(
+    torch::Tensor logits, int64_t k, const std::string& score, c10::optional<torch::Tensor> bias, int64_t groups,
+    int64_t keep, int64_t top, bool renorm, double scale);
 c10::optional<torch::Tensor> experts_autograd(torch::Tensor x, torch::Tensor w1, c10::optional<torch::Tensor> b1,
                                               torch::Tensor w2, c10::optional<torch::Tensor> b2, torch::Tensor idx,
                                               torch::Tensor gates);

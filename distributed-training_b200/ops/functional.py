@@ -205,6 +205,10 @@ def route(logits, k: int, *, score: str = "softmax", bias=None, groups: int = 1,
     idx (..., k) is int32, load int32 [experts] counts the slots of each expert.  The
     gates are differentiable in the logits.
     """
+    if logits.is_cuda:
+        out = K.route(logits, k, score, bias, groups, keep_groups, group_top, renorm, scale)
+        if out is not None:
+            return out
     if score not in ("softmax", "sigmoid"):
         raise ValueError(f"route: score must be 'softmax' or 'sigmoid', got {score!r}")
     e = logits.shape[-1]
@@ -216,18 +220,9 @@ def route(logits, k: int, *, score: str = "softmax", bias=None, groups: int = 1,
         raise ValueError(f"route: group_top must be 1, or 2 with groups of at least 2, got {group_top}")
     if bias is not None and (bias.shape != (e,) or bias.device != logits.device):
         raise ValueError(f"route: bias must be [{e}] on the logits' device")
-    softmax = score == "softmax"
-    z = logits.reshape(-1, e)
-    if z.is_cuda and z.dtype in (torch.float32, torch.bfloat16) and e <= 512 and k <= 32 and groups <= 32:
-        z = z.contiguous()
-        b = bias if bias is None else bias.detach().float().contiguous()
-        out = K.route(z, k, softmax, b, groups, keep_groups, group_top, renorm, scale)
-    else:
-        out = _route_math(z, k, softmax, bias, groups, keep_groups, group_top, renorm, scale)
-    gates, idx, load = out
-    if logits.dim() != 2:
-        gates, idx = gates.view(*logits.shape[:-1], k), idx.view(*logits.shape[:-1], k)
-    return gates, idx, load
+    gates, idx, load = _route_math(logits.reshape(-1, e), k, score == "softmax", bias, groups, keep_groups, group_top,
+                                   renorm, scale)
+    return gates.view(*logits.shape[:-1], k), idx.view(*logits.shape[:-1], k), load
 
 
 def _experts_math(x, w1, b1, w2, b2, idx, gates):

@@ -144,9 +144,10 @@ def route_bwd(logits, gates, idx, dgates, *, softmax: bool = True, renorm: bool 
     return lib().route_bwd(logits, gates, idx, dgates, softmax, renorm, scale)
 
 
-def route(logits, k, softmax, bias, groups, keep, top, renorm, scale):
-    """``route_fwd`` with autograd (csrc/autograd_ops.cpp): the gates are differentiable in the logits."""
-    return lib().route(logits, k, softmax, bias, groups, keep, top, renorm, scale)
+def route(logits, k, score, bias, groups, keep, top, renorm, scale):
+    """(gates, idx, load) with autograd (csrc/autograd_ops.cpp), any leading shape and layout: the gates are
+    differentiable in the logits.  None where the kernels do not take the logits."""
+    return lib().route(logits, k, score, bias, groups, keep, top, renorm, scale)
 
 
 def experts(x, w1, b1, w2, b2, idx, gates) -> torch.Tensor | None:

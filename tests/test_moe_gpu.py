@@ -132,6 +132,10 @@ def test_route_refusals_gpu():
     z = torch.randn(4, 8, device="cuda")
     with pytest.raises(ValueError, match="bias"):
         F.route(z, 2, bias=torch.zeros(8))
+    for bad in (dict(k=0), dict(k=9), dict(k=3, score="tanh"), dict(k=3, groups=3), dict(k=3, groups=4, keep_groups=5),
+                dict(k=3, groups=4, keep_groups=1), dict(k=3, group_top=3), dict(k=3, bias=torch.zeros(7).cuda())):
+        with pytest.raises(ValueError, match="route"):
+            F.route(z, **bad)
     with pytest.raises(RuntimeError, match="route"):
         K.route_fwd(z, 9)
     with pytest.raises(RuntimeError, match="route"):
