@@ -1,8 +1,9 @@
 // Autograd of the router and the experts' products as C++ functions.
 //
-// The kernels of a small call take a few microseconds; a Python autograd.Function adds
-// about 90 to a forward and backward pass (its Python frames, the zero gradients it makes
-// for integer outputs), a C++ one about a third of that.
+// The kernels of a small call take a few microseconds.  A forward and backward pass of the
+// router (16384 x 16) took 131 us through a Python autograd.Function (its frames, the zero
+// gradients it makes for integer outputs) and takes 62 through this one, of which the
+// engine's own share is about 40.
 #include <torch/extension.h>
 
 namespace dtb {

@@ -1581,23 +1581,41 @@ static MoeGemmArgs moe_args(const MoeExtra& x, const MoePlan& pl, const MoeSizes
   return g;
 }
 
-// Columns of an output tile: 128 where there are no more, else 256.
-static int moe_tile_n(int N) { return N <= 128 ? 128 : 256; }
+struct MoeTiling {
+  bool pair;  // 256 x 256 by a CTA pair
+  int bn;     // else 128 x bn
+};
+// 256-row pair tiles once the experts have 256 rows on average (below, half of a tile is padding).  Pairs against
+// 1-SM tiles, 16 experts 2048 x 2048, forward, 256 / 512 / 1024 / 2048 rows each: 118 / 178 / 289 / 533 us
+// (129 / 174 / 302 / 562).  Where 256-wide tiles do not fill the SMs, 128 x 128: forward and
+// backward in a CUDA graph, 4 experts 768 x 1536, 600 tokens, two a token, 82 us (256-wide 93); 8 experts 512 x 1024,
+// 2048 tokens, 107 (111).
+static MoeTiling moe_rows_tiling(int N, const MoeSizes& z) {
+  if (N <= 128 || (z.P / 256 + std::min(z.P, z.E)) * ((N + 255) / 256) < num_sms() / 2) return {false, 128};
+  return {z.P >= 256 * z.E, 256};
+}
+static MoeTiling moe_weight_tiling(int M, int N, const MoeSizes& z) {
+  if (N <= 128 || z.E * ((M + 255) / 256) * ((N + 255) / 256) < num_sms() / 2) return {false, 128};
+  return {M > 128, 256};
+}
+// Parts of each row's product that the dpre GEMM leaves.
+static int moe_dot_parts(int N, const MoeSizes& z) {
+  const int bn = moe_rows_tiling(N, z).bn;
+  return (N + bn - 1) / bn * 2;
+}
 
 // rows [R, N] = rows [R, K] . W_e (MOE_FWD, w [E, K, N]) or . W_e^T (MOE_DX, w [E, N, K])
 static void moe_rows_gemm(int mode, const bf16* a, const bf16* w, bf16* out, int N, int K, const MoeExtra& x,
                           const MoePlan& pl, const MoeSizes& z, cudaStream_t st) {
-  // 256-row pair tiles once the experts have 256 rows on average (below, half of a tile is padding).  Pairs against
-  // 1-SM tiles, 16 experts 2048 x 2048, forward, 256 / 512 / 1024 / 2048 rows each: 118 / 178 / 289 / 533 us
-  // (129 / 174 / 302 / 562)
-  const bool pair = N > 128 && z.P >= 256 * z.E;
+  const MoeTiling t = moe_rows_tiling(N, z);
+  const bool pair = t.pair;
   MoeGemmArgs g = moe_args(x, pl, z);
   g.tile = pair ? pl.tile2 : pl.tile;
   g.ntile = pl.ntile + (pair ? 1 : 0);
   g.N = N;
   g.K = K;
   g.M = 1;
-  const int bn = moe_tile_n(N);
+  const int bn = t.bn;
   const CUtensorMap ta = make_map(a, z.R, K, K, 64, kBM);
   const CUtensorMap tb = mode == MOE_FWD ? make_map3(w, z.E, K, N, 64, 64) : make_map3(w, z.E, N, K, 64, pair ? 128 : bn);
   const CUtensorMap to = make_store_map(out, false, z.R, N, N);
@@ -1624,11 +1642,12 @@ static void moe_weight_gemm(const bf16* a, const bf16* b, const at::Tensor& out,
   MoeGemmArgs g = moe_args(x, pl, z);
   g.M = M;
   g.N = N;
-  const int bn = moe_tile_n(N);
+  const MoeTiling t = moe_weight_tiling(M, N, z);
+  const int bn = t.bn;
   const CUtensorMap ta = make_map(a, z.R, M, M, 64, 64);
   const CUtensorMap tb = make_map(b, z.R, N, N, 64, 64);
   const CUtensorMap to = make_store_map(out.data_ptr(), f32, M, N, N, z.E);
-  if (M > 128 && N > 128) {
+  if (t.pair) {
     launch_moe2<MOE_DW>(ta, tb, to, to, g, z.E * ((M + 255) / 256) * ((N + 255) / 256), st);
     return;
   }
@@ -1912,7 +1931,7 @@ std::vector<at::Tensor> experts_bwd(at::Tensor dy, at::Tensor x, at::Tensor w1, 
   const bf16 *xp = bptr(rows), *act = xp + z.R * C;
   bf16* pre = bptr_mut(rows) + z.R * (C + H);
   // scratch: dpre, dy's rows (later dx's); fp32: the rows' products, the column sums of blocks of rows
-  const int parts = 2 * (int)((H + moe_tile_n((int)H) - 1) / moe_tile_n((int)H));
+  const int parts = moe_dot_parts((int)H, z);
   const int bparts = has2 ? (int)((Co + 255) / 256) : 0;
   const long sums = has1 ? z.R / 32 * H : 0, sums2 = has2 ? z.R / kRowPad * Co : 0;
   const long wide = std::max(C, Co);
