@@ -11,8 +11,8 @@ namespace dtb {
 // route.cu
 std::vector<torch::Tensor> route_fwd(torch::Tensor logits, int64_t k, bool softmax, c10::optional<torch::Tensor> bias,
                                      int64_t groups, int64_t keep, int64_t top, bool renorm, double scale);
-torch::Tensor route_bwd(torch::Tensor logits, torch::Tensor gates, torch::Tensor idx, torch::Tensor dgates,
-                        bool softmax, bool renorm, double scale);
+torch::Tensor route_bwd(torch::Tensor logits, torch::Tensor idx, torch::Tensor dgates, bool softmax, bool renorm,
+                        double scale);
 // moe.cu
 std::vector<torch::Tensor> experts_fwd(torch::Tensor x, torch::Tensor w1, c10::optional<torch::Tensor> b1,
                                        torch::Tensor w2, c10::optional<torch::Tensor> b2, torch::Tensor idx,
@@ -33,7 +33,7 @@ struct RouteFn : public torch::autograd::Function<RouteFn> {
                                bool renorm, double scale) {
     at::AutoDispatchBelowADInplaceOrView guard;
     auto out = route_fwd(logits, k, softmax, bias, groups, keep, top, renorm, scale);
-    ctx->save_for_backward({logits, out[0], out[1]});
+    ctx->save_for_backward({logits, out[1]});
     ctx->saved_data["softmax"] = softmax;
     ctx->saved_data["renorm"] = renorm;
     ctx->saved_data["scale"] = scale;
@@ -46,7 +46,7 @@ struct RouteFn : public torch::autograd::Function<RouteFn> {
     if (!grads[0].defined()) return out;
     const auto saved = ctx->get_saved_variables();
     at::AutoDispatchBelowADInplaceOrView guard;
-    out[0] = route_bwd(saved[0], saved[1], saved[2], grads[0].contiguous(), ctx->saved_data["softmax"].toBool(),
+    out[0] = route_bwd(saved[0], saved[1], grads[0].contiguous(), ctx->saved_data["softmax"].toBool(),
                        ctx->saved_data["renorm"].toBool(), ctx->saved_data["scale"].toDouble());
     return out;
   }

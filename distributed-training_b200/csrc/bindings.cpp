@@ -49,8 +49,8 @@ torch::Tensor attn_bwd(torch::Tensor qkv, torch::Tensor out, torch::Tensor dout,
 // route.cu
 std::vector<torch::Tensor> route_fwd(torch::Tensor logits, int64_t k, bool softmax, c10::optional<torch::Tensor> bias,
                                      int64_t groups, int64_t keep, int64_t top, bool renorm, double scale);
-torch::Tensor route_bwd(torch::Tensor logits, torch::Tensor gates, torch::Tensor idx, torch::Tensor dgates,
-                        bool softmax, bool renorm, double scale);
+torch::Tensor route_bwd(torch::Tensor logits, torch::Tensor idx, torch::Tensor dgates, bool softmax, bool renorm,
+                        double scale);
 // moe.cu
 std::vector<torch::Tensor> experts_fwd(torch::Tensor x, torch::Tensor w1, c10::optional<torch::Tensor> b1,
                                        torch::Tensor w2, c10::optional<torch::Tensor> b2, torch::Tensor idx,

@@ -50,7 +50,6 @@ struct MoePlan {
   int4* tile3;  // and of 64, with the end of the expert's rows that are not padding; their number is off[E] / 64
   int* ntile;   // [2] the numbers of the first two, padded to 4
   int* off;    // [E + 1] first row of each expert, a multiple of 64
-  int* count;  // [E] rows of each expert, without the padding
   int* order;  // [E] the experts by falling number of rows
   int* inv;    // [P] row of a slot, -1: none
   int* src;    // [R] slot of a row, -1: padding
@@ -64,7 +63,7 @@ constexpr int kPlanThreads = 256;
 constexpr int kPlanChunk = 1024;  // slots a block sorts: 8 warps x 128
 static long plan_blocks(long P) { return std::max<long>(1, (P + kPlanChunk - 1) / kPlanChunk); }
 static long plan_ints(long P, long E) {
-  return 8 * moe_max_tiles(P, E) + moe_max_rows(P, E) / kRowPad * 4 + 4 + (E + 1) + 2 * E + P + moe_max_rows(P, E) + plan_blocks(P) * E;
+  return 8 * moe_max_tiles(P, E) + moe_max_rows(P, E) / kRowPad * 4 + 4 + (E + 1) + E + P + moe_max_rows(P, E) + plan_blocks(P) * E;
 }
 static MoePlan plan_views(int* p, long P, long E) {
   MoePlan v;
@@ -74,8 +73,7 @@ static MoePlan plan_views(int* p, long P, long E) {
   v.ntile = reinterpret_cast<int*>(v.tile3 + moe_max_rows(P, E) / kRowPad);
   v.src = v.ntile + 4;
   v.off = v.src + moe_max_rows(P, E);
-  v.count = v.off + E + 1;
-  v.order = v.count + E;
+  v.order = v.off + E + 1;
   v.inv = v.order + E;
   v.hist = v.inv + P;
   return v;
@@ -131,7 +129,6 @@ __device__ __forceinline__ int plan_expert(const MoePlan& pl, int e, int E, int 
     int place = 0;
     for (int o = 0; o < E; ++o) place += s_total[o] > total || (s_total[o] == total && o < e);
     pl.order[place] = e;
-    pl.count[e] = total;
     pl.off[e + 1] = end;
     if (e == 0) pl.off[0] = 0;
     for (int t = 0; t < t1; ++t) pl.tile[n1 - t1 + t] = make_int4(e, start + t * kBM, end, 0);

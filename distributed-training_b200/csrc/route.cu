@@ -369,7 +369,6 @@ __global__ void __launch_bounds__(256) route_fwd_wide_kernel(RouteArgs a) {
 
 struct RouteBwdArgs {
   const void* logits;
-  const float* gates;
   const int* idx;
   const float* dgates;
   void* dlogits;
@@ -529,24 +528,21 @@ std::vector<at::Tensor> route_fwd(at::Tensor logits, int64_t k, bool softmax, st
 }
 
 // d(logits) in the logits' type from the gates' gradient (fp32 [n, k]).
-at::Tensor route_bwd(at::Tensor logits, at::Tensor gates, at::Tensor idx, at::Tensor dgates,
-                        bool softmax, bool renorm, double scale) {
+at::Tensor route_bwd(at::Tensor logits, at::Tensor idx, at::Tensor dgates, bool softmax, bool renorm, double scale) {
   TORCH_CHECK(logits.is_cuda() && logits.dim() == 2 && logits.is_contiguous(), "route_bwd: contiguous CUDA logits");
   const bool f32 = logits.scalar_type() == at::kFloat;
   TORCH_CHECK(f32 || logits.scalar_type() == at::kBFloat16, "route_bwd: fp32 or bf16 logits");
   const long n = logits.size(0), e = logits.size(1);
-  TORCH_CHECK(gates.dim() == 2 && gates.size(0) == n && gates.is_contiguous() && gates.scalar_type() == at::kFloat,
-              "route_bwd: gates");
-  const long k = gates.size(1);
+  TORCH_CHECK(idx.dim() == 2 && idx.size(0) == n && idx.scalar_type() == at::kInt && idx.is_contiguous(), "route_bwd: idx");
+  const long k = idx.size(1);
   TORCH_CHECK(e <= kRouteMaxExperts && k >= 1 && k <= kRouteMaxK && k <= e, "route_bwd: sizes");
-  TORCH_CHECK(idx.sizes() == gates.sizes() && idx.scalar_type() == at::kInt && idx.is_contiguous(), "route_bwd: idx");
-  TORCH_CHECK(dgates.sizes() == gates.sizes() && dgates.scalar_type() == at::kFloat && dgates.is_contiguous(),
+  TORCH_CHECK(dgates.sizes() == idx.sizes() && dgates.scalar_type() == at::kFloat && dgates.is_contiguous() &&
+                  dgates.device() == logits.device() && idx.device() == logits.device(),
               "route_bwd: dgates");
   c10::cuda::CUDAGuard guard(logits.device());
   auto dl = at::empty_like(logits);
   if (n == 0) return dl;
-  RouteBwdArgs a{logits.data_ptr(), gates.data_ptr<float>(), idx.data_ptr<int>(), dgates.data_ptr<float>(),
-                 dl.data_ptr(), (int)n, (int)e, (int)k, softmax, renorm, 0, (float)scale};
+  RouteBwdArgs a{logits.data_ptr(), idx.data_ptr<int>(), dgates.data_ptr<float>(), dl.data_ptr(), (int)n, (int)e, (int)k, softmax, renorm, 0, (float)scale};
   const int V = e <= 32 ? 1 : e <= 64 ? 2 : e <= 128 ? 4 : e <= 256 ? 8 : 16;
   const int es = f32 ? 4 : 2;
   a.vec = (V * es) % 16 == 0 && (e * es) % 16 == 0 &&

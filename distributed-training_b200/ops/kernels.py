@@ -138,10 +138,10 @@ def route_fwd(logits: torch.Tensor, k: int, *, softmax: bool = True, bias: torch
     return lib().route_fwd(logits, k, softmax, bias, groups, keep, top, renorm, scale)
 
 
-def route_bwd(logits, gates, idx, dgates, *, softmax: bool = True, renorm: bool = True,
+def route_bwd(logits, idx, dgates, *, softmax: bool = True, renorm: bool = True,
               scale: float = 1.0) -> torch.Tensor:
     """d(logits), in the logits' type, from the gates' gradient (fp32 [n, k])."""
-    return lib().route_bwd(logits, gates, idx, dgates, softmax, renorm, scale)
+    return lib().route_bwd(logits, idx, dgates, softmax, renorm, scale)
 
 
 def route(logits, k, score, bias, groups, keep, top, renorm, scale):
