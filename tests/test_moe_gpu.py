@@ -188,6 +188,8 @@ EXPERTS = [  # n, c, h, co, e, k, bias, skew
     (257, 320, 640, 320, 3, 3, True, 0.0),
     (700, 136, 264, 520, 40, 6, False, 0.1),
     (2000, 512, 384, 512, 4, 2, True, 0.3),
+    (200, 64, 72, 64, 512, 32, True, 0.0),      # the most experts and slots
+    (5000, 64, 136, 64, 3, 1, True, 0.0),       # the plan of many slots, several row tiles an expert
 ]
 
 
