@@ -424,16 +424,19 @@ struct ClipRange {
   bool out;
 };
 
-// Outputs must not overlap one another, nor another tensor's input.
+// Outputs must not overlap one another, nor any input; a tensor scaled in place has one range.
 static void check_ranges(std::vector<ClipRange>& r) {
   const auto less = [](const ClipRange& a, const ClipRange& b) { return a.lo < b.lo; };
   if (!std::is_sorted(r.begin(), r.end(), less)) std::sort(r.begin(), r.end(), less);
+  const auto apart = [](bool ok, int i, int j) {
+    TORCH_CHECK(ok || i == j, "clip_grads: tensors ", i, " and ", j, " overlap in memory");
+    TORCH_CHECK(ok, "clip_grads: output ", i, " overlaps its gradient in memory without being it");
+  };
   uintptr_t out_hi = 0, any_hi = 0;
   int out_i = -1, any_i = -1;
   for (const auto& x : r) {
-    TORCH_CHECK(!(x.lo < out_hi && out_i != x.i), "clip_grads: tensors ", out_i, " and ", x.i, " overlap in memory");
-    TORCH_CHECK(!(x.out && x.lo < any_hi && any_i != x.i), "clip_grads: tensors ", any_i, " and ", x.i,
-                " overlap in memory");
+    apart(x.lo >= out_hi, out_i, x.i);
+    apart(!x.out || x.lo >= any_hi, any_i, x.i);
     if (x.out && x.hi > out_hi) { out_hi = x.hi; out_i = x.i; }
     if (x.hi > any_hi) { any_hi = x.hi; any_i = x.i; }
   }

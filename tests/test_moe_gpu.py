@@ -476,6 +476,25 @@ def test_clip_refusals_gpu():
     assert float(global_norm([None, torch.full((4,), 2.0, device="cuda"), None])) == 4.0
 
 
+def test_clip_refuses_outputs_that_overlap_their_own_gradients():
+    # each output overlaps the gradient that it is made from, at another address or in another type
+    buf = torch.randn(20001, device="cuda")
+    keep = buf.clone()
+    narrow = buf.view(torch.bfloat16)
+    for g, o in ((buf[:20000], buf[1:20001]), (buf[4:10004], buf[:10000]), (narrow[20000:30000], buf[5000:15000]),
+                 (buf[:5000], narrow[9998:14998])):
+        with pytest.raises(RuntimeError, match="overlap"):
+            clip_grads([torch.ones(3, device="cuda"), g], 1e-3, out=[torch.empty(3, device="cuda"), o])
+    assert torch.equal(buf, keep)
+    # side by side they are fine, and so is a gradient in its own place
+    a, b = buf[:10000], buf[10000:20000]
+    want = a.double()
+    clip_grads([a], 1e9, out=[b])
+    assert torch.equal(b.double(), want)
+    clip_grads([a], 1e9, out=[a.view(100, 100).view(-1)])
+    assert torch.equal(a.double(), want)
+
+
 # ----------------------------------------------------------------------- together
 def test_example_learns_and_layer_matches_fp32():
     import numpy as np
