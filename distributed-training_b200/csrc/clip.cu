@@ -20,7 +20,6 @@
 // fp32: 113 and 261 us.  A few small tensors: two launches, 7.5 us on the GPU.
 #include <ATen/core/Tensor.h>
 #include <ATen/ops/empty.h>
-#include <ATen/MemoryOverlap.h>
 #include <ATen/cuda/CUDAContext.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <cuda_fp16.h>
@@ -29,6 +28,7 @@
 #include <type_traits>
 
 #include "common.cuh"
+#include "overlap.h"
 
 namespace dtb {
 
@@ -418,27 +418,46 @@ static ClipStrided strided_desc(const at::Tensor& a, const at::Tensor* b) {
   return d;
 }
 
+// Bytes that a tensor spans; `t`: the tensor where it leaves gaps between its elements, else null.
 struct ClipRange {
   uintptr_t lo, hi;
   int i;
   bool out;
+  const at::Tensor* t;
 };
 
-// Outputs must not overlap one another, nor any input; a tensor scaled in place has one range.
+static MemView mem_view(const at::Tensor& t) {
+  MemView v{reinterpret_cast<uintptr_t>(t.const_data_ptr()), (int)t.element_size(), t.sizes().vec(), t.strides().vec()};
+  for (long& s : v.stride) s *= v.elem;
+  return v;
+}
+static MemView mem_view(const ClipRange& r) {
+  return r.t ? mem_view(*r.t) : MemView{r.lo, 1, {(long)(r.hi - r.lo)}, {1}};
+}
+
+static ClipRange clip_range(const at::Tensor& t, bool dense, int i, bool out) {
+  const uintptr_t lo = reinterpret_cast<uintptr_t>(t.const_data_ptr());
+  if (dense) return {lo, lo + t.numel() * t.element_size(), i, out, nullptr};
+  long last = 0;
+  for (int64_t k = 0; k < t.dim(); ++k) last += (t.size(k) - 1) * t.stride(k);
+  return {lo, lo + (last + 1) * t.element_size(), i, out, &t};
+}
+
+// Outputs must not overlap one another, nor any input; a tensor scaled in place has one range.  Ranges
+// that meet are looked at closer where one of them has gaps: interleaved views share no element.
 static void check_ranges(std::vector<ClipRange>& r) {
   const auto less = [](const ClipRange& a, const ClipRange& b) { return a.lo < b.lo; };
   if (!std::is_sorted(r.begin(), r.end(), less)) std::sort(r.begin(), r.end(), less);
-  const auto apart = [](bool ok, int i, int j) {
-    TORCH_CHECK(ok || i == j, "clip_grads: tensors ", i, " and ", j, " overlap in memory");
-    TORCH_CHECK(ok, "clip_grads: output ", i, " overlaps its gradient in memory without being it");
-  };
-  uintptr_t out_hi = 0, any_hi = 0;
-  int out_i = -1, any_i = -1;
+  std::vector<const ClipRange*> open;  // those that reach past the start of the present one
   for (const auto& x : r) {
-    apart(x.lo >= out_hi, out_i, x.i);
-    apart(!x.out || x.lo >= any_hi, any_i, x.i);
-    if (x.out && x.hi > out_hi) { out_hi = x.hi; out_i = x.i; }
-    if (x.hi > any_hi) { any_hi = x.hi; any_i = x.i; }
+    open.erase(std::remove_if(open.begin(), open.end(), [&](const ClipRange* y) { return y->hi <= x.lo; }), open.end());
+    for (const ClipRange* y : open) {
+      if (!x.out && !y->out) continue;
+      const bool apart = (x.t || y->t) && !views_overlap(mem_view(x), mem_view(*y));
+      TORCH_CHECK(apart || x.i == y->i, "clip_grads: tensors ", y->i, " and ", x.i, " overlap in memory");
+      TORCH_CHECK(apart, "clip_grads: output ", x.i, " overlaps its gradient in memory without being it");
+    }
+    open.push_back(&x);
   }
 }
 
@@ -501,22 +520,9 @@ at::Tensor clip_grads(std::vector<std::optional<at::Tensor>> in,
     const bool dense_b = b && (b == &a ? dense_a : b->is_non_overlapping_and_dense());
     const bool flat = dense_a && (!b || same || (dense_b && same_order(a, *b)));
     if (b) {
-      TORCH_CHECK(dense_b || at::has_internal_overlap(*b) != at::MemOverlap::Yes, "clip_grads: output ", i,
-                  " overlaps itself");
-      if (flat) {
-        const uintptr_t lo = reinterpret_cast<uintptr_t>(pa), lb = reinterpret_cast<uintptr_t>(pb);
-        if (!same) ranges.push_back({lo, lo + numel * a.element_size(), (int)i, false});
-        ranges.push_back({lb, lb + numel * b->element_size(), (int)i, true});
-      } else if (dense_b) {
-        const auto range = [&](const at::Tensor& t, bool o) {
-          long last = 0;
-          for (int64_t k = 0; k < t.dim(); ++k) last += (t.size(k) - 1) * t.stride(k);
-          const uintptr_t lo = reinterpret_cast<uintptr_t>(t.const_data_ptr());
-          ranges.push_back({lo, lo + (last + 1) * t.element_size(), (int)i, o});
-        };
-        if (!same) range(a, false);
-        range(*b, true);
-      }
+      TORCH_CHECK(dense_b || !view_overlaps_itself(mem_view(*b)), "clip_grads: output ", i, " overlaps itself");
+      if (!same) ranges.push_back(clip_range(a, dense_a, (int)i, false));
+      ranges.push_back(clip_range(*b, dense_b, (int)i, true));
     }
     if (flat) dense.push_back({pa, pb, numel, 0, ta, tb});
     else strided.push_back(strided_desc(a, b));

@@ -495,6 +495,64 @@ def test_clip_refuses_outputs_that_overlap_their_own_gradients():
     assert torch.equal(a.double(), want)
 
 
+def _cells(shape, stride, at):
+    cells = torch.tensor([at])
+    for n, s in zip(shape, stride):
+        cells = (cells[:, None] + s * torch.arange(n)).flatten()
+    return cells.tolist()
+
+
+def test_clip_refuses_overlapping_strided_outputs():
+    a = torch.randn(60, 66, device="cuda")
+    keep = a.clone()
+    v = a[:, ::2]
+    other = torch.randn(60, 33, device="cuda")
+    for grads, out in (([v, v], None), ([v, a[:, 30:50]], None), ([a[:, 1::3], v], None), ([a[5:9], v], None),
+                       ([other, other + 1], [v, v]), ([other, a[3]], [v, a[3]]),
+                       ([v, other], [torch.empty_like(v), v]), ([v[1:]], [v[:-1]]),
+                       ([a.as_strided((40, 50), (40, 1))], None), ([a.t(), v], None)):
+        with pytest.raises(RuntimeError, match="overlap"):
+            clip_grads(grads, 1e-3, out=out)
+    assert torch.equal(a, keep)
+    # interleaved views, and the columns of one tensor, share nothing
+    want = math.sqrt(float((a.double() ** 2).sum()))
+    for parts in ([v, a[:, 1::2]], [a[:, 1::2], v], [a[:, :7], a[:, 7:20], a[:, 20:]], [a[::3], a[1::3], a[2::3]],
+                  [a.t()[::2], a.t()[1::2]], [a[:30, ::2], a[30:, ::2], a[:, 1::2]]):
+        a.copy_(keep)
+        assert float(clip_grads(parts, want / 2)) == pytest.approx(want, rel=1e-6)
+        torch.testing.assert_close(a, keep / 2, rtol=1e-6, atol=0)
+    # gradients read from between the outputs' elements
+    a.copy_(keep)
+    clip_grads([a[:, 1::2]], 1e9, out=[v])
+    assert torch.equal(v, keep[:, 1::2]) and torch.equal(a[:, 1::2], keep[:, 1::2])
+    # gradients may overlap one another: each counts in the norm
+    assert float(clip_grads([v, v], 1e9, out=[other, torch.empty_like(other)])) == pytest.approx(
+        math.sqrt(2.0) * float(v.double().norm()), rel=1e-6)
+
+
+def test_clip_overlap_of_any_views():
+    g = torch.Generator().manual_seed(11)
+    pick = lambda lo, hi: int(torch.randint(lo, hi + 1, (1,), generator=g))  # noqa: E731
+    buf = torch.ones(4096, device="cuda")
+    refused = 0
+    for _ in range(600):
+        views = []
+        for _ in range(2):
+            nd = pick(1, 3)
+            views.append(([pick(1, 4) for _ in range(nd)], [pick(1, 14) for _ in range(nd)], pick(0, 20)))
+        cells = sum((_cells(*v) for v in views), [])
+        ts = [buf.as_strided(*v) for v in views]
+        if len(set(cells)) < len(cells):
+            refused += 1
+            with pytest.raises(RuntimeError, match="overlap"):
+                clip_grads(ts, 1.0)
+        else:
+            buf.fill_(1.0)
+            clip_grads(ts, math.sqrt(len(cells)) / 2)
+            assert int((buf < 0.75).sum()) == len(cells) and torch.all(buf[cells] < 0.75)
+    assert 100 < refused < 500
+
+
 # ----------------------------------------------------------------------- together
 def test_example_learns_and_layer_matches_fp32():
     import numpy as np
