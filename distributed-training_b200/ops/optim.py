@@ -43,6 +43,41 @@ def _floating(name, grads):
     return ts
 
 
+def _bytes(t, lo: int, hi: int) -> torch.Tensor:
+    """Which of the addresses [lo, hi) belong to ``t``."""
+    hit = torch.zeros(hi - lo, dtype=torch.bool)
+    n = t.element_size()
+    hit.as_strided((*t.shape, n), (*(s * n for s in t.stride()), 1), t.data_ptr() - lo).fill_(True)
+    return hit
+
+
+def _check_apart(grads, outs) -> None:
+    """Outputs share no memory with one another nor with a gradient, their own in place apart (as csrc/clip.cu)."""
+    ranges = []
+    for i, (g, o) in enumerate(zip(grads, outs)):
+        if g.numel() == 0 or g.layout != torch.strided or o.layout != torch.strided:
+            continue
+        place = lambda t: (t.data_ptr(), t.dtype, [s for n, s in zip(t.shape, t.stride()) if n > 1])  # noqa: E731
+        for t, out in ((g, False), (o, True)) if place(g) != place(o) else ((o, True),):
+            lo = t.data_ptr()
+            hi = lo + (sum((n - 1) * s for n, s in zip(t.shape, t.stride())) + 1) * t.element_size()
+            if out and hi - lo < t.numel() * t.element_size() or (
+                    out and not t.is_contiguous() and int(_bytes(t, lo, hi).sum()) < t.numel() * t.element_size()):
+                raise RuntimeError(f"clip_grads: output {i} overlaps itself")
+            ranges.append((lo, hi, i, out, t))
+    ranges.sort(key=lambda r: r[0])
+    near = []                                       # ranges that reach past the start of the present one
+    for r in ranges:
+        near = [q for q in near if q[1] > r[0]]
+        for q in near:
+            if r[3] or q[3]:
+                lo, hi = q[0], max(q[1], r[1])
+                if torch.any(_bytes(q[4], lo, hi) & _bytes(r[4], lo, hi)):
+                    raise RuntimeError(f"clip_grads: tensors {q[2]} and {r[2]} overlap in memory" if q[2] != r[2] else
+                                       f"clip_grads: output {r[2]} overlaps its gradient in memory without being it")
+        near.append(r)
+
+
 def global_norm(grads) -> torch.Tensor:
     """L2 norm of all tensors together (a scalar tensor on their device; fp32 on a GPU).
     None stands for an absent gradient.  Nothing waits on the host."""
@@ -79,6 +114,7 @@ def clip_grads(grads, max_norm: float, out=None) -> torch.Tensor:
     to = ts if out is None else _floating("clip_grads", [o for g, o in zip(grads, out) if g is not None])
     if len(to) != len(ts) or any(o.shape != g.shape for g, o in zip(ts, to)):
         raise ValueError("clip_grads: every gradient needs an output of its own shape")
+    _check_apart(ts, to)
     norm = global_norm(ts)
     with torch.no_grad():
         f = torch.where((norm <= max_norm) | (norm == 0), 1.0, max_norm / (norm + 1e-6))

@@ -123,6 +123,25 @@ def test_clip_refusals():
     assert float(global_norm([])) == 0.0 and float(clip_grads([None], 1.0)) == 0.0
 
 
+def test_clip_refuses_overlapping_outputs():
+    a = torch.randn(60, 66)
+    keep, v, other = a.clone(), a[:, ::2], torch.randn(60, 33)
+    for grads, out in (([a, a], None), ([a[:31], a[30:]], None), ([v, v], None), ([v, a[:, 30:50]], None), ([a[5:9], v], None),
+                       ([other, a[3]], [v, a[3]]), ([v, other], [torch.empty_like(v), v]), ([v[1:]], [v[:-1]]),
+                       ([a[:50]], [a[1:51]]), ([a.as_strided((40, 50), (40, 1))], None), ([torch.randn(1).expand(5)], None)):
+        with pytest.raises(RuntimeError, match="overlap"):
+            clip_grads(grads, 1e-3, out=out)
+    assert torch.equal(a, keep)
+    for parts in ([v, a[:, 1::2]], [a[:, :7], a[:, 7:20], a[:, 20:]], [a.t()[::2], a.t()[1::2]], [a.t()]):
+        a.copy_(keep)
+        clip_grads(parts, float(keep.norm()) / 2)
+        torch.testing.assert_close(a, keep / 2, rtol=1e-6, atol=0)
+    a.copy_(keep)
+    clip_grads([a[:, 1::2]], 1e9, out=[v])
+    assert torch.equal(v, keep[:, 1::2])
+    clip_grads([v, v], 1e9, out=[other, torch.empty_like(other)])
+
+
 def _example():
     import importlib.util
     import os
