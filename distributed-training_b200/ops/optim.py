@@ -119,7 +119,7 @@ def clip_grads(grads, max_norm: float, out=None) -> torch.Tensor:
     with torch.no_grad():
         f = torch.where((norm <= max_norm) | (norm == 0), 1.0, max_norm / (norm + 1e-6))
         for g, o in zip(ts, to):
-            o.copy_(g * f.to(g.device))
+            o.copy_((g if g.dtype == torch.float64 else g.float()) * f.to(g.device))  # rounded once, to o's type
     return norm
 
 

@@ -123,6 +123,16 @@ def test_clip_refusals():
     assert float(global_norm([])) == 0.0 and float(clip_grads([None], 1.0)) == 0.0
 
 
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+def test_clip_of_16_bits_into_fp32_keeps_fp32(dtype):
+    g = torch.randn(1000).to(dtype)
+    o = torch.empty(1000)
+    f = clip_scale(float(g.double().square().sum()), 0.7)
+    clip_grads([g], 0.7, out=[o])
+    # the factor's rounding and the product's
+    torch.testing.assert_close(o.double(), g.double() * f, rtol=3 * 2.0 ** -24, atol=0)
+
+
 def test_clip_refuses_overlapping_outputs():
     a = torch.randn(60, 66)
     keep, v, other = a.clone(), a[:, ::2], torch.randn(60, 33)
