@@ -171,7 +171,7 @@ def _route_math(z, k, softmax, bias, groups, keep, top, renorm, scale):
         else:
             c = (s if bias is None else s + bias.to(s.dtype)).masked_fill(gone, -math.inf)
         if groups > 1:
-            per = c.view(n, groups, -1)
+            per = c.view(n, groups, e // groups)
             best = torch.sort(per, dim=-1, descending=True).values[..., :top]
             score = best[..., 0] + best[..., 1:].masked_fill(best[..., 1:] == -math.inf, 0.0).sum(-1)
             order = torch.sort(score, dim=-1, descending=True, stable=True).indices

@@ -42,6 +42,15 @@ def test_route_cpu(kw):
     assert g3.shape == (41, 1, 3) and torch.equal(i3.view(41, 3), idx)
 
 
+@pytest.mark.parametrize("kw", ROUTES)
+def test_route_without_tokens(kw):
+    z, kw, _ = _case(kw, 1, 12)
+    for shape in ((0, 12), (3, 0, 12)):
+        gates, idx, load = F.route(torch.empty(shape, requires_grad=True), 3, **kw)
+        assert gates.shape == idx.shape == (*shape[:-1], 3) and load.tolist() == [0] * 12
+        gates.sum().backward()
+
+
 def test_route_gradient_cpu():
     z = torch.randn(5, 8, dtype=torch.float64, requires_grad=True)
     for kw in (dict(), dict(renorm=False), dict(score="sigmoid", scale=2.5)):
