@@ -226,17 +226,19 @@ def route(logits, k: int, *, score: str = "softmax", bias=None, groups: int = 1,
 
 
 def _experts_math(x, w1, b1, w2, b2, idx, gates):
-    """``expert_mlp`` with torch ops, expert by expert."""
-    y = x.new_zeros(x.shape[0], w2.shape[2])
+    """``expert_mlp`` with torch ops, expert by expert.  The products are of the inputs' type; a token's sums over
+    its slots (and those of its gradient) are fp32 at least."""
+    wide = torch.promote_types(x.dtype, torch.float32)
+    rows, y = x.to(wide), x.new_zeros(x.shape[0], w2.shape[2], dtype=wide)
     for e in range(w1.shape[0]):
         tok, slot = torch.nonzero(idx == e, as_tuple=True)
         if tok.numel() == 0:
             continue
-        h = x[tok] @ w1[e]
+        h = rows[tok].to(x.dtype) @ w1[e]
         h = F.gelu(h if b1 is None else h + b1[e], approximate="tanh") @ w2[e]
         h = h if b2 is None else h + b2[e]
-        y = y.index_add(0, tok, gates[tok, slot][:, None].to(h.dtype) * h)
-    return y
+        y = y.index_add(0, tok, gates[tok, slot][:, None].to(wide) * h.to(wide))
+    return y.to(x.dtype)
 
 
 def expert_mlp(x, w1, b1, w2, b2, idx, gates):

@@ -92,6 +92,28 @@ def test_expert_mlp_gradient_cpu():
     assert torch.autograd.gradcheck(lambda x, w1, b1, w2, b2, g: F.expert_mlp(x, w1, b1, w2, b2, idx, g), leaves)
 
 
+def test_expert_mlp_sums_of_bf16_rows():
+    # 64 slots a token, outputs and input gradients of one sign: the sums over a token's slots are fp32.  Each
+    # value passes four roundings to bf16 at most, 0.43 u each in the 2-norm; bf16 sums are off by 0.43 u sqrt(64 / 3).
+    u = 2.0 ** -8
+    g = torch.Generator().manual_seed(5)
+    r = lambda *s: torch.rand(*s, generator=g)  # noqa: E731
+    n, c, e = 40, 8, 64
+    t = [r(n, c), r(e, c, 16), r(e, 16), r(e, 16, 6), r(e, 6)]
+    idx = torch.stack([torch.randperm(e, generator=g) for _ in range(n)])
+    t = [v.bfloat16().requires_grad_() for v in t]
+    gates = (0.5 + r(n, e)).requires_grad_()
+    dy = r(n, 6).bfloat16()
+    y = F.expert_mlp(*t, idx, gates)
+    d = [v.detach().double().requires_grad_() for v in (*t, gates)]
+    ref = experts64(*d[:5], idx, d[5])
+    rel = lambda a, b: float(((a.double() - b).norm() / b.norm()).detach())  # noqa: E731
+    assert y.dtype == torch.bfloat16 and rel(y, ref) <= 1.0 * u
+    dx, dg = torch.autograd.grad(y, (t[0], gates), dy)
+    wx, wg = torch.autograd.grad(ref, (d[0], d[5]), dy.double())
+    assert dg.dtype == torch.float32 and rel(dx, wx) <= 1.0 * u and rel(dg, wg) <= 1.0 * u
+
+
 def test_expert_mlp_refusals():
     x, w1, b1, w2, b2, idx, gates = _experts(4, 3, 4, 3, 3, 2)
     for bad in ((x[:, :2], w1, b1, w2, b2, idx, gates), (x, w1, b1, w2[:2], b2, idx, gates),
