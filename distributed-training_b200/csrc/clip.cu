@@ -480,7 +480,7 @@ static void launch_lists(const std::vector<ClipDesc>& all, size_t at, size_t cou
 
 // The norm (fp32 scalar) of the tensors `in` together (those that are there); with `scale`
 // also in[i] *= factor or, with `out` (aligned with `in`, of the same shapes),
-// out[i] = in[i] * factor.  out[i] may be in[i].
+// out[i] = in[i] * factor (0 where there is no in[i]).  out[i] may be in[i].
 at::Tensor clip_grads(std::vector<std::optional<at::Tensor>> in,
                       std::optional<std::vector<std::optional<at::Tensor>>> out, double max_norm, bool scale) {
   TORCH_CHECK_VALUE(max_norm >= 0.0, "clip_grads: max_norm must not be negative, got ", max_norm);
@@ -501,8 +501,17 @@ at::Tensor clip_grads(std::vector<std::optional<at::Tensor>> in,
   std::vector<ClipRange> ranges;
   dense.reserve(in.size());
   if (scale) ranges.reserve(out ? 2 * in.size() : in.size());
+  std::vector<const at::Tensor*> absent;  // outputs without a gradient
   for (size_t i = 0; i < in.size(); ++i) {
-    if (!in[i]) continue;
+    if (!in[i]) {
+      if (scale && out && (*out)[i] && (*out)[i]->numel()) {
+        const at::Tensor& b = *(*out)[i];
+        TORCH_CHECK(b.device() == dev, "clip_grads: tensor ", i, " is on another device");
+        ranges.push_back(clip_range(b, b.is_non_overlapping_and_dense(), (int)i, true));
+        absent.push_back(&b);
+      }
+      continue;
+    }
     const at::Tensor& a = *in[i];
     TORCH_CHECK_VALUE(!scale || !out || (*out)[i], "clip_grads: every gradient needs an output of its own shape");
     const at::Tensor* b = !scale ? nullptr : out ? &*(*out)[i] : &a;
@@ -528,6 +537,7 @@ at::Tensor clip_grads(std::vector<std::optional<at::Tensor>> in,
     else strided.push_back(strided_desc(a, b));
   }
   check_ranges(ranges);
+  for (const at::Tensor* b : absent) b->zero_();
 
   // launches: lists of at most 960 tensors, each with a grid fixed by its number of chunks
   struct Part { size_t at, count; int grid; };

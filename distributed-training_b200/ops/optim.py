@@ -98,9 +98,11 @@ def clip_grads(grads, max_norm: float, out=None) -> torch.Tensor:
     ``grads`` may differ in size, layout and type (fp32, bf16, fp16); None stands for an
     absent one.  They are scaled in place, or, with ``out`` (a list aligned with
     ``grads``), written there scaled - possibly in another type, such as bf16 gradients
-    into the slices of a flat fp32 buffer - and left as they are.  A NaN or infinite
-    norm shows in the result: the gradients become NaN or 0, as with any clipping that
-    does not look at the norm on the host.
+    into the slices of a flat fp32 buffer - and left as they are; the output of an absent
+    gradient becomes 0, so that nothing of an earlier step stays in the buffer.  Outputs
+    that overlap one another or a gradient (other than in place) are refused.  A NaN or
+    infinite norm shows in the result: the gradients become NaN or 0, as with any clipping
+    that does not look at the norm on the host.
     """
     grads = list(grads)
     if _on_gpu(grads):
@@ -112,14 +114,17 @@ def clip_grads(grads, max_norm: float, out=None) -> torch.Tensor:
         raise ValueError(f"clip_grads: {len(grads)} gradients but {len(out)} outputs")
     ts = _floating("clip_grads", grads)
     to = ts if out is None else _floating("clip_grads", [o for g, o in zip(grads, out) if g is not None])
+    absent = [] if out is None else _floating("clip_grads", [o for g, o in zip(grads, out) if g is None])
     if len(to) != len(ts) or any(o.shape != g.shape for g, o in zip(ts, to)):
         raise ValueError("clip_grads: every gradient needs an output of its own shape")
-    _check_apart(ts, to)
+    _check_apart(ts + absent, to + absent)
     norm = global_norm(ts)
     with torch.no_grad():
         f = torch.where((norm <= max_norm) | (norm == 0), 1.0, max_norm / (norm + 1e-6))
         for g, o in zip(ts, to):
             o.copy_((g if g.dtype == torch.float64 else g.float()) * f.to(g.device))  # rounded once, to o's type
+        for o in absent:
+            o.zero_()
     return norm
 
 

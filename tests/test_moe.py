@@ -164,6 +164,17 @@ def test_clip_of_16_bits_into_fp32_keeps_fp32(dtype):
     torch.testing.assert_close(o.double(), g.double() * f, rtol=3 * 2.0 ** -24, atol=0)
 
 
+def test_clip_without_a_gradient_zeroes_its_output():
+    flat = torch.full((12,), 7.0)
+    g = [torch.ones(4), None, torch.ones(4)]
+    assert float(clip_grads(g, 1e9, out=[flat[:4], flat[4:8], flat[8:]])) == pytest.approx(math.sqrt(8))
+    assert flat.tolist() == [1.0] * 4 + [0.0] * 4 + [1.0] * 4
+    clip_grads([None, None], 1.0, out=[flat[:6], None])
+    assert flat.tolist() == [0.0] * 8 + [1.0] * 4
+    with pytest.raises(RuntimeError, match="overlap"):
+        clip_grads([torch.ones(4), None], 1.0, out=[flat[:4], flat[2:6]])
+
+
 def test_clip_refuses_overlapping_outputs():
     a = torch.randn(60, 66)
     keep, v, other = a.clone(), a[:, ::2], torch.randn(60, 33)

@@ -495,6 +495,15 @@ def test_clip_refuses_outputs_that_overlap_their_own_gradients():
     assert torch.equal(a.double(), want)
 
 
+def test_clip_without_a_gradient_zeroes_its_output_gpu():
+    flat = torch.full((12,), 7.0, device="cuda")
+    g = [torch.ones(4, device="cuda"), None, torch.ones(4, device="cuda"), None]
+    clip_grads(g, 1e9, out=[flat[:4], flat[4:8:2], flat[8:], None])
+    assert flat.tolist() == [1.0] * 4 + [0.0, 7.0, 0.0, 7.0] + [1.0] * 4
+    with pytest.raises(RuntimeError, match="overlap"):
+        clip_grads(g[:2], 1.0, out=[flat[:4], flat[2:6]])
+
+
 def _cells(shape, stride, at):
     cells = torch.tensor([at])
     for n, s in zip(shape, stride):
