@@ -27,6 +27,13 @@ using torch::autograd::AutogradContext;
 using torch::autograd::Variable;
 using torch::autograd::variable_list;
 
+// Whether a tensor carries a forward-mode derivative.  The kernels have none, so the callers compute such inputs
+// with torch ops, which do.
+static bool is_dual(const torch::Tensor& t) { return t.defined() && t._fw_grad(/*level=*/0).defined(); }
+static void check_not_dual(const torch::Tensor& dy, const char* what) {
+  TORCH_CHECK_NOT_IMPLEMENTED(!is_dual(dy), what, ": a forward-mode derivative through the kernels' backward is not implemented");
+}
+
 struct RouteFn : public torch::autograd::Function<RouteFn> {
   static variable_list forward(AutogradContext* ctx, Variable logits, int64_t k, bool softmax,
                                c10::optional<torch::Tensor> bias, int64_t groups, int64_t keep, int64_t top,
@@ -44,6 +51,7 @@ struct RouteFn : public torch::autograd::Function<RouteFn> {
   static variable_list backward(AutogradContext* ctx, variable_list grads) {
     variable_list out(9);
     if (!grads[0].defined()) return out;
+    check_not_dual(grads[0], "route");
     const auto saved = ctx->get_saved_variables();
     at::AutoDispatchBelowADInplaceOrView guard;
     out[0] = route_bwd(saved[0], saved[1], grads[0].contiguous(), ctx->saved_data["softmax"].toBool(),
@@ -53,7 +61,7 @@ struct RouteFn : public torch::autograd::Function<RouteFn> {
 };
 
 // route on logits of any leading shape and layout; nothing where the kernels do not take them (other types or
-// devices, more than 512 experts, 32 slots or 32 groups).
+// devices, more than 512 experts, 32 slots or 32 groups, forward-mode derivatives).
 c10::optional<std::tuple<torch::Tensor, torch::Tensor, torch::Tensor>> route_autograd(
     torch::Tensor logits, int64_t k, const std::string& score, c10::optional<torch::Tensor> bias, int64_t groups,
     int64_t keep, int64_t top, bool renorm, double scale) {
@@ -70,7 +78,9 @@ c10::optional<std::tuple<torch::Tensor, torch::Tensor, torch::Tensor>> route_aut
   TORCH_CHECK_VALUE(!biased || (bias->dim() == 1 && bias->size(0) == e && bias->device() == logits.device()),
                     "route: bias must be [", e, "] on the logits' device");
   const auto t = logits.scalar_type();
-  if (!logits.is_cuda() || (t != at::kFloat && t != at::kBFloat16) || e > 512 || k > 32 || groups > 32) return c10::nullopt;
+  if (!logits.is_cuda() || (t != at::kFloat && t != at::kBFloat16) || e > 512 || k > 32 || groups > 32 ||
+      is_dual(logits))
+    return c10::nullopt;
   if (biased) bias = bias->detach().to(at::kFloat).contiguous();
   const bool two = logits.dim() == 2;
   auto shape = logits.sizes().vec();
@@ -98,6 +108,7 @@ struct ExpertsFn : public torch::autograd::Function<ExpertsFn> {
   static variable_list backward(AutogradContext* ctx, variable_list grads) {
     variable_list out(7);
     if (!grads[0].defined()) return out;
+    check_not_dual(grads[0], "expert_mlp");
     const auto saved = ctx->get_saved_variables();
     at::AutoDispatchBelowADInplaceOrView guard;
     const auto &x = saved[0], &w1 = saved[1], &w2 = saved[2], &gates = saved[3];
@@ -122,7 +133,7 @@ struct ExpertsFn : public torch::autograd::Function<ExpertsFn> {
 };
 
 // expert_mlp on inputs of any leading shape and layout; nothing where the kernels do not take them (other
-// types or devices, widths that are not multiples of 8).
+// types or devices, widths that are not multiples of 8, forward-mode derivatives).
 c10::optional<torch::Tensor> experts_autograd(torch::Tensor x, torch::Tensor w1, c10::optional<torch::Tensor> b1,
                                               torch::Tensor w2, c10::optional<torch::Tensor> b2, torch::Tensor idx,
                                               torch::Tensor gates) {
@@ -139,7 +150,8 @@ c10::optional<torch::Tensor> experts_autograd(torch::Tensor x, torch::Tensor w1,
   const int64_t c = x.size(-1), k = idx.size(-1);
   if (!fast(x) || !fast(w1) || !fast(w2) || (there(b1) && !fast(*b1)) || (there(b2) && !fast(*b2)) ||
       !gates.is_cuda() || (gt != at::kFloat && gt != at::kBFloat16) || c % 8 || w1.size(2) % 8 || w2.size(2) % 8 ||
-      w1.size(0) > 512 || k > 32)
+      w1.size(0) > 512 || k > 32 || is_dual(x) || is_dual(w1) || is_dual(w2) || is_dual(gates) ||
+      (there(b1) && is_dual(*b1)) || (there(b2) && is_dual(*b2)))
     return c10::nullopt;
   const bool two = x.dim() == 2;
   auto shape = x.sizes().vec();

@@ -358,6 +358,43 @@ def test_experts_bwd_fp32_weight_gradients():
     assert all(torch.equal(p, q.to(torch.bfloat16)) for p, q in zip(b, f))
 
 
+# ----------------------------------------------------------------------- derivatives of other kinds
+@pytest.mark.parametrize("score", ["softmax", "sigmoid"])
+def test_route_forward_mode(score):
+    import torch.autograd.forward_ad as fwd
+    z, d = torch.randn(33, 12), torch.randn(33, 12)
+    kw = dict(score=score, scale=1.5)
+    with torch.no_grad(), fwd.dual_level():
+        gates, idx, _ = F.route(fwd.make_dual(z.cuda(), d.cuda()), 3, **kw)
+        got = fwd.unpack_dual(gates).tangent
+    at = [gates64(z.double() + s * 1e-6 * d.double(), idx.cpu().long(), softmax=score == "softmax", scale=1.5) for s in (1, -1)]
+    # the difference's own error is about h^2; fp32 tangents
+    torch.testing.assert_close(got.cpu().double(), (at[0] - at[1]) / 2e-6, rtol=1e-5, atol=1e-6)
+    zg = z.cuda().requires_grad_()
+    with fwd.dual_level():
+        with pytest.raises(NotImplementedError, match="route"):
+            g, _, _ = F.route(zg, 3, **kw)
+            torch.autograd.grad(g, zg, fwd.make_dual(torch.ones_like(g), torch.ones_like(g)))
+
+
+@pytest.mark.parametrize("name", ["x", "w1", "b1", "w2", "b2", "gates"])
+def test_expert_mlp_forward_mode(name):
+    import torch.autograd.forward_ad as fwd
+    t, dy = _inputs(20, 64, 96, 64, 4, 2, gate=torch.float32)
+    d = torch.randn_like(t[name])
+    with torch.no_grad(), fwd.dual_level():
+        y = F.expert_mlp(**dict(t, **{name: fwd.make_dual(t[name], d)}))
+        got = fwd.unpack_dual(y).tangent
+    t64 = {m: v.double() if v.is_floating_point() else v for m, v in t.items()}
+    h = 1e-5
+    at = [experts64(**dict(t64, **{name: t64[name] + s * h * d.double()})) for s in (1, -1)]
+    assert got is not None and _rel(got, (at[0] - at[1]) / (2 * h)) <= 2 * U
+    x = t["x"].requires_grad_()
+    with fwd.dual_level():
+        with pytest.raises(NotImplementedError, match="expert_mlp"):
+            torch.autograd.grad(F.expert_mlp(**t), x, fwd.make_dual(dy, dy))
+
+
 # ----------------------------------------------------------------------- clipping
 def _clip_check(grads, max_norm, outs=None):
     want = [g.double().clone() for g in grads]
