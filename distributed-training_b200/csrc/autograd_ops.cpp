@@ -6,6 +6,9 @@
 // engine's own share is about 40.
 #include <torch/extension.h>
 
+#include <torch/csrc/autograd/functions/basic_ops.h>
+#include <torch/csrc/autograd/functions/utils.h>
+
 namespace dtb {
 
 // route.cu
@@ -34,6 +37,18 @@ static void check_not_dual(const torch::Tensor& dy, const char* what) {
   TORCH_CHECK_NOT_IMPLEMENTED(!is_dual(dy), what, ": a forward-mode derivative through the kernels' backward is not implemented");
 }
 
+// The kernels' gradients have no graph of their own.  Where one is asked for (create_graph), they hang on a node that
+// raises, and whose edges lead to what they were made from: no derivative passes it by.
+static variable_list once_differentiable(variable_list grads, const variable_list& from, const char* what) {
+  if (!torch::GradMode::is_enabled()) return grads;
+  auto node = std::make_shared<torch::autograd::Error>(
+      std::string(what) + ": the gradient of the kernels' gradient is not implemented",
+      torch::autograd::collect_next_edges(from));
+  for (auto& g : grads)
+    if (g.defined()) torch::autograd::set_history(g, node);
+  return grads;
+}
+
 struct RouteFn : public torch::autograd::Function<RouteFn> {
   static variable_list forward(AutogradContext* ctx, Variable logits, int64_t k, bool softmax,
                                c10::optional<torch::Tensor> bias, int64_t groups, int64_t keep, int64_t top,
@@ -53,10 +68,12 @@ struct RouteFn : public torch::autograd::Function<RouteFn> {
     if (!grads[0].defined()) return out;
     check_not_dual(grads[0], "route");
     const auto saved = ctx->get_saved_variables();
-    at::AutoDispatchBelowADInplaceOrView guard;
-    out[0] = route_bwd(saved[0], saved[1], grads[0].contiguous(), ctx->saved_data["softmax"].toBool(),
-                       ctx->saved_data["renorm"].toBool(), ctx->saved_data["scale"].toDouble());
-    return out;
+    {
+      at::AutoDispatchBelowADInplaceOrView guard;
+      out[0] = route_bwd(saved[0], saved[1], grads[0].contiguous(), ctx->saved_data["softmax"].toBool(),
+                         ctx->saved_data["renorm"].toBool(), ctx->saved_data["scale"].toDouble());
+    }
+    return once_differentiable(std::move(out), {saved[0], grads[0]}, "route");
   }
 };
 
@@ -98,10 +115,9 @@ struct ExpertsFn : public torch::autograd::Function<ExpertsFn> {
                           c10::optional<Variable> b2, Variable idx, Variable gates) {
     at::AutoDispatchBelowADInplaceOrView guard;
     auto out = experts_fwd(x, w1, b1, w2, b2, idx, gates, true);
-    variable_list keep{x, w1, w2, gates, b2.has_value() ? *b2 : torch::Tensor()};
+    variable_list keep{x, w1, w2, gates, b2.value_or(torch::Tensor()), b1.value_or(torch::Tensor())};
     keep.insert(keep.end(), out.begin() + 1, out.end());
     ctx->save_for_backward(keep);
-    ctx->saved_data["b1"] = b1.has_value() && b1->defined();
     ctx->set_materialize_grads(false);
     return out[0];
   }
@@ -110,25 +126,30 @@ struct ExpertsFn : public torch::autograd::Function<ExpertsFn> {
     if (!grads[0].defined()) return out;
     check_not_dual(grads[0], "expert_mlp");
     const auto saved = ctx->get_saved_variables();
+    compute(ctx, saved, grads[0], out);
+    variable_list from(saved.begin(), saved.begin() + 6);  // x, w1, w2, gates, b2, b1
+    from.push_back(grads[0]);
+    return once_differentiable(std::move(out), from, "expert_mlp");
+  }
+  static void compute(AutogradContext* ctx, const variable_list& saved, const Variable& dy, variable_list& out) {
     at::AutoDispatchBelowADInplaceOrView guard;
     const auto &x = saved[0], &w1 = saved[1], &w2 = saved[2], &gates = saved[3];
     auto dw1 = torch::empty_like(w1), dw2 = torch::empty_like(w2);
     c10::optional<torch::Tensor> db1, db2;
-    if (ctx->saved_data["b1"].toBool()) db1 = torch::empty({w1.size(0), w1.size(2)}, w1.options());
+    if (saved[5].defined()) db1 = torch::empty_like(saved[5]);
     c10::optional<torch::Tensor> b2;
     if (saved[4].defined()) {
       b2 = saved[4];
       db2 = torch::empty_like(*b2);
     }
-    auto d = experts_bwd(grads[0].contiguous(), x, w1, w2, b2, gates,
-                         std::vector<torch::Tensor>(saved.begin() + 5, saved.end()), dw1, db1, dw2, db2);
+    auto d = experts_bwd(dy.contiguous(), x, w1, w2, b2, gates, std::vector<torch::Tensor>(saved.begin() + 6, saved.end()),
+                         dw1, db1, dw2, db2);
     out[0] = d[0];
     out[1] = dw1;
     if (db1) out[2] = *db1;
     out[3] = dw2;
     if (db2) out[4] = *db2;
     out[6] = d[1];
-    return out;
   }
 };
 

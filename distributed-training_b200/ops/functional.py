@@ -203,7 +203,8 @@ def route(logits, k: int, *, score: str = "softmax", bias=None, groups: int = 1,
     idx -1 and gate 0.  A NaN counts as the largest value and shows in the gates.
 
     idx (..., k) is int32, load int32 [experts] counts the slots of each expert.  The
-    gates are differentiable in the logits.
+    gates are differentiable in the logits (through the kernels once: a second derivative
+    raises; forward mode runs torch ops).
     """
     if logits.is_cuda:
         out = K.route(logits, k, score, bias, groups, keep_groups, group_top, renorm, scale)
@@ -247,8 +248,9 @@ def expert_mlp(x, w1, b1, w2, b2, idx, gates):
     x (..., c); w1 [experts, c, h], w2 [experts, h, co] (in, out) as in ``linear``; b1
     [experts, h], b2 [experts, co] or None; idx (..., k) int32 or int64, where -1 is a
     slot without an expert; gates (..., k).  y (..., co) has x's type; gradients reach
-    x, the weights, the biases and the gates, each in its own type.  An expert that no
-    slot names gets a gradient of zeros.
+    x, the weights, the biases and the gates, each in its own type (through the kernels once:
+    a second derivative raises; forward mode runs torch ops).  An expert that no slot names
+    gets a gradient of zeros.
     """
     if x.is_cuda:
         y = K.experts(x, w1, b1, w2, b2, idx, gates)

@@ -395,6 +395,28 @@ def test_expert_mlp_forward_mode(name):
             torch.autograd.grad(F.expert_mlp(**t), x, fwd.make_dual(dy, dy))
 
 
+def test_second_derivatives_raise():
+    z = torch.randn(20, 8, device="cuda").requires_grad_()
+    gates, _, _ = F.route(z, 2)
+    w = torch.randn(20, 2, device="cuda")
+    dz, = torch.autograd.grad((gates * w).sum() + (z ** 3).sum(), z, create_graph=True)
+    plain, = torch.autograd.grad((F.route(z, 2)[0] * w).sum() + (z ** 3).sum(), z)
+    assert torch.equal(dz, plain)                   # the first derivative is there
+    with pytest.raises(RuntimeError, match="route.*not implemented"):
+        (dz ** 2).sum().backward()
+    for bias in (True, False):
+        t, dy = _inputs(20, 64, 96, 64, 4, 2, bias)
+        names = [m for m in ("x", "w1", "b1", "w2", "b2", "gates") if t[m] is not None]
+        for m in names:
+            t[m].requires_grad_()
+        first = torch.autograd.grad(F.expert_mlp(**t), [t[m] for m in names], dy, create_graph=True)
+        plain = torch.autograd.grad(F.expert_mlp(**t), [t[m] for m in names], dy)
+        for m, a, b in zip(names, first, plain):
+            assert torch.equal(a, b)
+            with pytest.raises(RuntimeError, match="expert_mlp.*not implemented"):
+                torch.autograd.grad(a.float().square().sum() + t[m].float().sum(), t[m], retain_graph=True)
+
+
 # ----------------------------------------------------------------------- clipping
 def _clip_check(grads, max_norm, outs=None):
     want = [g.double().clone() for g in grads]
