@@ -110,6 +110,12 @@ c10::optional<std::tuple<torch::Tensor, torch::Tensor, torch::Tensor>> route_aut
   return std::make_tuple(out[0].view(shape), out[1].view(shape), out[2]);
 }
 
+// Contiguous, and at a 16-byte boundary as the experts' loads need it: views of a flat buffer may start anywhere.
+static torch::Tensor aligned(const torch::Tensor& t) {
+  auto c = t.contiguous();
+  return reinterpret_cast<uintptr_t>(c.const_data_ptr()) % 16 ? c.clone() : c;
+}
+
 struct ExpertsFn : public torch::autograd::Function<ExpertsFn> {
   static Variable forward(AutogradContext* ctx, Variable x, Variable w1, c10::optional<Variable> b1, Variable w2,
                           c10::optional<Variable> b2, Variable idx, Variable gates) {
@@ -142,7 +148,7 @@ struct ExpertsFn : public torch::autograd::Function<ExpertsFn> {
       b2 = saved[4];
       db2 = torch::empty_like(*b2);
     }
-    auto d = experts_bwd(dy.contiguous(), x, w1, w2, b2, gates, std::vector<torch::Tensor>(saved.begin() + 6, saved.end()),
+    auto d = experts_bwd(aligned(dy), x, w1, w2, b2, gates, std::vector<torch::Tensor>(saved.begin() + 6, saved.end()),
                          dw1, db1, dw2, db2);
     out[0] = d[0];
     out[1] = dw1;
@@ -177,14 +183,14 @@ c10::optional<torch::Tensor> experts_autograd(torch::Tensor x, torch::Tensor w1,
   const bool two = x.dim() == 2;
   auto shape = x.sizes().vec();
   shape.back() = w2.size(2);
-  const auto flat = [two](const torch::Tensor& t, int64_t n) { return (two ? t : t.reshape({-1, n})).contiguous(); };
-  x = flat(x, c);
-  idx = flat(idx, k);
-  gates = flat(gates, k);
-  w1 = w1.contiguous();
-  w2 = w2.contiguous();
-  if (there(b1)) b1 = b1->contiguous();
-  if (there(b2)) b2 = b2->contiguous();
+  const auto flat = [two](const torch::Tensor& t, int64_t n) { return two ? t : t.reshape({-1, n}); };
+  x = aligned(flat(x, c));
+  idx = flat(idx, k).contiguous();
+  gates = flat(gates, k).contiguous();
+  w1 = aligned(w1);
+  w2 = aligned(w2);
+  if (there(b1)) b1 = aligned(*b1);
+  if (there(b2)) b2 = aligned(*b2);
   const auto wants = [&](const c10::optional<torch::Tensor>& t) { return there(t) && t->requires_grad(); };
   torch::Tensor y;
   if (!torch::GradMode::is_enabled() || !(x.requires_grad() || w1.requires_grad() || w2.requires_grad() ||

@@ -250,7 +250,8 @@ def expert_mlp(x, w1, b1, w2, b2, idx, gates):
     slot without an expert; gates (..., k).  y (..., co) has x's type; gradients reach
     x, the weights, the biases and the gates, each in its own type (through the kernels once:
     a second derivative raises; forward mode runs torch ops).  An expert that no slot names
-    gets a gradient of zeros.
+    gets a gradient of zeros.  Any layout will do: what is not contiguous from a 16-byte
+    boundary on is copied for the kernels first.
     """
     if x.is_cuda:
         y = K.experts(x, w1, b1, w2, b2, idx, gates)

@@ -286,6 +286,31 @@ def test_expert_mlp_shapes_and_streams():
     assert _rel(F.expert_mlp(**q), experts64(**{m: v.double() if v.is_floating_point() else v for m, v in q.items()})) < 2 * U
 
 
+def _off_by_one(t):
+    """The same values one element past a 16-byte boundary."""
+    v = torch.empty(t.numel() + 1, dtype=t.dtype, device=t.device)[1:].view(t.shape)
+    return v.copy_(t)
+
+
+@pytest.mark.parametrize("n", [2, 40, 300])         # streaming, 64-row and 128-row tiles
+@pytest.mark.parametrize("gate,idx_type", [(torch.bfloat16, torch.int32), (torch.float32, torch.int64)])
+def test_expert_mlp_unaligned(n, gate, idx_type):
+    t, dy = _inputs(n, 72, 136, 64, 4, 2, gate=gate, idx_type=idx_type)
+    y = F.expert_mlp(**t)
+    for m in t:
+        assert torch.equal(y, F.expert_mlp(**dict(t, **{m: _off_by_one(t[m])}))), m
+    names = ("x", "w1", "b1", "w2", "b2", "gates")
+    a = {m: t[m].clone().requires_grad_(m in names) for m in t}
+    b = {m: _off_by_one(t[m]).requires_grad_(m in names) for m in t}
+    ga = torch.autograd.grad(F.expert_mlp(**a), [a[m] for m in names], dy)
+    gb = torch.autograd.grad(F.expert_mlp(**b), [b[m] for m in names], _off_by_one(dy))
+    assert all(torch.equal(p, q) for p, q in zip(ga, gb))
+    # the output's gradient as a slice that starts at any element
+    z = torch.cat([torch.zeros(1, device="cuda", dtype=torch.bfloat16), F.expert_mlp(**a).view(-1)])
+    gc = torch.autograd.grad(z, [a[m] for m in names], torch.cat([z[:1].detach(), dy.view(-1)]))
+    assert all(torch.equal(p, q) for p, q in zip(ga, gc))
+
+
 def test_expert_mlp_all_slots_empty():
     for n in (2, 20, 600):
         t, dy = _inputs(n, 64, 136, 72, 4, 2)
