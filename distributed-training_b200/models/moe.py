@@ -44,7 +44,7 @@ class MoE(nn.Module):
         gates, idx, load = F.route(F.linear(x, self.gate), self.topk, bias=self.bias, **self.how)
         if self.training:
             self.load += load
-        return F.expert_mlp(x, self.w1, self.b1, self.w2, self.b2, idx, gates.to(x.dtype))
+        return F.expert_mlp(x, self.w1, self.b1, self.w2, self.b2, idx, gates)
 
     @torch.no_grad()
     def balance(self, rate: float = 1e-3):

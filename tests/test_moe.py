@@ -211,6 +211,19 @@ def test_example_learns_cpu(score):
     assert losses[0] == pytest.approx(math.log(32), abs=0.2) and losses[-1] < losses[0] - 0.3
 
 
+def test_layer_hands_the_gates_on_as_they_are(monkeypatch):
+    import numpy as np
+    from dtrain_b200.models import moe
+    seen = []
+    real = F.expert_mlp
+    monkeypatch.setattr(moe.F, "expert_mlp", lambda *a: (seen.append(a[-1]), real(*a))[1])
+    m = moe.MoE(8, 16, 4, 2, np.random.default_rng(0), torch.bfloat16)
+    x = torch.randn(12, 8).bfloat16()
+    m(x)
+    gates, _, _ = F.route(F.linear(x, m.gate), 2, score="sigmoid", bias=m.bias)
+    assert seen[0].dtype == torch.float32 and torch.equal(seen[0], gates)
+
+
 def test_balance_moves_the_bias_against_the_load():
     import numpy as np
     from dtrain_b200.models.moe import MoE
