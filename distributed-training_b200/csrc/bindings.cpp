@@ -60,6 +60,7 @@ std::vector<torch::Tensor> experts_bwd(torch::Tensor dy, torch::Tensor x, torch:
                                        std::vector<torch::Tensor> saved, torch::Tensor dw1,
                                        c10::optional<torch::Tensor> db1, torch::Tensor dw2,
                                        c10::optional<torch::Tensor> db2);
+std::vector<std::string> experts_tiles(int64_t n, int64_t k, int64_t E, int64_t C, int64_t H, int64_t Co);
 // autograd_ops.cpp
 c10::optional<std::tuple<torch::Tensor, torch::Tensor, torch::Tensor>> route_autograd(
     torch::Tensor logits, int64_t k, const std::string& score, c10::optional<torch::Tensor> bias, int64_t groups,
@@ -183,6 +184,7 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
         py::arg("idx"), py::arg("gates"), py::arg("save"));
   m.def("experts_bwd", &experts_bwd, py::arg("dy"), py::arg("x"), py::arg("w1"), py::arg("w2"), py::arg("b2"), py::arg("gates"),
         py::arg("saved"), py::arg("dw1"), py::arg("db1"), py::arg("dw2"), py::arg("db2"));
+  m.def("experts_tiles", &experts_tiles);
   m.def("route", &route_autograd);
   m.def("experts", &experts_autograd);
   m.def("clip_grads", &clip_grads, py::arg("grads"), py::arg("out"), py::arg("max_norm"), py::arg("scale"));

@@ -1595,6 +1595,15 @@ static MoeTiling moe_weight_tiling(int M, int N, const MoeSizes& z) {
   if (N <= 128 || z.E * ((M + 255) / 256) * ((N + 255) / 256) < num_sms() / 2) return {false, 128};
   return {M > 128, 256};
 }
+// The tiles of a training call's products: up (and dpre), down, dx, dw1, dw2.
+std::vector<std::string> experts_tiles(int64_t n, int64_t k, int64_t E, int64_t C, int64_t H, int64_t Co) {
+  const MoeSizes z{n, k, n * k, E, moe_max_rows(n * k, E)};
+  const auto name = [](const MoeTiling& t) {
+    return t.pair ? std::string("256x256 pair") : "128x" + std::to_string(t.bn);
+  };
+  return {name(moe_rows_tiling((int)H, z)), name(moe_rows_tiling((int)Co, z)), name(moe_rows_tiling((int)C, z)),
+          name(moe_weight_tiling((int)C, (int)H, z)), name(moe_weight_tiling((int)H, (int)Co, z))};
+}
 // Parts of each row's product that the dpre GEMM leaves.
 static int moe_dot_parts(int N, const MoeSizes& z) {
   const int bn = moe_rows_tiling(N, z).bn;

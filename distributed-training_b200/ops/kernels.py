@@ -168,6 +168,11 @@ def experts_bwd(dy, x, w1, w2, b2, gates, saved, dw1, db1, dw2, db2):
     return lib().experts_bwd(dy, x, w1, w2, b2, gates, list(saved), dw1, db1, dw2, db2)
 
 
+def experts_tiles(n: int, k: int, experts: int, c: int, h: int, co: int) -> dict:
+    """Which output tiles the products of a training call of these sizes take on the current GPU (for profiles and tests)."""
+    return dict(zip(("up", "down", "dx", "dw1", "dw2"), lib().experts_tiles(n, k, experts, c, h, co)))
+
+
 def clip_grads(grads, out, max_norm: float, scale: bool = True) -> torch.Tensor:
     """Norm (fp32 scalar) of the CUDA tensors ``grads`` together (None: absent); with
     ``scale`` also ``grads[i] *= factor`` or, with ``out``, ``out[i] = grads[i] * factor``."""

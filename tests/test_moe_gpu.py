@@ -228,6 +228,74 @@ def test_expert_mlp(n, c, h, co, e, k, bias, skew, gate, idx_type):
     assert all(torch.equal(a, b) for a, b in zip(grads, grads2)), "fixed orders of summation"
 
 
+PAIR = dict.fromkeys(("up", "down", "dx", "dw1", "dw2"), "256x256 pair")
+TILES = [  # the sizes of EXPERTS, and the tiles that they are to reach
+    ((4096, 776, 1544, 520, 4, 2, True, 0.3), PAIR),
+    ((6000, 520, 264, 520, 8, 2, True, 3.0), dict(PAIR, dw1="128x128", dw2="128x128")),     # experts without a row
+    ((6001, 264, 520, 328, 8, 2, False, 0.2), dict(PAIR, dw1="128x128", dw2="128x128")),
+    ((700, 264, 520, 328, 40, 6, True, 0.1), dict(PAIR, up="128x256", down="128x256", dx="128x256")),
+    ((900, 104, 264, 264, 40, 2, True, 0.1), dict(up="128x256", down="128x256", dx="128x128", dw1="128x256",
+                                                  dw2="256x256 pair")),
+    ((900, 264, 120, 264, 40, 2, True, 0.0), dict(up="128x128", down="128x256", dx="128x256", dw1="128x128",
+                                                  dw2="128x256")),
+]
+
+
+@pytest.mark.parametrize("sizes,tiles", TILES)
+@pytest.mark.parametrize("gate,idx_type", [(torch.bfloat16, torch.int64), (torch.float32, torch.int32)])
+def test_expert_mlp_on_every_tile(sizes, tiles, gate, idx_type):
+    n, c, h, co, e, k = sizes[:6]
+    assert K.experts_tiles(n, k, e, c, h, co) == tiles
+    test_expert_mlp(*sizes, gate, idx_type)
+
+
+def test_experts_bwd_fp32_weight_gradients_on_pairs():
+    assert K.experts_tiles(4096, 2, 4, 776, 1544, 520) == PAIR
+    t, dy = _inputs(4096, 776, 1544, 520, 4, 2)
+    y, *saved = K.experts_fwd(**t, save=True)
+    b = [torch.empty_like(t[m]) for m in ("w1", "b1", "w2", "b2")]
+    f = [torch.empty_like(v, dtype=torch.float32) for v in b]
+    a = K.experts_bwd(dy, t["x"], t["w1"], t["w2"], t["b2"], t["gates"], saved, *b)
+    c = K.experts_bwd(dy, t["x"], t["w1"], t["w2"], t["b2"], t["gates"], saved, *f)
+    assert all(torch.equal(p, q) for p, q in zip(a, c))
+    assert all(torch.equal(p, q.to(torch.bfloat16)) for p, q in zip(b, f))
+
+
+@pytest.mark.parametrize("n,c,h,co,e,k,train", [(2, 72, 136, 64, 4, 2, False), (40, 72, 136, 64, 4, 2, False),
+                                                (600, 72, 136, 64, 4, 2, False), (300, 72, 136, 64, 4, 2, True),
+                                                (4096, 776, 1544, 520, 4, 2, True)])
+def test_route_and_experts_in_a_graph(n, c, h, co, e, k, train):
+    names = ("x", "w1", "b1", "w2", "b2")
+
+    def inputs(seed):
+        t, dy = _inputs(n, c, h, co, e, k, seed=seed)
+        g = torch.Generator(device="cuda").manual_seed(seed)
+        return [t[m] for m in names] + [torch.randn(n, e, generator=g, device="cuda"), dy]
+    held = inputs(0)
+    leaves = [v.requires_grad_(train) for v in held[:6]]
+
+    def step():
+        x, w1, b1, w2, b2, z, dy = held
+        gates, idx, load = F.route(z, k, score="sigmoid")
+        y = F.expert_mlp(x, w1, b1, w2, b2, idx, gates)
+        return [gates, idx, load, y, *(torch.autograd.grad(y, leaves, dy) if train else ())]
+
+    s = torch.cuda.Stream()
+    s.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(s):
+        step()
+    torch.cuda.current_stream().wait_stream(s)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = step()
+    for seed in (1, 2):
+        with torch.no_grad():
+            for a, b in zip(held, inputs(seed)):
+                a.copy_(b)
+        graph.replay()
+        assert all(torch.equal(a, b) for a, b in zip(out, step()))
+
+
 def test_expert_mlp_gradient_against_differences():
     t, dy = _inputs(40, 64, 96, 64, 4, 2, gate=torch.float32)
     names = ("x", "w1", "b1", "w2", "b2", "gates")
