@@ -752,6 +752,21 @@ __device__ __forceinline__ void slab_get_bf16(const uint8_t* slab, int lane, flo
   for (int j = 0; j < 4; ++j) unpack8(src[slab_unit_bf16(lane, j)], v + 8 * j);
 }
 
+// What a role still has in flight when it leaves its loop, also by a wait that ran out: loads that would land in, and
+// products that would read from and signal to, a CTA that is gone.  Both wait (mbar_wait's limit; the CTA's abort flag
+// does not shorten it) until that is done.  `stage` and `phase`: where the ring's next round goes, so a stage before
+// it was last used in this round, the others in the round before (of which a fresh barrier counts as complete).
+template <int STAGES>
+__device__ __forceinline__ void finish_loads(uint64_t* full_bar, int stage, uint32_t phase) {
+  volatile int never = 0;
+  for (int s = 0; s < STAGES; ++s) mbar_wait(&full_bar[s], s < stage ? phase : phase ^ 1, &never);
+}
+template <int STAGES>
+__device__ __forceinline__ void finish_products(uint64_t* empty_bar, int stage, uint32_t phase) {
+  volatile int never = 0;  // products complete in order: the last stage's
+  mbar_wait(&empty_bar[stage ? stage - 1 : STAGES - 1], stage ? phase : phase ^ 1, &never);
+}
+
 // One 32x32 chunk: this lane's row of 32 accumulators -> slab -> TMA store.  `staged` (MOE_DGELU): the chunk's
 // pre-activations, already in shared memory; null: read from global memory.
 __device__ __forceinline__ void moe_epi_chunk(const MoeGemmArgs& a, const CUtensorMap* tmOut, const CUtensorMap* tmAux,
@@ -921,6 +936,7 @@ __global__ void __maxnreg__(DTB_CORESIDENT_MAXNREG)
           if (++stage == Cfg::STAGES) { stage = 0; phase ^= 1; }
         }
       }
+      finish_loads<Cfg::STAGES>(full_bar, stage, phase);
     }
   } else if (warp == 1) {
     if (lane == 0) {
@@ -959,6 +975,7 @@ __global__ void __maxnreg__(DTB_CORESIDENT_MAXNREG)
         tc_commit(&tfull_bar[ab]);
         if (++ab == 2) { ab = 0; aphase ^= 1; }
       }
+      finish_products<Cfg::STAGES>(empty_bar, stage, phase);
     }
   } else {
     // -------------------------------------------------------------- epilogue
@@ -1143,6 +1160,13 @@ __global__ void __maxnreg__(DTB_CORESIDENT_MAXNREG)
           if (++stage == Cfg::STAGES) { stage = 0; phase ^= 1; }
         }
       }
+      // Both CTAs' loads are counted on the leader's barriers.  The other one, should a wait have run out here, gives
+      // its own a millisecond.
+      if (leader) {
+        finish_loads<Cfg::STAGES>(full_bar, stage, phase);
+      } else if (!ok) {
+        for (const uint64_t t0 = globaltimer_ns(); globaltimer_ns() - t0 < 1000000;) {}
+      }
     }
   } else if (warp == 1) {
     if (lane == 0 && leader) {
@@ -1181,6 +1205,7 @@ __global__ void __maxnreg__(DTB_CORESIDENT_MAXNREG)
         tc_commit_pair(&tfull_bar[ab], 0x3);
         if (++ab == 2) { ab = 0; aphase ^= 1; }
       }
+      finish_products<Cfg::STAGES>(empty_bar, stage, phase);
     }
   } else {
     // -------------------------------------------------------------- epilogue (both CTAs)
@@ -1194,6 +1219,7 @@ __global__ void __maxnreg__(DTB_CORESIDENT_MAXNREG)
     // the tile's first two before its products are done.  (The dpre GEMM of 65536 rows x 1536, K 768, took 224 us
     // with the lanes reading a row each and scalar arithmetic, 198 with TMA, 179 with two operations an instruction.)
     const bool stage_aux = MODE == MOE_DX && args.epi == MOE_DGELU;
+    volatile int never = 0;  // these copies are waited for whatever the abort flag says: none stays in flight
     uint32_t ck = 0;
     int ab = 0;
     uint32_t aphase = 0;
@@ -1215,8 +1241,7 @@ __global__ void __maxnreg__(DTB_CORESIDENT_MAXNREG)
       }
       if (q.kb > 0) {
         if (!mbar_wait(&tfull_bar[ab], aphase, abort_flag)) {
-          if (stage_aux) {  // leave no copy in flight
-            volatile int never = 0;
+          if (stage_aux) {
             for (int i = 0; i < min(2, chunks); ++i) mbar_wait(&abar[(ck + i) & 1], ((ck + i) >> 1) & 1, &never);
           }
           break;
@@ -1237,7 +1262,7 @@ __global__ void __maxnreg__(DTB_CORESIDENT_MAXNREG)
           for (int j = 0; j < 32; ++j) v[j] = 0.f;
         }
         epi_slab_acquire(lane, true);
-        if (stage_aux) mbar_wait(&abar[ck & 1], (ck >> 1) & 1, abort_flag);
+        if (stage_aux) mbar_wait(&abar[ck & 1], (ck >> 1) & 1, &never);
         moe_epi_chunk(args, &tmOut, &tmAux, sl, lane, row0, c0 + 32 * i, q.e, MODE == MOE_DW, v, gate,
                       dot, stage_aux ? sl + 2048 : nullptr);
         if (stage_aux && i + 2 < chunks && lane == 0) {  // every lane has read the buffer (moe_epi_chunk synchronises)
@@ -1364,6 +1389,7 @@ __global__ void __launch_bounds__(kThinThreads)
           tma_load_2d(&tmX, smem + stage * Cfg::STAGE_BYTES + Cfg::A_BYTES, &full_bar[stage], kb * kBK, t.y);
           if (++stage == Cfg::STAGES) { stage = 0; phase ^= 1; }
         }
+        finish_loads<Cfg::STAGES>(full_bar, stage, phase);
       }
     } else if (warp == 1) {
       if (lane == 0) {
@@ -1384,6 +1410,7 @@ __global__ void __launch_bounds__(kThinThreads)
           if (++stage == Cfg::STAGES) { stage = 0; phase ^= 1; }
         }
         if (ok) tc_commit(done_bar);
+        finish_products<Cfg::STAGES>(empty_bar, stage, phase);
       }
     } else {
       // lane = a column of the output, TMEM column = a row

@@ -194,6 +194,21 @@ def test_clip_refuses_overlapping_outputs():
     clip_grads([v, v], 1e9, out=[other, torch.empty_like(other)])
 
 
+@pytest.mark.parametrize("stages", [3, 4, 5])
+def test_ring_position_names_the_copies_in_flight(stages):
+    # csrc/moe.cu finish_loads / finish_products: from the ring's next position, which phase of each barrier to wait for
+    passed = lambda done, parity: done % 2 != parity    # a barrier with `done` phases complete  # noqa: E731
+    for issued in range(4 * stages):
+        stage, phase = issued % stages, issued // stages % 2
+        done = [len(range(s, issued, stages)) for s in range(stages)]
+        waits = [phase if s < stage else phase ^ 1 for s in range(stages)]
+        assert all(passed(d, w) for d, w in zip(done, waits))       # all there: no wait
+        for s in range(stages):                                     # one missing: it is waited for
+            assert done[s] == 0 or not passed(done[s] - 1, waits[s])
+        last = stage - 1 if stage else stages - 1
+        assert issued == 0 or last == (issued - 1) % stages and waits[last] == (phase if stage else phase ^ 1)
+
+
 def _example():
     import importlib.util
     import os
