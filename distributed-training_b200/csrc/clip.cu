@@ -41,7 +41,7 @@ enum ClipType : int { CLIP_F32 = 0, CLIP_BF16 = 1, CLIP_F16 = 2 };
 
 struct ClipDesc {
   const void* in;
-  void* out;   // null: the norm only
+  void* out;   // null where only the norm is asked for
   long n;
   int first;   // chunks of the tensors before this one
   short in_t, out_t;
@@ -341,7 +341,7 @@ __global__ void __launch_bounds__(kClipThreads)
   // from the last chunk to the first: the norm has read the last ones last, so they are still in L2
   for (int c = l.chunks - 1 - (int)blockIdx.x; c >= 0; c -= gridDim.x) {
     const ClipDesc& d = l.d[clip_find(l, c)];
-    if (d.out == nullptr || (f == 1.f && d.in == d.out)) continue;
+    if (f == 1.f && d.in == d.out) continue;
     if (d.in_t == CLIP_F32) clip_chunk_scale_to<CLIP_F32>(d, c, f);
     else if (d.in_t == CLIP_BF16) clip_chunk_scale_to<CLIP_BF16>(d, c, f);
     else clip_chunk_scale_to<CLIP_F16>(d, c, f);

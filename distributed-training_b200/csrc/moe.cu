@@ -472,7 +472,7 @@ __global__ void __launch_bounds__(256) moe_join_sums_kernel(JoinArgs<O> first, J
 // For a token or a few the weights of the chosen experts are the whole work: they are
 // streamed once by all SMs, without a plan, in two launches.
 //   up    h[slot] = gelu(x W1_e + b1_e), fp32: a CTA per slot and 8 L columns, its threads in
-//         256 / L rows of W1 by L 16-byte column vectors
+//         512 / L rows of W1 by L 16-byte column vectors
 //   down  y[n] = sum_j gate_j (h W2_e + b2_e): a cluster of 8 CTAs per token and 8 L columns;
 //         each sums an eighth of the token's k H rows of W2, and the leader adds the eight
 //         up in order through distributed shared memory
@@ -486,7 +486,7 @@ __global__ void __launch_bounds__(256) moe_join_sums_kernel(JoinArgs<O> first, J
 constexpr int kFewCluster = 8;
 constexpr int kFewThreads = 512;
 
-// acc (8 columns a thread) summed over the CTA's 256 / L row lanes: s_out[0 .. 8 L), valid after the
+// acc (8 columns a thread) summed over the CTA's 512 / L row lanes: s_out[0 .. 8 L), valid after the
 // __syncthreads that the caller does.
 template <int L>
 __device__ __forceinline__ void few_reduce(float* acc, float (*s_part)[8 * L], float* s_out) {
@@ -1773,10 +1773,10 @@ template <typename I, typename G>
 static void moe_few_launch(const bf16* x, const bf16* w1, const bf16* b1, const bf16* w2, const bf16* b2, const I* idx,
                            const G* gates, float* h, bf16* y, int C, int H, int Co, const MoeSizes& z, cudaStream_t st) {
   const int E = (int)z.E, k = (int)z.k;
-  // the fewest column vectors a row that still leave two CTAs an SM or fewer
+  // the most column vectors a row (whole lines, fewer CTAs to join) that still give every SM a CTA
   const auto lanes = [](long cols, long per) {
     for (int l = 16; l > 4; l /= 2)
-      if ((cols + 8 * l - 1) / (8 * l) * per >= 148) return l;
+      if ((cols + 8 * l - 1) / (8 * l) * per >= num_sms()) return l;
     return 4;
   };
   const int l1 = lanes(H, z.P), l2 = lanes(Co, z.n * kFewCluster);
