@@ -18,6 +18,18 @@
 //
 // The gates are applied in the epilogues, so the backward reads neither the rows' outputs nor a scaled copy of dy.
 //
+// Sums are fp32 (in the products, over a token's slots, over rows).  What is rounded to bf16 on the way, and why;
+// errors in the 2-norm relative to 64 bits, 512 tokens, 4 experts of 768 x 1536, 2 slots a token, where the results'
+// own rounding to bf16 is 0.0017:
+//   act, dpre    operands of a tensor core product.  With them every result but d(gate) is off by 0.0023.
+//   pre          saved for the backward's gelu and its slope: d(gate) 0.0027 (exact pre: 0.0017), dx and dW1 0.0024.
+//                In fp32 it would be twice the bytes of the largest tensor that the backward reads.
+//   yp, dxp      each slot's part of y and dx: 0.0029 and 0.0030 (in fp32 0.0023 and 0.0024, as the forms for few rows
+//                have it, whose parts stay in L2).  Stored in fp32 the pass forward and backward took 1155 us
+//                for 1088 (16384 tokens, 16 experts 768 x 1536) and 1859 for 1777 (8192, 32 of 2048 x 2048).
+// db1 sums dpre as rounded, as its product does.  tanh.approx is off by 2^-11 at most, a quarter of the
+// largest bf16 rounding.
+//
 // The number of rows of each expert stays on the device: grids are sized by the most
 // tiles that the slots can fill, and the kernels read the real counts from the plan.
 // Every sum has a fixed order (no float atomics).
@@ -659,7 +671,8 @@ struct MoeUnit {
 // The unit that worker `w` of `n` takes in its round that starts at `base`.  The weight GEMMs' units cost as much as
 // their experts have rows; they stand in falling order, and every other round is dealt backwards, so that the workers'
 // sums come out nearly even.  (In the experts' order one pair of CTAs had up to 1.3 times the mean, 16 experts with
-// 1,800 to 7,900 rows, 768 x 1536: forward and backward 1107 us, in this one 1085.)
+// 1,800 to 7,900 rows, 768 x 1536: forward and backward 1111-1116 us in five long runs, in this one 1079-1090 in five
+// between them.)
 template <int MODE>
 __device__ __forceinline__ int unit_of(int base, int w, int n) {
   return base + (MODE == MOE_DW && (base / n & 1) ? n - 1 - w : w);
@@ -689,8 +702,8 @@ __device__ __forceinline__ MoeUnit moe_unit(const MoeGemmArgs& a, int u, int mt,
   return q;
 }
 
-// Two fp32 operations an instruction: the epilogues with an activation are bound by instruction issue (one
-// 32x32 chunk of dpre took 1,100 instructions a warp with scalar ones).
+// Two fp32 operations an instruction: in an epilogue with an activation a warp's arithmetic is most of a chunk's time
+// (a 32x32 chunk of dpre took 1,100 instructions with scalar ones; its GEMM 198 us, with these 179).
 __device__ __forceinline__ uint64_t f2(float a, float b) {
   uint64_t r;
   asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
@@ -1049,8 +1062,11 @@ __global__ void __maxnreg__(DTB_CORESIDENT_MAXNREG)
 //
 // Bound: at K 2048 by the tensor cores at the power limit (32768 rows x 2048 x 2048: 218 us a
 // product, 1.26 PFLOP/s, with an eighth of the tiles' rows padding; the dense pair GEMM of the
-// same size 190); at K 768 with an activation by the epilogue's issue slots and its two tensors
-// of rows x 1536 in DRAM (153 us forward, 179 backward; 112 us without them).
+// same size 190).  At K 768 the products with an activation take 153 us forward and 179 backward
+// (65536 rows x 1536) where one without takes 112.  No unit is full there (counters at 32768 rows,
+// forward / backward: tensor pipe 43 / 36%, issue 28 / 36%, DRAM 31 / 29%).  The likely bound, not
+// shown, is the chain in each epilogue warp: a chunk is read from TMEM, computed, packed and handed
+// to its store before the next one is read.  Twice the epilogue warps (96 registers) were no faster.
 __device__ __forceinline__ void tma_load_3d_pair(const CUtensorMap* map, void* dst, uint32_t leader_bar, int x, int y,
                                                  int z) {
   asm volatile(

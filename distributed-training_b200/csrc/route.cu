@@ -157,11 +157,11 @@ __device__ __forceinline__ void store_logits(T* p, int valid, bool vec, const fl
 // heads of its lanes' lists by xor-shuffles, all groups at once, and each of the k rounds
 // takes the largest head of the warp (redux) and pops it.
 //
-// Bound by the integer pipe (half rate: selects, compares, minima): per token about 28 V for
-// scores and keys, 5 V (V - 1) / 2 for the sort, 5 a group and 25 a round, 1050 instructions at
-// V = 8.  65536 tokens x 256 fp32 logits in 8 groups, 8 a token: 82 us (71 MB, 11 us at the copy
-// rate); unsorted values rescanned each round (route_fwd_wide_kernel, 7 V a round and 10 V a
-// group) took 194 us there.  That form serves V > 8, where the sort would cost more.
+// Bound by instruction issue, most of it integer work (scores, keys, the sort, the pops): 1055 instructions a
+// token at 256 experts in 8 groups, 8 a token (issue 71% of the active cycles, the half-rate integer pipe 54% of
+// all).  65536 such tokens, fp32: 82 us (71 MB, 11 us at the copy rate).  The experts of groups that are dropped
+// are sorted too, since that comes first.  Unsorted values rescanned each round (route_fwd_wide_kernel) took
+// 194 us there; that form serves V > 8, where the sort would cost more.
 template <typename T, int V>
 __global__ void __launch_bounds__(256) route_fwd_kernel(RouteArgs a) {
   extern __shared__ int s_load[];

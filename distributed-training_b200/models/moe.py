@@ -9,6 +9,8 @@ the mean and down for the others, by a fixed amount.
 
 ``MoEGPT`` is a GPT whose blocks use it.  Its parameters are separate tensors of one
 type: bf16 on a GPU runs the kernels, fp32 and fp64 the torch math on any device.
+Both serve one device: DDP, ZeroAdamW and Trainer need a model's flat buffers, which
+``MoEGPT`` does not have, and ``balance`` goes by the load of its own process.
 """
 from __future__ import annotations
 
