@@ -427,8 +427,11 @@ struct ClipRange {
 };
 
 static MemView mem_view(const at::Tensor& t) {
-  MemView v{reinterpret_cast<uintptr_t>(t.const_data_ptr()), (int)t.element_size(), t.sizes().vec(), t.strides().vec()};
-  for (long& s : v.stride) s *= v.elem;
+  MemView v{reinterpret_cast<uintptr_t>(t.const_data_ptr()), (int)t.element_size(), {}, {}};
+  for (int64_t k = 0; k < t.dim(); ++k) {
+    v.size.push_back(t.size(k));
+    v.stride.push_back(t.stride(k) * v.elem);
+  }
   return v;
 }
 static MemView mem_view(const ClipRange& r) {
@@ -448,16 +451,24 @@ static ClipRange clip_range(const at::Tensor& t, bool dense, int i, bool out) {
 static void check_ranges(std::vector<ClipRange>& r) {
   const auto less = [](const ClipRange& a, const ClipRange& b) { return a.lo < b.lo; };
   if (!std::is_sorted(r.begin(), r.end(), less)) std::sort(r.begin(), r.end(), less);
-  std::vector<const ClipRange*> open;  // those that reach past the start of the present one
+  uintptr_t hi = 0;
+  bool meet = false;
   for (const auto& x : r) {
-    open.erase(std::remove_if(open.begin(), open.end(), [&](const ClipRange* y) { return y->hi <= x.lo; }), open.end());
-    for (const ClipRange* y : open) {
+    meet |= x.lo < hi;
+    hi = std::max(hi, x.hi);
+  }
+  if (!meet) return;
+  std::vector<std::pair<const ClipRange*, MemView>> open;  // those that reach past the start of the present one
+  for (const auto& x : r) {
+    open.erase(std::remove_if(open.begin(), open.end(), [&](const auto& o) { return o.first->hi <= x.lo; }), open.end());
+    MemView v = mem_view(x);
+    for (const auto& [y, w] : open) {
       if (!x.out && !y->out) continue;
-      const bool apart = (x.t || y->t) && !views_overlap(mem_view(x), mem_view(*y));
+      const bool apart = (x.t || y->t) && !views_overlap(v, w);
       TORCH_CHECK(apart || x.i == y->i, "clip_grads: tensors ", y->i, " and ", x.i, " overlap in memory");
       TORCH_CHECK(apart, "clip_grads: output ", x.i, " overlaps its gradient in memory without being it");
     }
-    open.push_back(&x);
+    open.emplace_back(&x, std::move(v));
   }
 }
 

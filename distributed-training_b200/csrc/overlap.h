@@ -9,27 +9,31 @@
 // the smaller ones, so at most three values a term are tried.
 #pragma once
 
+#include <c10/util/SmallVector.h>
+
 #include <algorithm>
 #include <cstdint>
 #include <numeric>
-#include <vector>
+#include <utility>
 
 namespace dtb {
 
 struct MemView {
   uintptr_t base;
   int elem;  // bytes of an element
-  std::vector<long> size, stride;  // stride in bytes
+  c10::SmallVector<long, 6> size, stride;  // stride in bytes
 };
 
 struct OverlapTerm {
   long c, lo, hi;  // c x with lo <= x <= hi, c > 0
 };
 
+using OverlapTerms = c10::SmallVector<OverlapTerm, 13>;
+
 // Whether sum c x = d has a solution.  Gives up after `budget` steps, and then says yes.
 class BoundedSum {
  public:
-  explicit BoundedSum(std::vector<OverlapTerm> terms) : t_(std::move(terms)) {
+  explicit BoundedSum(OverlapTerms terms) : t_(std::move(terms)) {
     std::sort(t_.begin(), t_.end(), [](const OverlapTerm& a, const OverlapTerm& b) { return a.c > b.c; });
     size_t m = 0;  // terms of one coefficient are one term
     for (const auto& x : t_) {
@@ -66,13 +70,13 @@ class BoundedSum {
       if (search(i + 1, d - t.c * x)) return true;
     return false;
   }
-  std::vector<OverlapTerm> t_;
-  std::vector<long> lo_, hi_, div_;  // of the terms from i on: least and greatest sum, common divisor
+  OverlapTerms t_;
+  c10::SmallVector<long, 14> lo_, hi_, div_;  // of the terms from i on: least and greatest sum, common divisor
   long budget_ = 0;
 };
 
 inline bool views_overlap(const MemView& a, const MemView& b) {
-  std::vector<OverlapTerm> t;
+  OverlapTerms t;
   for (size_t k = 0; k < a.size.size(); ++k)
     if (a.size[k] > 1 && a.stride[k]) t.push_back({a.stride[k], 0, a.size[k] - 1});
   for (size_t k = 0; k < b.size.size(); ++k)
@@ -82,7 +86,7 @@ inline bool views_overlap(const MemView& a, const MemView& b) {
 }
 
 inline bool view_overlaps_itself(const MemView& a) {
-  std::vector<std::pair<long, long>> d;  // stride, size
+  c10::SmallVector<std::pair<long, long>, 6> d;  // stride, size
   for (size_t k = 0; k < a.size.size(); ++k)
     if (a.size[k] > 1) d.push_back({a.stride[k], a.size[k]});
   std::sort(d.begin(), d.end());
@@ -96,7 +100,7 @@ inline bool view_overlaps_itself(const MemView& a) {
   // two index vectors of one address: they differ first in dimension k, by x >= 1
   for (size_t k = 0; k < d.size(); ++k) {
     if (d[k].first == 0) return true;
-    std::vector<OverlapTerm> t{{d[k].first, 1, d[k].second - 1}, {1, 1 - a.elem, a.elem - 1}};
+    OverlapTerms t{{d[k].first, 1, d[k].second - 1}, {1, 1 - a.elem, a.elem - 1}};
     for (size_t j = k + 1; j < d.size(); ++j) t.push_back({d[j].first, 1 - d[j].second, d[j].second - 1});
     if (BoundedSum(std::move(t)).reaches(0)) return true;
   }
