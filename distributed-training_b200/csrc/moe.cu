@@ -767,8 +767,8 @@ __device__ __forceinline__ void slab_get_bf16(const uint8_t* slab, int lane, flo
 
 // What a role still has in flight when it leaves its loop, also by a wait that ran out: loads that would land in, and
 // products that would read from and signal to, a CTA that is gone.  Both wait (mbar_wait's limit; the CTA's abort flag
-// does not shorten it) until that is done.  `stage` and `phase`: where the ring's next round goes, so a stage before
-// it was last used in this round, the others in the round before (of which a fresh barrier counts as complete).
+// does not shorten it) until that is done.  `stage` and `phase`: where the ring goes next, so a stage before it was
+// last used in this pass over the ring, the others in the pass before (which a fresh barrier counts as complete).
 template <int STAGES>
 __device__ __forceinline__ void finish_loads(uint64_t* full_bar, int stage, uint32_t phase) {
   volatile int never = 0;
